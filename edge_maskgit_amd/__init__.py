@@ -44,6 +44,8 @@ MGH_SYMBOLS = [
     "mgh_conv2d_i8_pack_weights", "mgh_conv2d_i8",
     "mgh_packed_weight_bytes_dq", "mgh_pack_weights_dq", "mgh_gemm_dq", "mgh_gemm_dq_f32in",
     "mgh_gemm_dq_y16", "mgh_gemm_dq_ln", "mgh_dequant_weights_f32",
+    "mgh_attn_masked", "mgh_kv8_code_bytes", "mgh_kv8_scale_bytes", "mgh_kv8_tail_bytes", "mgh_kv8_append",
+    "mgh_kv8_advance", "mgh_kv8_attn", "mgh_kv8_read", "mgh_logits_process",
 ]
 
 _lib = None
@@ -141,6 +143,19 @@ def lib():
         L.mgh_conv2d_i8.argtypes = [P, P, I, I, I, I, P, I, I, I, I, I, P, P, P]
         L.mgh_group_norm.argtypes = [P, P, I, I, I, I, I, ctypes.c_float, P, P, P]
         L.mgh_upscale.argtypes = [P, P, I, I, I, I, I, P]
+        F = ctypes.c_float
+        L.mgh_attn_masked.argtypes = [P, P, P, P, I, P, P, I, I, I, I, I, I, F, P, P, P, P]
+        L.mgh_kv8_code_bytes.argtypes = [I64, I, I]
+        L.mgh_kv8_code_bytes.restype = SZ
+        L.mgh_kv8_scale_bytes.argtypes = [I64, I]
+        L.mgh_kv8_scale_bytes.restype = SZ
+        L.mgh_kv8_tail_bytes.argtypes = [I, I, I]
+        L.mgh_kv8_tail_bytes.restype = SZ
+        L.mgh_kv8_append.argtypes = [P, P, P, P, I, P, I, P, P]
+        L.mgh_kv8_advance.argtypes = [P, P, P, I, I]
+        L.mgh_kv8_attn.argtypes = [P, P, P, I, P, I, P, P, I, F, F, P, P, P, P]
+        L.mgh_kv8_read.argtypes = [P, P, P, I, P, P, P, P, P]
+        L.mgh_logits_process.argtypes = [P, P, I, I64, I, I, P, P, I64]
         L.mgh_graph_begin.argtypes = [P]
         L.mgh_graph_end.argtypes = [P, ctypes.POINTER(P)]
         L.mgh_graph_launch.argtypes = [P, P]
@@ -191,6 +206,51 @@ class DeviceBuffer:
     @property
     def p(self):
         return ctypes.c_void_p(self.ptr)
+
+
+class _AttnOpts(ctypes.Structure):
+    _fields_ = [("cap", ctypes.c_float), ("causal", ctypes.c_int), ("d_slopes", ctypes.c_void_p),
+                ("d_prefix", ctypes.c_void_p), ("d_docs", ctypes.c_void_p), ("doc_stride", ctypes.c_int64)]
+
+
+class _LogitsOpts(ctypes.Structure):
+    _fields_ = [("d_hist", ctypes.c_void_p), ("hist_stride", ctypes.c_int64), ("max_hist", ctypes.c_int),
+                ("d_hist_len", ctypes.c_void_p), ("d_rep", ctypes.c_void_p), ("d_freq", ctypes.c_void_p),
+                ("d_pres", ctypes.c_void_p), ("d_bias", ctypes.c_void_p), ("bias_stride", ctypes.c_int64),
+                ("d_allowed", ctypes.c_void_p), ("allowed_stride", ctypes.c_int64)]
+
+
+def _addr(b):
+    """address of a DeviceBuffer, an int or None, as a ctypes structure's pointer field takes it"""
+    return b.ptr if isinstance(b, DeviceBuffer) else b
+
+
+class Kv8(ctypes.Structure):
+    """mgh_kv8: a key / value cache in 8 bits over buffers that the caller owns (include/mgh.h has their
+    layout and sizes). table: B rows of max_blocks page numbers (int32), table_stride apart."""
+
+    _fields_ = [("d_k", ctypes.c_void_p), ("d_v", ctypes.c_void_p), ("d_scales", ctypes.c_void_p),
+                ("d_k_tail", ctypes.c_void_p), ("d_v_tail", ctypes.c_void_p), ("d_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("pages", ctypes.c_int64), ("max_blocks", ctypes.c_int),
+                ("Hkv", ctypes.c_int), ("D", ctypes.c_int), ("B", ctypes.c_int)]
+
+    def __init__(self, k, v, scales, k_tail, v_tail, table, max_blocks, pages, Hkv, D, B, table_stride=None):
+        super().__init__(*map(_addr, (k, v, scales, k_tail, v_tail, table)),
+                         max_blocks if table_stride is None else table_stride, pages, max_blocks, Hkv, D, B)
+
+
+def kv8_code_bytes(pages: int, Hkv: int, D: int) -> int:
+    """bytes of a Kv8's k, and of its v"""
+    return int(lib().mgh_kv8_code_bytes(pages, Hkv, D))
+
+
+def kv8_scale_bytes(pages: int, Hkv: int) -> int:
+    return int(lib().mgh_kv8_scale_bytes(pages, Hkv))
+
+
+def kv8_tail_bytes(B: int, Hkv: int, D: int) -> int:
+    """bytes of a Kv8's k_tail, and of its v_tail"""
+    return int(lib().mgh_kv8_tail_bytes(B, Hkv, D))
 
 
 class Context:
@@ -479,6 +539,53 @@ class Context:
 
     def upscale(self, x, W, H, C, N, factor, y):
         self._check(lib().mgh_upscale(self.h, self._ptr(x), W, H, C, N, factor, self._ptr(y)))
+
+    # ---- generating token by token: masked attention, the 8-bit cache, logits ----
+    def attn_masked(self, q, k, v, q_strides, kv_strides, D, Sq, Sk, H, Hkv, B, scale, o=None, o16=None, o_strides=None,
+                    in16=True, cap=0.0, slopes=None, causal=False, prefix=None, docs=None, doc_stride=0):
+        """Attention of {D, Sq, H, B} queries at positions Sk - Sq + i over {D, Sk, Hkv, B} keys (fp16, or
+        fp32 with in16=False); exactly one of o (fp32) and o16 (fp16) is given."""
+        P = self._ptr
+        op = _AttnOpts(cap, bool(causal), _addr(slopes), _addr(prefix), _addr(docs), doc_stride)
+        ost = None if o_strides is None else (ctypes.c_int64 * 4)(*o_strides)
+        self._check(lib().mgh_attn_masked(self.h, P(q), P(k), P(v), int(in16), (ctypes.c_int64 * 4)(*q_strides),
+                                          (ctypes.c_int64 * 4)(*kv_strides), D, Sq, Sk, H, Hkv, B, scale,
+                                          ctypes.byref(op), P(o), P(o16), ost))
+
+    def kv8_append(self, cache, k, v, strides, S, lens, new=None, in16=True):
+        """The keys and values of up to S new tokens per sequence ({D, S, Hkv, B} views) into the cache at
+        positions lens[b] + i."""
+        P = self._ptr
+        self._check(lib().mgh_kv8_append(self.h, ctypes.byref(cache), P(k), P(v), int(in16),
+                                         (ctypes.c_int64 * 4)(*strides), S, P(lens), P(new)))
+
+    def kv8_advance(self, lens, new, B, S):
+        """lens[b] += new[b] (S where new is None)"""
+        self._check(lib().mgh_kv8_advance(self.h, self._ptr(lens), self._ptr(new), B, S))
+
+    def kv8_attn(self, cache, q, q_strides, S, lens, new, H, scale, o=None, o16=None, o_strides=None, in16=True, cap=0.0,
+                 slopes=None):
+        """Attention of up to S new tokens per sequence ({D, S, H, B} queries at positions lens[b] + i) over
+        the cache, which already holds them; exactly one of o and o16 is given."""
+        P = self._ptr
+        ost = None if o_strides is None else (ctypes.c_int64 * 4)(*o_strides)
+        self._check(lib().mgh_kv8_attn(self.h, ctypes.byref(cache), P(q), int(in16), (ctypes.c_int64 * 4)(*q_strides), S,
+                                       P(lens), P(new), H, scale, cap, P(slopes), P(o), P(o16), ost))
+
+    def kv8_read(self, cache, first, n, lens, k=None, v=None, k16=None, v16=None):
+        """The values at positions first[b] + i (first None: i), i < n, of sequences of lens[b] tokens, to
+        [B][Hkv][n][D] in k and v (fp32) or k16 and v16 (fp16)."""
+        P = self._ptr
+        self._check(lib().mgh_kv8_read(self.h, ctypes.byref(cache), P(first), n, P(lens), P(k), P(v), P(k16), P(v16)))
+
+    def logits_process(self, x, rows, V, y, f16=False, x_stride=None, y_stride=None, hist=None, hist_stride=None,
+                       max_hist=0, hist_len=None, rep=None, freq=None, pres=None, bias=None, bias_stride=0, allowed=None,
+                       allowed_stride=0):
+        """Penalties for the tokens of a history, a bias and a bit mask of allowed tokens on rows of V logits."""
+        op = _LogitsOpts(_addr(hist), max_hist if hist_stride is None else hist_stride, max_hist, _addr(hist_len),
+                         _addr(rep), _addr(freq), _addr(pres), _addr(bias), bias_stride, _addr(allowed), allowed_stride)
+        self._check(lib().mgh_logits_process(self.h, self._ptr(x), int(f16), V if x_stride is None else x_stride, rows, V,
+                                             ctypes.byref(op), self._ptr(y), V if y_stride is None else y_stride))
 
     # ---- graphs ----
     def graph_begin(self):

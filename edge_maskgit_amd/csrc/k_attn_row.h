@@ -1,0 +1,71 @@
+// k_attn_row.h — one query row of the masked and the 8-bit-cache attention, by one wave.
+//
+// s_j = scale q . k_j; capped: s <- cap tanh(s / cap); sloped: s <- s - slope |p - j|; over the keys
+// that the row sees, o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with a running m (fp32 throughout).
+// A masked key is not read, and a key whose weight is zero adds nothing whatever its value holds, so
+// neither infinities nor NaN there reach the row. The tiled kernels, whose matrix products multiply a
+// masked key's value by a zero weight, take this path for the rows that came out not finite.
+#pragma once
+#include "mgh_common.h"
+#include "mgh_kernels.h"
+
+namespace mgh {
+
+// The score in log2 units from q . k. tanh(x) = 1 - 2 / (exp(2x) + 1): exp2 of an overflowing argument
+// is inf (its reciprocal 0: +cap), of an underflowing one 0 (-cap). The hardware's exp2 and reciprocal
+// are 1 ulp off; near zero the difference costs an absolute 1.2e-7 cap.
+__device__ __forceinline__ float cap_score(float s, const ScoreMod& m) {
+    const float e = __builtin_amdgcn_exp2f(s * m.cap_in);
+    return fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * m.cap2, m.cap2);
+}
+
+// A row's partial result: weights relative to 2^m
+struct RowState {
+    float m, l;
+    float o[2];        // features lane and lane + 64
+};
+
+// keys [lo, hi) of one row. qs: the row's q in LDS (fp32, D values), pl: 64 floats of LDS; both this
+// wave's own. src.seen(j), src.dot(j, qs), src.value(j, d).
+template <class Src>
+__device__ __forceinline__ RowState attn_row(const Src& src, const ScoreMod& mod, float slope2, int64_t p, int64_t lo,
+                                             int64_t hi, int D, const float* qs, float* pl, int lane) {
+    RowState st{-INFINITY, 0.f, {0.f, 0.f}};
+    for (int64_t j0 = lo; j0 < hi; j0 += 64) {
+        const int64_t j = j0 + lane;
+        float s = -INFINITY;
+        if (j < hi && src.seen(j)) {
+            const float x = src.dot(j, qs);
+            s = mod.cap2 != 0.f ? cap_score(x, mod) : x * mod.scale2;
+            s -= slope2 * fabsf((float)(p - j));
+        }
+        float mx = s;
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
+        if (__all(s == -INFINITY)) continue;
+        const float m = fmaxf(st.m, mx);
+        const float al = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+        const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - m);
+        float sum = w;
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
+        st.l = st.l * al + sum;
+        st.m = m;
+        st.o[0] *= al;
+        st.o[1] *= al;
+        pl[lane] = w;
+        __builtin_amdgcn_wave_barrier();
+        const int n = (int)(hi - j0 < 64 ? hi - j0 : 64);
+        for (int k = 0; k < n; k++) {
+            const float pk = pl[k];
+            if (pk == 0.f) continue;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (lane + 64 * i < D) st.o[i] = fmaf(pk, src.value(j0 + k, lane + 64 * i), st.o[i]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    return st;
+}
+
+}  // namespace mgh

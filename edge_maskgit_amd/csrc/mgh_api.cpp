@@ -1231,3 +1231,209 @@ int mgh_debug_block_dots(mgh_ctx* c, int wtype, const void* w, int N, int K, con
 }
 
 }  // extern "C"
+
+namespace {
+
+// what both attentions ask of their scores and outputs
+int check_scores(mgh_ctx* c, const char* fn, int D, int H, int Hkv, float scale, float cap, const float* o, const void* o16) {
+    const std::string f(fn);
+    if (H <= 0 || Hkv <= 0 || H % Hkv) return fail(c, MGH_ERR_ARG, f + ": need H and Hkv > 0 and H % Hkv == 0");
+    if (D <= 0 || D % 16 || D > 128) return fail(c, MGH_ERR_UNSUPPORTED, f + ": D must be a multiple of 16 up to 128");
+    if (!(scale - scale == 0.f)) return fail(c, MGH_ERR_ARG, f + ": scale must be finite");
+    if (!(cap >= 0.f) || cap - cap != 0.f) return fail(c, MGH_ERR_ARG, f + ": cap must be finite and >= 0");
+    if ((o != nullptr) == (o16 != nullptr)) return fail(c, MGH_ERR_ARG, f + ": exactly one of d_o and d_o16 is needed");
+    return MGH_OK;
+}
+
+bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+int check_kv8(mgh_ctx* c, const char* fn, const mgh_kv8* kv, mgh::Kv8* out) {
+    const std::string f(fn);
+    if (!kv) return fail(c, MGH_ERR_ARG, f + ": null cache");
+    if (kv->Hkv <= 0 || kv->D <= 0 || kv->B < 0 || kv->pages < 0 || kv->max_blocks < 0 || kv->table_stride < 0)
+        return fail(c, MGH_ERR_ARG, f + ": the cache needs Hkv, D > 0 and no negative size");
+    if (kv->D % 16 || kv->D > 128) return fail(c, MGH_ERR_UNSUPPORTED, f + ": D must be a multiple of 16 up to 128");
+    if (kv->table_stride < kv->max_blocks && kv->B > 1)
+        return fail(c, MGH_ERR_ARG, f + ": table_stride must be at least max_blocks");
+    if (kv->Hkv > 65535 || kv->B > 65535 || kv->max_blocks > (1 << 24) || kv->pages > INT32_MAX)
+        return fail(c, MGH_ERR_UNSUPPORTED, f + ": at most 65535 heads and sequences, 2^24 blocks each, 2^31 - 1 pages");
+    if (kv->B && (!kv->d_k_tail || !kv->d_v_tail)) return fail(c, MGH_ERR_ARG, f + ": null pointer");
+    if (kv->B && ((kv->pages && (!kv->d_k || !kv->d_v || !kv->d_scales)) || (kv->max_blocks && !kv->d_table)))
+        return fail(c, MGH_ERR_ARG, f + ": null pointer");
+    if (!aligned16(kv->d_k) || !aligned16(kv->d_v) || !aligned16(kv->d_k_tail) || !aligned16(kv->d_v_tail) ||
+        !aligned_to(kv->d_scales, 8) || !aligned_to(kv->d_table, 4))
+        return fail(c, MGH_ERR_ARG, f + ": codes and tails must be 16-byte, scales 8-byte and the table 4-byte aligned");
+    *out = mgh::Kv8{(uint8_t*)kv->d_k, (uint8_t*)kv->d_v, kv->d_scales, (_Float16*)kv->d_k_tail, (_Float16*)kv->d_v_tail,
+                    kv->d_table, kv->table_stride, kv->pages, kv->max_blocks, kv->Hkv, kv->D, kv->B};
+    return MGH_OK;
+}
+
+int check_step(mgh_ctx* c, const char* fn, int S, const int32_t* lens, const int32_t* fresh) {
+    const std::string f(fn);
+    if (S < 0) return fail(c, MGH_ERR_ARG, f + ": negative number of tokens");
+    if (S > (1 << 29)) return fail(c, MGH_ERR_UNSUPPORTED, f + ": at most 2^29 tokens");
+    if (!lens) return fail(c, MGH_ERR_ARG, f + ": null lengths");
+    if (!aligned_to(lens, 4) || !aligned_to(fresh, 4)) return fail(c, MGH_ERR_ARG, f + ": lengths must be 4-byte aligned");
+    return MGH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mgh_attn_masked(mgh_ctx* c, const void* q, const void* k, const void* v, int in_f16, const int64_t qst[4],
+                    const int64_t kvst[4], int D, int Sq, int Sk, int H, int Hkv, int B, float scale,
+                    const mgh_attn_opts* opts, float* o, void* o16, const int64_t ost[4]) {
+    if (!c) return MGH_ERR_ARG;
+    const mgh_attn_opts none{};
+    const mgh_attn_opts& op = opts ? *opts : none;
+    if (int r = check_scores(c, "attn_masked", D, H, Hkv, scale, op.cap, o, o16)) return r;
+    if (Sq < 0 || Sk < 0 || B < 0) return fail(c, MGH_ERR_ARG, "attn_masked: negative shape");
+    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "attn_masked: in_f16 must be 0 or 1");
+    if (op.causal != 0 && op.causal != 1) return fail(c, MGH_ERR_ARG, "attn_masked: causal must be 0 or 1");
+    if (op.d_prefix && !op.causal) return fail(c, MGH_ERR_ARG, "attn_masked: a prefix needs causal");
+    if (op.d_docs && (op.doc_stride < 0 || (B > 1 && op.doc_stride && op.doc_stride < Sk)))
+        return fail(c, MGH_ERR_ARG, "attn_masked: doc_stride must be 0 or at least Sk");
+    if (Sq == 0 || B == 0) return MGH_OK;
+    if (!q || !qst || (Sk && (!k || !v || !kvst))) return fail(c, MGH_ERR_ARG, "attn_masked: null pointer");
+    const size_t eb = in_f16 ? 2 : 4;
+    if (!aligned_to(q, eb) || !aligned_to(k, eb) || !aligned_to(v, eb) || !aligned_to(o, 4) || !aligned_to(o16, 2) ||
+        !aligned_to(op.d_slopes, 4) || !aligned_to(op.d_prefix, 4) || !aligned_to(op.d_docs, 4))
+        return fail(c, MGH_ERR_ARG, "attn_masked: pointers must be aligned to their elements");
+    if (H > 65535 || B > 65535 || Sk > (1 << 24) || (int64_t)Sq * (H / Hkv) > (1 << 24))
+        return fail(c, MGH_ERR_UNSUPPORTED, "attn_masked: at most 65535 heads and sequences, 2^24 keys and rows of a key head");
+    mgh::MaskedAttnArgs a{};
+    a.q = q; a.k = k; a.v = v; a.o = o; a.o16 = (_Float16*)o16;
+    for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.kvst[i] = kvst ? kvst[i] : 0;
+    const int64_t packed[4] = {1, D, (int64_t)D * Sq, (int64_t)D * Sq * H};
+    for (int i = 0; i < 4; i++) a.ost[i] = ost ? ost[i] : packed[i];
+    a.D = D; a.Sq = Sq; a.Sk = Sk; a.H = H; a.Hkv = Hkv; a.B = B;
+    a.in16 = in_f16 != 0; a.causal = op.causal != 0;
+    a.mod = mgh::score_mod(scale, op.cap);
+    a.slopes = op.d_slopes; a.prefix = op.d_prefix; a.docs = op.d_docs; a.doc_stride = op.doc_stride;
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_attn_masked(a, c->stream), "k_attn_masked");
+    return MGH_OK;
+}
+
+size_t mgh_kv8_code_bytes(int64_t pages, int Hkv, int D) {
+    return pages > 0 && Hkv > 0 && D > 0 ? (size_t)pages * Hkv * D * mgh::kKvBlock : 0;
+}
+
+size_t mgh_kv8_scale_bytes(int64_t pages, int Hkv) {
+    return pages > 0 && Hkv > 0 ? (size_t)pages * Hkv * 2 * sizeof(float) : 0;
+}
+
+size_t mgh_kv8_tail_bytes(int B, int Hkv, int D) {
+    return B > 0 && Hkv > 0 && D > 0 ? (size_t)B * Hkv * D * mgh::kKvRing * 2 : 0;
+}
+
+int mgh_kv8_append(mgh_ctx* c, const mgh_kv8* kv, const void* k, const void* v, int in_f16, const int64_t st[4], int S,
+                   const int32_t* lens, const int32_t* fresh) {
+    if (!c) return MGH_ERR_ARG;
+    mgh::Kv8AppendArgs a{};
+    if (int r = check_kv8(c, "kv8_append", kv, &a.c)) return r;
+    if (kv->B == 0 || S == 0) return MGH_OK;
+    if (int r = check_step(c, "kv8_append", S, lens, fresh)) return r;
+    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "kv8_append: in_f16 must be 0 or 1");
+    if (!k || !v || !st) return fail(c, MGH_ERR_ARG, "kv8_append: null pointer");
+    if (!aligned_to(k, in_f16 ? 2 : 4) || !aligned_to(v, in_f16 ? 2 : 4))
+        return fail(c, MGH_ERR_ARG, "kv8_append: pointers must be aligned to their elements");
+    a.k = k; a.v = v; a.S = S; a.lens = lens; a.fresh = fresh; a.in16 = in_f16 != 0;
+    for (int i = 0; i < 4; i++) a.st[i] = st[i];
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_kv8_append(a, c->stream), "k_kv8_append");
+    return MGH_OK;
+}
+
+int mgh_kv8_advance(mgh_ctx* c, int32_t* lens, const int32_t* fresh, int B, int S) {
+    if (!c) return MGH_ERR_ARG;
+    if (B < 0) return fail(c, MGH_ERR_ARG, "kv8_advance: negative number of sequences");
+    if (B == 0) return MGH_OK;
+    if (int r = check_step(c, "kv8_advance", S, lens, fresh)) return r;
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_kv8_advance(lens, fresh, B, S, c->stream), "k_kv8_advance");
+    return MGH_OK;
+}
+
+int mgh_kv8_attn(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const int64_t qst[4], int S,
+                 const int32_t* lens, const int32_t* fresh, int H, float scale, float cap, const float* slopes, float* o,
+                 void* o16, const int64_t ost[4]) {
+    if (!c) return MGH_ERR_ARG;
+    mgh::Kv8AttnArgs a{};
+    if (int r = check_kv8(c, "kv8_attn", kv, &a.c)) return r;
+    if (int r = check_scores(c, "kv8_attn", kv->D, H, kv->Hkv, scale, cap, o, o16)) return r;
+    if (kv->B == 0 || S == 0) return MGH_OK;
+    if (int r = check_step(c, "kv8_attn", S, lens, fresh)) return r;
+    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "kv8_attn: in_f16 must be 0 or 1");
+    if (!q || !qst) return fail(c, MGH_ERR_ARG, "kv8_attn: null pointer");
+    if (!aligned_to(q, in_f16 ? 2 : 4) || !aligned_to(o, 4) || !aligned_to(o16, 2) || !aligned_to(slopes, 4))
+        return fail(c, MGH_ERR_ARG, "kv8_attn: pointers must be aligned to their elements");
+    if (H > 65535 || (int64_t)S * (H / kv->Hkv) > (1 << 24))
+        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn: at most 65535 heads and 2^24 rows of a key head");
+    a.q = q; a.o = o; a.o16 = (_Float16*)o16; a.S = S; a.H = H; a.in16 = in_f16 != 0;
+    a.lens = lens; a.fresh = fresh; a.slopes = slopes;
+    a.mod = mgh::score_mod(scale, cap);
+    const int64_t packed[4] = {1, kv->D, (int64_t)kv->D * S, (int64_t)kv->D * S * H};
+    for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.ost[i] = ost ? ost[i] : packed[i];
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_kv8_attn(a, c->stream), "k_kv8_attn");
+    return MGH_OK;
+}
+
+int mgh_kv8_read(mgh_ctx* c, const mgh_kv8* kv, const int32_t* first, int n, const int32_t* lens, float* k, float* v,
+                 void* k16, void* v16) {
+    if (!c) return MGH_ERR_ARG;
+    mgh::Kv8ReadArgs a{};
+    if (int r = check_kv8(c, "kv8_read", kv, &a.c)) return r;
+    if (kv->B == 0 || n == 0) return MGH_OK;
+    if (int r = check_step(c, "kv8_read", n, lens, first)) return r;
+    if (!((k && v && !k16 && !v16) || (!k && !v && k16 && v16)))
+        return fail(c, MGH_ERR_ARG, "kv8_read: either d_k and d_v or d_k16 and d_v16 are needed");
+    if (!aligned_to(k, 4) || !aligned_to(v, 4) || !aligned_to(k16, 2) || !aligned_to(v16, 2))
+        return fail(c, MGH_ERR_ARG, "kv8_read: pointers must be aligned to their elements");
+    a.first = first; a.lens = lens; a.n = n;
+    a.k = k; a.v = v; a.k16 = (_Float16*)k16; a.v16 = (_Float16*)v16;
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_kv8_read(a, c->stream), "k_kv8_read");
+    return MGH_OK;
+}
+
+int mgh_logits_process(mgh_ctx* c, const void* x, int f16, int64_t xs, int rows, int V, const mgh_logits_opts* opts, void* y,
+                       int64_t ys) {
+    if (!c) return MGH_ERR_ARG;
+    const mgh_logits_opts none{};
+    const mgh_logits_opts& op = opts ? *opts : none;
+    if (rows < 0 || V < 0) return fail(c, MGH_ERR_ARG, "logits_process: negative shape");
+    if (f16 != 0 && f16 != 1) return fail(c, MGH_ERR_ARG, "logits_process: f16 must be 0 or 1");
+    if (op.max_hist < 0 || op.hist_stride < 0 || op.bias_stride < 0 || op.allowed_stride < 0)
+        return fail(c, MGH_ERR_ARG, "logits_process: negative history, bias or mask size");
+    if (rows == 0 || V == 0) return MGH_OK;
+    if (V > (1 << 30) || (int64_t)rows * ((V + 4095) / 4096) >= (1 << 24))
+        return fail(c, MGH_ERR_UNSUPPORTED, "logits_process: shape too large");
+    if (!x || !y) return fail(c, MGH_ERR_ARG, "logits_process: null pointer");
+    if (rows > 1 && (xs < V || ys < V)) return fail(c, MGH_ERR_ARG, "logits_process: rows must be at least V apart");
+    if (x == y && rows > 1 && xs != ys) return fail(c, MGH_ERR_ARG, "logits_process: in place needs equal strides");
+    if (op.d_hist && rows > 1 && op.hist_stride && op.hist_stride < op.max_hist)
+        return fail(c, MGH_ERR_ARG, "logits_process: hist_stride must be 0 or at least max_hist");
+    if (op.d_bias && rows > 1 && op.bias_stride && op.bias_stride < V)
+        return fail(c, MGH_ERR_ARG, "logits_process: bias_stride must be 0 or at least V");
+    if (op.d_allowed && rows > 1 && op.allowed_stride && op.allowed_stride < ((int64_t)V + 31) / 32)
+        return fail(c, MGH_ERR_ARG, "logits_process: allowed_stride must be 0 or at least V / 32 rounded up");
+    const size_t eb = f16 ? 2 : 4;
+    const void* words[] = {op.d_hist, op.d_hist_len, op.d_rep, op.d_freq, op.d_pres, op.d_bias, op.d_allowed};
+    bool ok = aligned_to(x, eb) && aligned_to(y, eb);
+    for (const void* p : words) ok = ok && aligned_to(p, 4);
+    if (!ok) return fail(c, MGH_ERR_ARG, "logits_process: pointers must be aligned to their elements");
+    mgh::LogitsArgs a{};
+    a.x = x; a.y = y; a.x_stride = xs; a.y_stride = ys; a.rows = rows; a.V = V; a.f16 = f16 != 0;
+    if (op.d_hist && op.max_hist) a.hist = op.d_hist;
+    a.hist_len = op.d_hist_len; a.hist_stride = op.hist_stride; a.max_hist = op.max_hist;
+    a.rep = op.d_rep; a.freq = op.d_freq; a.pres = op.d_pres;
+    a.bias = op.d_bias; a.bias_stride = op.bias_stride; a.allowed = op.d_allowed; a.allowed_stride = op.allowed_stride;
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_logits_process(a, c->stream), "k_logits");
+    return MGH_OK;
+}
+
+}  // extern "C"

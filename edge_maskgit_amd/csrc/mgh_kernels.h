@@ -277,6 +277,105 @@ hipError_t launch_group_norm(const float* x, int64_t W, int64_t H, int C, int N,
                              const float* gamma, const float* beta, float* y, void* ws, hipStream_t s);
 hipError_t launch_upscale(const float* x, int IW, int IH, int64_t CN, int f, float* y, hipStream_t s);
 
+// Attention under masks and over the 8-bit cache (k_attn_masked.hip, k_kv8.hip). Scores become log2
+// units: s scale2, or cap2 tanh(s scale / cap) = cap2 (1 - 2 / (exp2(s cap_in) + 1)).
+constexpr float kLog2e = 1.4426950408889634f;
+struct ScoreMod {
+    float scale2;          // scale log2(e)
+    float cap_in;          // 2 scale log2(e) / cap
+    float cap2;            // cap log2(e); 0: not capped
+};
+inline ScoreMod score_mod(float scale, float cap) {
+    return {scale * kLog2e, cap > 0.f ? (float)(2.0 * scale * 1.4426950408889634 / cap) : 0.f, cap > 0.f ? cap * kLog2e : 0.f};
+}
+struct MaskedAttnArgs {
+    const void* q;         // fp16 (in16) or fp32 views, element strides for d, s, h, b
+    const void* k;
+    const void* v;
+    float* o;              // one of o and o16
+    _Float16* o16;
+    int64_t qst[4], kvst[4], ost[4];
+    int D, Sq, Sk, H, Hkv, B;
+    bool in16, causal;
+    ScoreMod mod;
+    const float* slopes;   // [H] or null
+    const int32_t* prefix; // [B] or null
+    const int32_t* docs;   // [B] rows of Sk ids, doc_stride apart, or null
+    int64_t doc_stride;
+};
+hipError_t launch_attn_masked(const MaskedAttnArgs& a, hipStream_t s);
+
+// The 8-bit cache (include/mgh.h has the layout)
+constexpr int kKvBlock = 32, kKvRing = 64;
+struct Kv8 {
+    uint8_t* k;            // [pages][Hkv][32][D] codes + 128
+    uint8_t* v;            // [pages][Hkv][D / 2][4][2][8]
+    float* scales;         // [pages][Hkv][2]
+    _Float16* k_tail;      // [B][Hkv][64][D]
+    _Float16* v_tail;      // [B][Hkv][D][64]
+    const int32_t* table;  // [B] rows of max_blocks page numbers, table_stride apart
+    int64_t table_stride, pages;
+    int max_blocks, Hkv, D, B;
+};
+struct Kv8AppendArgs {
+    Kv8 c;
+    const void* k;
+    const void* v;
+    int64_t st[4];         // d, token, head, sequence
+    const int32_t* lens;
+    const int32_t* fresh;  // [B] new tokens, or null: S
+    int S;
+    bool in16;
+};
+hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t s);
+struct Kv8ReadArgs {
+    Kv8 c;
+    const int32_t* first;  // [B] or null: 0
+    const int32_t* lens;
+    int n;
+    float* k;              // [B][Hkv][n][D], or fp16 in k16 / v16
+    float* v;
+    _Float16* k16;
+    _Float16* v16;
+};
+hipError_t launch_kv8_read(const Kv8ReadArgs& a, hipStream_t s);
+hipError_t launch_kv8_advance(int32_t* lens, const int32_t* fresh, int B, int S, hipStream_t s);
+struct Kv8AttnArgs {
+    Kv8 c;
+    const void* q;
+    float* o;
+    _Float16* o16;
+    int64_t qst[4], ost[4];
+    int S, H;
+    bool in16;
+    const int32_t* lens;
+    const int32_t* fresh;
+    ScoreMod mod;
+    const float* slopes;
+};
+hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t s);
+
+// Penalties, bias and grammar mask on logits (k_logits.hip)
+struct LogitsArgs {
+    const void* x;
+    void* y;
+    int64_t x_stride, y_stride;
+    int rows, V;
+    bool f16;
+    const int32_t* hist;
+    const int32_t* hist_len;
+    int64_t hist_stride;
+    int max_hist;
+    const float* rep;
+    const float* freq;
+    const float* pres;
+    const float* bias;
+    int64_t bias_stride;
+    const uint32_t* allowed;
+    int64_t allowed_stride;
+};
+hipError_t launch_logits_process(const LogitsArgs& a, hipStream_t s);
+
 size_t noalloc_scratch_bytes();
 hipError_t noalloc_scratch(int device, void** out);
 // order a call's launches on `s` after the previous call's on this device (event wait; takes a

@@ -380,6 +380,118 @@ int mgh_decode_step(mgh_ctx* ctx, void* d_state, void* d_work, const float* d_lo
                     int V, int codebook, int mask_id, int n_tokens, int step, int n_steps,
                     float choice_temp, int32_t* d_tokens, int32_t* d_result);
 
+/* ---- attention under masks, with capped or sloped scores, grouped heads and queries that may be fewer
+ *      than the keys. No counterpart in the reference, whose attention sees every key
+ *      (mg-opencl.cpp:859-937). q is a {D, Sq, H, B} view and k and v are {D, Sk, Hkv, B} views with
+ *      element strides q_strides and kv_strides (d, s, h, b), fp16 (in_f16) or fp32, rounded to fp16
+ *      as mgh_flash_attn_f16kv does; head h reads the keys of head h / (H / Hkv). Query i stands at
+ *      position p = Sk - Sq + i of the keys. Exactly one of d_o (fp32) and d_o16 is non-NULL, with
+ *      element strides o_strides (NULL: contiguous {D, Sq, H, B}).
+ *        s = scale q . k_j;  cap > 0: s <- cap tanh(s / cap);  d_slopes [H]: s <- s - slopes[h] |p - j|
+ *      Key j is seen where
+ *        causal is 0, or j <= p, or j < d_prefix[b] (d_prefix [B], with causal only); and
+ *        d_docs is NULL, or docs[b][j] == docs[b][p] >= 0 (ids of the Sk positions, rows doc_stride
+ *        apart, 0: one row for all; negative: padding; a query before position 0 has none).
+ *      o = softmax over the seen keys, times v; a row that sees none, or only scores of -infinity, is 0.
+ *      What masked keys hold, infinities and NaN included, does not matter, nor does the value of a key
+ *      whose weight is zero. Sums and softmax in fp32; with an fp16 output the weights are rounded to
+ *      fp16 before they meet v, with an fp32 output they keep 22 bits.
+ *      D a multiple of 16 up to 128. Rows that are not fp16, 16-byte aligned (pointers and all
+ *      strides but the first) with unit feature stride are first packed into the context's scratch,
+ *      and calls with few rows keep partial results in its workspace: run a shape once before it is
+ *      captured. */
+typedef struct mgh_attn_opts {
+    float cap;                   /* 0: none */
+    int causal;
+    const float* d_slopes;
+    const int32_t* d_prefix;
+    const int32_t* d_docs;
+    int64_t doc_stride;
+} mgh_attn_opts;
+int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* d_v, int in_f16,
+                    const int64_t q_strides[4], const int64_t kv_strides[4], int D, int Sq, int Sk, int H, int Hkv,
+                    int B, float scale, const mgh_attn_opts* opts /* NULL: none */, float* d_o, void* d_o16,
+                    const int64_t o_strides[4]);
+
+/* ---- a cache of keys and values in 8 bits, and attention over it, for generating token by token. No
+ *      counterpart in the reference, which generates by whole bidirectional forwards. Values are held
+ *      as Q8 codes (the reference's rule, mg-opencl.cpp:424-434: d = max|x| / 127 in fp32, codes x / d
+ *      rounded half away from zero, here of the exact quotient) with one scale per block of 32 tokens,
+ *      head, and K or V. Block i of sequence b is page table[b][i] of a pool that all sequences share:
+ *        d_k      [pages][Hkv][32][D] bytes, code + 128
+ *        d_v      [pages][Hkv][D/2][4][2][8] bytes: token t, feature d at
+ *                 ((d/2)*4 + t/8)*16 + (d%2)*8 + t%8 of its block
+ *        d_scales [pages][Hkv][2] fp32, K's and V's
+ *        d_k_tail [B][Hkv][64][D], d_v_tail [B][Hkv][D][64] fp16: the last 64 tokens as they came, token
+ *                 t at t % 64. The tokens behind the last whole block are read from here; a block gets
+ *                 its codes from here once its 32 tokens are there. So the cache does not depend on how
+ *                 tokens were grouped into calls, and a sequence may be shortened (its length lowered)
+ *                 by up to 32 tokens.
+ *      d_lens [B] holds each sequence's length before the step, d_new [B] its new tokens, 0 .. S (NULL:
+ *      S each): append writes them at positions lens[b] + i, attention takes them as queries at those
+ *      positions (each sees the cache up to its own position), and after the last layer mgh_kv8_advance
+ *      adds them to the lengths. Rows past a sequence's new tokens are neither read nor written.
+ *      A sequence whose numbers do not fit (negative, more than S new tokens, past max_blocks * 32) is
+ *      left alone by append and gives NaN rows in attention and read, as does a page number outside the
+ *      pool among the blocks a call reads; nothing outside the buffers is touched. Two sequences may
+ *      share pages that are whole. A block that holds an infinity or NaN reads as NaN.
+ *      D a multiple of 16 up to 128; d_k, d_v and the tails 16-byte, d_scales 8-byte aligned;
+ *      max_blocks * 32 and S up to 2^29. */
+typedef struct mgh_kv8 {
+    void* d_k;
+    void* d_v;
+    float* d_scales;
+    void* d_k_tail;
+    void* d_v_tail;
+    const int32_t* d_table;      /* rows of max_blocks page numbers, table_stride apart */
+    int64_t table_stride;
+    int64_t pages;
+    int max_blocks;
+    int Hkv, D, B;
+} mgh_kv8;
+size_t mgh_kv8_code_bytes(int64_t pages, int Hkv, int D);    /* of d_k, and of d_v */
+size_t mgh_kv8_scale_bytes(int64_t pages, int Hkv);
+size_t mgh_kv8_tail_bytes(int B, int Hkv, int D);            /* of d_k_tail, and of d_v_tail */
+/* k, v: {D, S, Hkv, B} views (element strides d, token, head, sequence), fp16 or fp32 (rounded to fp16) */
+int mgh_kv8_append(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_k, const void* d_v, int in_f16,
+                   const int64_t strides[4], int S, const int32_t* d_lens, const int32_t* d_new);
+int mgh_kv8_advance(mgh_ctx* ctx, int32_t* d_lens, const int32_t* d_new, int B, int S);
+/* q, o: {D, S, H, B} views, scores as mgh_attn_masked (cap, d_slopes [H] or NULL); calls with few rows keep
+ * partial results in the context's workspace: run a shape once before it is captured */
+int mgh_kv8_attn(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_q, int in_f16, const int64_t q_strides[4], int S,
+                 const int32_t* d_lens, const int32_t* d_new, int H, float scale, float cap, const float* d_slopes,
+                 float* d_o, void* d_o16, const int64_t o_strides[4]);
+/* the values that the cache holds at positions first[b] + i (d_first NULL: i), i < n, of a sequence of
+ * lens[b] tokens -> [B][Hkv][n][D], fp32 in d_k and d_v or fp16 in d_k16 and d_v16; rows at or past lens[b]
+ * are left as they were */
+int mgh_kv8_read(mgh_ctx* ctx, const mgh_kv8* cache, const int32_t* d_first, int n, const int32_t* d_lens, float* d_k,
+                 float* d_v, void* d_k16, void* d_v16);
+
+/* ---- what is done to logits before sampling (mgh_decode_step, or an arg max). No counterpart in the
+ *      reference, which samples from the head's output (mg-generate.cpp:82-121). x and y: rows of V logits
+ *      x_stride and y_stride apart, fp32 or fp16 (f16); y may be x with the same stride. Token v
+ *      with n > 0 occurrences in the row's history: l <- (l > 0 ? l / rep : l rep) - (freq n + pres); then
+ *      l <- l + bias[v]; then -infinity where bit v % 32 of allowed word v / 32 is 0. fp32 arithmetic.
+ *      Each part is left out where its pointer is NULL: d_hist (rows of max_hist ids, hist_stride apart;
+ *      d_hist_len [rows]: the ids that count, clamped to 0 .. max_hist; ids outside 0 .. V - 1 count
+ *      nowhere), d_rep, d_freq, d_pres [rows] (rep > 0), d_bias (rows bias_stride apart, 0: one for all)
+ *      and d_allowed (rows allowed_stride words apart, 0: one for all). V up to 2^30. */
+typedef struct mgh_logits_opts {
+    const int32_t* d_hist;
+    int64_t hist_stride;
+    int max_hist;
+    const int32_t* d_hist_len;
+    const float* d_rep;
+    const float* d_freq;
+    const float* d_pres;
+    const float* d_bias;
+    int64_t bias_stride;
+    const uint32_t* d_allowed;
+    int64_t allowed_stride;
+} mgh_logits_opts;
+int mgh_logits_process(mgh_ctx* ctx, const void* d_x, int f16, int64_t x_stride, int rows, int V,
+                       const mgh_logits_opts* opts, void* d_y, int64_t y_stride);
+
 /* ---- debug: the int32 per-block dot products exactly as the production GEMM's MFMA
  *      computes them, out[m][n][t] (t = K/32 blocks). The reference has no counterpart;
  *      it exposes the quantity mg-opencl.cpp:472-478 / :571-576 accumulates. ---- */
