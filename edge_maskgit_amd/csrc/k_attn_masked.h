@@ -1,0 +1,441 @@
+// k_attn_masked.h — the tiled kernel of k_attn_masked*.hip: attention under masks (gfx950).
+//
+// Rows: the G = H / Hkv query heads of a key head are G rows of each query position, so a workgroup's 4
+// waves hold 64 QT rows (row r = query r / G, head r % G) against one head's keys, taken 64 at a time.
+//  * K and V chunks go from memory to LDS by 16-byte buffer loads, two buffers in turn, one barrier per
+//    chunk; pieces are XOR-swizzled by their row (a property of the lane's source address) so that both
+//    ways of reading are free of bank conflicts. Rows past the last key and features past D arrive as
+//    zeros (outside the buffer's range). V needs no transposed copy: ds_read_b64_tr_b16 hands each lane
+//    4 keys of its feature.
+//  * S^T = K Q^T on v_mfma_f32_16x16x32_f16: a lane holds scores of one row (query l16), 4 keys per
+//    register quadruple, which is the operand of O^T = V^T P^T as it stands. Row sums by the same
+//    instruction on ones, so they add exactly the weights that meet V.
+//  * The softmax reference of a row stays within [-7, 15] (log2 units) of its maximum: it moves, and O is
+//    rescaled, only when a score passes it by 15, a wave-uniform branch. Weights lie in fp16's normal
+//    range up to 2^15; with an fp32 output (PS) a weight is hi + lo in fp16, both to nearest, and a
+//    chunk's products are summed apart from O.
+//  * Which keys a row sees is one bound per row (causal and prefix together), known per wave, so that whole
+//    chunks need no test; ids of documents are compared only in chunks where they can differ: a first
+//    pass over the ids notes for each chunk whether any row of the workgroup can see it and whether all
+//    see all of it.
+// A masked key's weight is 0, but 0 times an infinity or NaN of V is not: rows that come out not finite are
+// taken again by attn_row, which reads what a row sees and nothing else.
+#pragma once
+#include "k_attn_row.h"
+
+namespace mgh {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kMaskKeys = 64;              // keys per chunk
+constexpr int kMaskScan = 16384;           // chunks whose documents are noted (1 M keys)
+
+struct MaskedSrc {
+    const MaskedAttnArgs& a;
+    const _Float16* k;     // the head's rows
+    const _Float16* v;
+    int64_t stride;
+    int lim;               // the last key that causal and prefix leave
+    const int32_t* docs;   // the sequence's ids, or null
+    int doc;
+    __device__ bool seen(int64_t j) const { return j <= lim && (!docs || (docs[j] == doc && doc >= 0)); }
+    __device__ float dot(int64_t j, const float* qs) const {
+        const _Float16* p = k + j * stride;
+        float s = 0.f;
+        for (int d = 0; d < a.D; d++) s = fmaf(qs[d], (float)p[d], s);
+        return s;
+    }
+    __device__ float value(int64_t j, int d) const { return (float)v[j * stride + d]; }
+};
+
+// XOR of a 16-byte piece's place in its LDS row: 8 rows of a score operand's pieces, and the 4 rows x 2
+// pieces of a transposing read, fall on different banks
+template <int PPR>
+__device__ __forceinline__ int piece_swz(int r) {
+    return PPR >= 8 ? 2 * (r & 3) + ((r >> 2) & 1) : 2 * ((r >> 1) & 1) + ((r >> 2) & 1);
+}
+
+// DC 16-feature chunks (D <= 16 DC), QT 16-row tiles per wave, PS: weights as hi + lo; MOD 0: scores times a
+// positive scale, 1: any scale and slopes (0: none), 2: capped, then slopes.
+template <int DC, int QT, bool PS, int MOD>
+__global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int tiles, int splits) {
+    constexpr int PPR = DC <= 2 ? 4 : DC <= 4 ? 8 : 16;       // 16-byte pieces of an LDS row
+    constexpr int KC = (DC + 1) / 2, NT = kMaskKeys / 16, NI = kMaskKeys * PPR / 256;
+    constexpr int ROWB = PPR * 16, CH = kMaskKeys * ROWB;     // bytes of an LDS row, of a K or V chunk
+    constexpr int WROWS = 16 * QT;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * CH + 2 * kMaskKeys * 4];
+    __shared__ uint32_t bits[2][kMaskScan / 32];              // chunks that some row sees; that all rows see all of
+    __shared__ int range[3][4];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, lg = lane >> 4;
+    // each XCD takes contiguous runs of (sequence, key head); of a head the last rows, which see most, first
+    const int lid = xcd_remap(blockIdx.x, gridDim.x);
+    const int hb = lid / (tiles * splits), in_h = lid - hb * (tiles * splits);
+    const int tile = tiles - 1 - in_h / splits, sp = in_h % splits;
+    const int hk = hb % a.Hkv, b = hb / a.Hkv, G = a.H / a.Hkv, R = a.Sq * G, off = a.Sk - a.Sq;
+    const int prefix = a.prefix ? min(a.prefix[b], a.Sk) : 0;
+    auto bound_of = [&](int i) { return a.causal ? min(max(off + i, prefix - 1), a.Sk - 1) : a.Sk - 1; };
+    const int r0 = tile * 4 * WROWS, rw = r0 + wave * WROWS;
+    const int wg_hi = bound_of((min(r0 + 4 * WROWS, R) - 1) / G);
+    const int w_lo = rw < R ? bound_of(rw / G) : -1, w_hi = rw < R ? bound_of((min(rw + WROWS, R) - 1) / G) : -1;
+
+    // this lane's rows
+    int lim[QT], doc[QT];
+    float pos[QT], slope2[QT];
+    const int32_t* docs = a.docs ? a.docs + (int64_t)b * a.doc_stride : nullptr;
+    f16x8 qf[QT][KC];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const int r = rw + 16 * t + l16, i = min(r, R - 1) / G, g = min(r, R - 1) - i * G;
+        lim[t] = r < R ? bound_of(i) : -1;
+        pos[t] = (float)(off + i);
+        doc[t] = docs && off + i >= 0 && r < R ? docs[off + i] : -1;
+        slope2[t] = MOD && a.slopes ? a.slopes[hk * G + g] * kLog2e : 0.f;
+        const _Float16* q = (const _Float16*)a.q + b * a.qst[3] + (int64_t)(hk * G + g) * a.qst[2] + i * a.qst[1];
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            const int d = 32 * c + 8 * lg;
+            qf[t][c] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (d < a.D) qf[t][c] = *(const f16x8*)(q + d);
+        }
+    }
+
+    // this split's chunks
+    const int nch = wg_hi / kMaskKeys + 1, per = (nch + splits - 1) / splits;
+    const int c0 = wg_hi < 0 ? 0 : sp * per, c1 = wg_hi < 0 ? 0 : min(nch, c0 + per);
+    const bool scan = docs && c1 - c0 <= kMaskScan;
+    if (scan) {
+        // the workgroup's ids: smallest, largest, and whether every row has one
+        const int i0 = r0 / G, i1 = (min(r0 + 4 * WROWS, R) - 1) / G;
+        int lo = INT32_MAX, hi = -1, all = 1;
+        for (int i = i0 + tid; i <= i1; i += 256) {
+            const int x = off + i >= 0 ? docs[off + i] : -1;
+            if (x < 0) all = 0;
+            else lo = min(lo, x), hi = max(hi, x);
+        }
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) lo = min(lo, __shfl_xor(lo, s)), hi = max(hi, __shfl_xor(hi, s)), all &= __shfl_xor(all, s);
+        if (lane == 0) range[0][wave] = lo, range[1][wave] = hi, range[2][wave] = all;
+        for (int i = tid; i < (c1 - c0 + 31) / 32; i += 256) bits[0][i] = bits[1][i] = 0;
+        __syncthreads();
+        for (int w = 0; w < 4; w++) lo = min(lo, range[0][w]), hi = max(hi, range[1][w]), all &= range[2][w];
+        all = all && lo == hi;
+        for (int c = c0 + wave; c < c1; c += 4) {
+            const int j = c * kMaskKeys + lane;
+            const int x = j < a.Sk ? docs[j] : -1;
+            const bool some = __any(x >= lo && x <= hi), whole = __all(x == hi || j >= a.Sk) && all;
+            if (lane == 0 && some) {
+                atomicOr(&bits[0][(c - c0) >> 5], 1u << ((c - c0) & 31));
+                if (whole) atomicOr(&bits[1][(c - c0) >> 5], 1u << ((c - c0) & 31));
+            }
+        }
+        __syncthreads();
+    }
+    // the next chunk from c on that some row sees, or c1
+    auto find = [&](int c) {
+        if (!scan) return c;
+        while (c < c1) {
+            const uint32_t w = __builtin_amdgcn_readfirstlane(bits[0][(c - c0) >> 5]) >> ((c - c0) & 31);
+            if (w) return min(c1, c + __builtin_ctz(w));
+            c = c0 + (((c - c0) >> 5) + 1) * 32;
+        }
+        return c1;
+    };
+
+    // staging: thread n = 256 u + tid of a chunk fills slot n of the buffer; the piece that belongs there
+    const int64_t kv0 = b * a.kvst[3] + hk * a.kvst[2];
+    const uint32_t rowb = (uint32_t)a.kvst[1] * 2;
+    uint32_t src[NI];
+#pragma unroll
+    for (int u = 0; u < NI; u++) {
+        const int n = 256 * u + tid, r = n / PPR, p = (n % PPR) ^ piece_swz<PPR>(r);
+        src[u] = 8 * p < a.D ? r * rowb + 16 * p : 0x80000000u;
+    }
+    auto stage = [&](int c, int buf) {
+        const int left = a.Sk - c * kMaskKeys;               // rows from this chunk on, >= 1
+        const uint32_t ext = (uint32_t)(min(left, kMaskKeys) - 1) * rowb + 2 * a.D;
+        const int64_t at = kv0 + (int64_t)c * kMaskKeys * a.kvst[1];
+        auto rsrc = [&](const void* p) {
+            return __builtin_amdgcn_make_buffer_rsrc((void*)((const _Float16*)p + at), (short)0, (int)ext, 0x00020000);
+        };
+        const __amdgpu_buffer_rsrc_t rk = rsrc(a.k), rv = rsrc(a.v);
+        char* B = lds + buf * 2 * CH + wave * 1024;
+#pragma unroll
+        for (int u = 0; u < NI; u++) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(B + 4096 * u), 16, (int)src[u], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(B + CH + 4096 * u), 16, (int)src[u], 0, 0, 0);
+        }
+        if (docs && wave == 0) {
+            const __amdgpu_buffer_rsrc_t rd =
+                __builtin_amdgcn_make_buffer_rsrc((void*)(docs + c * kMaskKeys), (short)0, 4 * min(left, kMaskKeys), 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (lds_void*)(lds + 4 * CH + buf * 4 * kMaskKeys), 4, 4 * lane, 0, 0, 0);
+        }
+    };
+    // where this lane reads: K row l16 of a tile, pieces 4 c + lg; V rows 4 lg + l16 / 4 (of 16), 4 features at
+    // 16 c + 4 (l16 % 4)
+    uint32_t ka[2], va[4];
+#pragma unroll
+    for (int c = 0; c < 2; c++) ka[c] = l16 * ROWB + (((4 * c + lg) ^ piece_swz<PPR>(l16)) & (PPR - 1)) * 16;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const int r = 4 * lg + (l16 >> 2), p = 2 * c + ((l16 & 3) >> 1);
+        va[c] = r * ROWB + ((p ^ piece_swz<PPR>(r)) & (PPR - 1)) * 16 + 8 * (l16 & 1);
+    }
+
+    float mref[QT], S1[QT];
+    f32x4 O[QT][DC];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        mref[t] = -1e30f;
+        S1[t] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DC; c++) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    const float scale2 = a.mod.scale2;
+
+    int buf = 0;
+    int c = find(c0);
+    if (c < c1) stage(c, 0);
+    while (c < c1) {
+        const int cn = find(c + 1);
+        stage_sync<0>();                     // this buffer is filled, the other one no longer read
+        if (cn < c1) stage(cn, buf ^ 1);
+        const int k0 = c * kMaskKeys;
+        if (k0 <= w_hi) {
+            const char* K = lds + buf * 2 * CH;
+            const char* V = K + CH;
+            const bool same = !docs || (scan && (__builtin_amdgcn_readfirstlane(bits[1][(c - c0) >> 5]) >> ((c - c0) & 31) & 1));
+            f32x4 sc[QT][NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                f16x8 kf[KC];
+#pragma unroll
+                for (int i = 0; i < KC; i++) kf[i] = *(const f16x8*)(K + ka[i & 1] + 128 * (i >> 1) + 16 * n * ROWB);
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < KC; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf[t][i], acc, 0, 0, 0);
+                    sc[t][n] = acc;
+                }
+            }
+            if (MOD) {
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const float x = MOD == 2 ? cap_score(sc[t][n][r], a.mod) : sc[t][n][r] * scale2;
+                            sc[t][n][r] = fmaf(-slope2[t], fabsf(pos[t] - (float)(k0 + 16 * n + 4 * lg + r)), x);
+                        }
+            }
+            // the results are in their registers before a branch looks at them
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+            if (k0 + kMaskKeys - 1 > w_lo) {
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (k0 + 16 * n + 4 * lg + r > lim[t]) sc[t][n][r] = -INFINITY;
+            }
+            if (!same) {
+                const int32_t* ids = (const int32_t*)(lds + 4 * CH + buf * 4 * kMaskKeys);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const i32x4 id = *(const i32x4*)(ids + 16 * n + 4 * lg);
+#pragma unroll
+                    for (int t = 0; t < QT; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            if (id[r] != doc[t] || doc[t] < 0) sc[t][n][r] = -INFINITY;
+                }
+            }
+            float mx[QT];
+            bool up[QT], any = false;
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float v = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    v = fmaxf(fmaxf(v, sc[t][n][0]), sc[t][n][1]);
+                    v = fmaxf(fmaxf(v, sc[t][n][2]), sc[t][n][3]);
+                }
+                mx[t] = MOD ? v : v * scale2;
+                up[t] = __any(mx[t] > mref[t] + 15.f);
+                any = any || up[t];
+            }
+            if (any) {
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    float v = up[t] ? fmaxf(mx[t] - 7.f, mref[t]) : mref[t];
+                    v = fmaxf(v, __shfl_xor(v, 16));
+                    v = fmaxf(v, __shfl_xor(v, 32));
+                    const float al = __builtin_amdgcn_exp2f(mref[t] - v);
+                    mref[t] = v;
+                    S1[t] *= al;
+#pragma unroll
+                    for (int cc = 0; cc < DC; cc++) O[t][cc] *= al;
+                }
+            }
+            f32x4 s1[QT], oc[QT][DC];
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                s1[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int cc = 0; cc < DC; cc++) oc[t][cc] = PS ? f32x4{0.f, 0.f, 0.f, 0.f} : O[t][cc];
+            }
+#pragma unroll
+            for (int p = 0; p < NT / 2; p++) {
+                f16x8 ph[QT], pl[QT];
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    float e[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float s = sc[t][2 * p + j / 4][j % 4];
+                        e[j] = __builtin_amdgcn_exp2f(MOD ? s - mref[t] : fmaf(s, scale2, -mref[t]));
+                    }
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const f16x2 h = __builtin_convertvector((f32x2{e[2 * j], e[2 * j + 1]}), f16x2);
+                        hi[j] = __builtin_bit_cast(uint32_t, h);
+                        if (PS) {
+                            const f32x2 d = {e[2 * j] - (float)h[0], e[2 * j + 1] - (float)h[1]};
+                            lo[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, f16x2));
+                        }
+                    }
+                    ph[t] = __builtin_bit_cast(f16x8, hi);
+                    if (PS) pl[t] = __builtin_bit_cast(f16x8, lo);
+                }
+#pragma unroll
+                for (int cc = 0; cc < DC; cc++) {
+                    const char* at = V + va[cc & 3] + 128 * (cc >> 2) + 32 * p * ROWB;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * ROWB));
+                    const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int t = 0; t < QT; t++) {
+                        if (PS) oc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], oc[t][cc], 0, 0, 0);
+                        oc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], oc[t][cc], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    if (PS) s1[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t], s1[t], 0, 0, 0);
+                    s1[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[t], s1[t], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                S1[t] += s1[t][0];
+#pragma unroll
+                for (int cc = 0; cc < DC; cc++) O[t][cc] = PS ? O[t][cc] + oc[t][cc] : oc[t][cc];
+            }
+        }
+        c = cn;
+        buf ^= 1;
+    }
+
+    // rows that are not finite: again, key by key
+    __syncthreads();
+    float* qs = (float*)lds + wave * 256;
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        float z = S1[t];
+#pragma unroll
+        for (int cc = 0; cc < DC; cc++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) z += O[t][cc][r] * 0.f;
+        uint64_t m = __ballot(!(z - z == 0.f) && rw + 16 * t + l16 < R);
+        m = (m | m >> 16 | m >> 32 | m >> 48) & 0xffff;
+        while (m) {
+            const int l = __builtin_ctzll(m), r = rw + 16 * t + l, i = r / G, g = r - i * G;
+            m &= m - 1;
+            const _Float16* q = (const _Float16*)a.q + b * a.qst[3] + (int64_t)(hk * G + g) * a.qst[2] + i * a.qst[1];
+            for (int d = lane; d < 128; d += 64) qs[d] = d < a.D ? (float)q[d] : 0.f;
+            __builtin_amdgcn_wave_barrier();
+            const MaskedSrc s{a, (const _Float16*)a.k + kv0, (const _Float16*)a.v + kv0, a.kvst[1], bound_of(i), docs,
+                              docs && off + i >= 0 ? docs[off + i] : -1};
+            const float sl = a.slopes ? a.slopes[hk * G + g] * kLog2e : 0.f;
+            const RowState st = attn_row(s, a.mod, sl, off + i, (int64_t)c0 * kMaskKeys, min((int64_t)c1 * kMaskKeys, (int64_t)a.Sk), a.D, qs,
+                                         qs + 128, lane);
+            __builtin_amdgcn_wave_barrier();
+            qs[lane] = st.o[0], qs[lane + 64] = st.o[1];
+            __builtin_amdgcn_wave_barrier();
+            if (l16 == l) {
+                mref[t] = st.m == -INFINITY ? -1e30f : st.m;
+                S1[t] = st.l;
+#pragma unroll
+                for (int cc = 0; cc < DC; cc++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) O[t][cc][x] = qs[16 * cc + 4 * lg + x];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const int r = rw + 16 * t + l16;
+        if (r >= R) continue;
+        if (splits > 1) {
+            const int64_t rows = (int64_t)a.B * a.Hkv * R, row = (int64_t)hb * R + r;
+            float* w = a.ws + (sp * rows + row) * a.D;
+#pragma unroll
+            for (int cc = 0; cc < DC; cc++)
+                if (16 * cc < a.D) *(f32x4*)(w + 16 * cc + 4 * lg) = O[t][cc];
+            if (lg == 0) *(f32x2*)(a.ws + splits * rows * a.D + 2 * (sp * rows + row)) = f32x2{mref[t], S1[t]};
+            continue;
+        }
+        const int i = r / G, g = r - i * G;
+        const float inv = S1[t] == 0.f ? 0.f : 1.f / S1[t];
+        const int64_t ro = (int64_t)b * a.ost[3] + (int64_t)(hk * G + g) * a.ost[2] + (int64_t)i * a.ost[1];
+#pragma unroll
+        for (int cc = 0; cc < DC; cc++) {
+            const int d = 16 * cc + 4 * lg;
+            if (d >= a.D) continue;
+            const f32x4 v = S1[t] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : O[t][cc] * inv;
+            if (a.vec_o) {
+                if (a.o16) *(f16x4*)(a.o16 + ro + d) = __builtin_convertvector(v, f16x4);
+                else *(f32x4*)(a.o + ro + d) = v;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int64_t e = ro + (int64_t)(d + x) * a.ost[0];
+                    if (a.o16) a.o16[e] = (_Float16)v[x];
+                    else a.o[e] = v[x];
+                }
+            }
+        }
+    }
+}
+
+template <int DC, int QT, bool PS>
+hipError_t launch_masked_t(const MaskedAttnArgs& a, int splits, hipStream_t s) {
+    const int tiles = (int)(((int64_t)a.Sq * (a.H / a.Hkv) + 64 * QT - 1) / (64 * QT));
+    const dim3 grid((unsigned)((int64_t)tiles * splits * a.Hkv * a.B));
+    if (a.mod.cap2 != 0.f) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
+    else if (a.slopes || !(a.mod.scale2 > 0.f)) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 1>), grid, dim3(256), 0, s, a, tiles, splits);
+    else hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 0>), grid, dim3(256), 0, s, a, tiles, splits);
+    return hipGetLastError();
+}
+
+template <int DC>
+hipError_t launch_masked_d(const MaskedAttnArgs& a, const MaskedPlan& p, hipStream_t s) {
+    if (p.qt == 2) return a.o16 ? launch_masked_t<DC, 2, false>(a, p.splits, s) : launch_masked_t<DC, 2, true>(a, p.splits, s);
+    return a.o16 ? launch_masked_t<DC, 1, false>(a, p.splits, s) : launch_masked_t<DC, 1, true>(a, p.splits, s);
+}
+
+}  // namespace mgh

@@ -1,63 +1,110 @@
-// k_attn_masked.hip — attention under causal, prefix and document masks with capped or sloped scores.
-#include "k_attn_row.h"
+// k_attn_masked.hip — attention under causal, prefix and document masks with capped or sloped scores: the
+// narrow heads of the tiled kernel (k_attn_masked.h), the packing of rows that it does not take as they are,
+// and the joining of what a head's keys gave in parts.
+#include <algorithm>
+
+#include "k_attn_masked.h"
 
 namespace mgh {
 
 namespace {
 
-// q, k, v as they come, rounded to fp16
-__device__ __forceinline__ float elem(const void* p, bool f16, int64_t e) {
-    return f16 ? (float)((const _Float16*)p)[e] : (float)(_Float16)((const float*)p)[e];
+// {D, S, H, B} views of any type and strides -> fp16 [B][H][S][D]; blockIdx.y: q, k, v. One thread per 8
+// features.
+__global__ __launch_bounds__(256) void k_attn_pack(PackArgs p) {
+    const PackArgs::View& v = p.v[blockIdx.y];
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int D8 = p.D / 8;
+    if (n >= (int64_t)p.B * v.H * v.S * D8) return;
+    const int d = 8 * (int)(n % D8);
+    const int64_t row = n / D8;
+    const int64_t e = row / v.S / v.H * v.st[3] + row / v.S % v.H * v.st[2] + row % v.S * v.st[1] + d * v.st[0];
+    f16x8 x;
+    if (p.in16) {
+        const _Float16* s = (const _Float16*)v.src + e;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = s[i * v.st[0]];
+    } else {
+        const float* s = (const float*)v.src + e;
+        if (v.vec) {
+            const f32x4 lo = *(const f32x4*)s, hi = *(const f32x4*)(s + 4);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (_Float16)(i < 4 ? lo[i] : hi[i - 4]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (_Float16)s[i * v.st[0]];
+        }
+    }
+    *(f16x8*)(v.dst + row * p.D + d) = x;
 }
 
-struct MaskedSrc {
-    const MaskedAttnArgs& a;
-    int64_t kv;            // element offset of the sequence's and head's first row
-    int64_t p;             // the row's position
-    int prefix;
-    const int32_t* docs;   // the sequence's ids, or null
-    int doc;
-    __device__ bool seen(int64_t j) const {
-        return (!a.causal || j <= p || j < prefix) && (!docs || (docs[j] == doc && doc >= 0));
+// one wave per row: the parts' states, joined in their order
+__global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const f32x2* ml = (const f32x2*)(a.ws + a.splits * a.rows * a.D);
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; s++) m = fmaxf(m, ml[s * a.rows + row][0]);
+    float l = 0.f, o[2] = {0.f, 0.f};
+    for (int s = 0; s < a.splits; s++) {
+        const f32x2 x = ml[s * a.rows + row];
+        const float w = x[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - m);
+        if (x[1] == 0.f) continue;
+        l = fmaf(w, x[1], l);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (lane + 64 * i < a.D) o[i] = fmaf(w, a.ws[(s * a.rows + row) * a.D + lane + 64 * i], o[i]);
     }
-    __device__ float dot(int64_t j, const float* qs) const {
-        const int64_t e = kv + j * a.kvst[1];
-        float s = 0.f;
-        for (int d = 0; d < a.D; d++) s = fmaf(qs[d], elem(a.k, a.in16, e + d * a.kvst[0]), s);
-        return s;
-    }
-    __device__ float value(int64_t j, int d) const { return elem(a.v, a.in16, kv + j * a.kvst[1] + d * a.kvst[0]); }
-};
-
-__global__ __launch_bounds__(256) void k_attn_masked(MaskedAttnArgs a) {
-    __shared__ float qs[4][128], pl[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.Hkv);
-    const int64_t i = (int64_t)blockIdx.x * 4 + wave;
-    if (i >= a.Sq) return;
-    const int64_t p = (int64_t)a.Sk - a.Sq + i;
-    const int64_t qe = b * a.qst[3] + h * a.qst[2] + i * a.qst[1];
-    for (int d = lane; d < a.D; d += 64) qs[wave][d] = elem(a.q, a.in16, qe + d * a.qst[0]);
-    __builtin_amdgcn_wave_barrier();
-    MaskedSrc src{a, b * a.kvst[3] + hk * a.kvst[2], p, a.prefix ? a.prefix[b] : 0, a.docs ? a.docs + b * a.doc_stride : nullptr, -1};
-    if (src.docs && p >= 0) src.doc = src.docs[p];
-    const float slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
-    const RowState st = attn_row(src, a.mod, slope2, p, 0, a.Sk, a.D, qs[wave], pl[wave], lane);
-    const int64_t oe = b * a.ost[3] + h * a.ost[2] + i * a.ost[1];
-    for (int t = 0; t < 2; t++) {
-        const int d = lane + 64 * t;
+    const int64_t hb = row / a.R;
+    const int r = (int)(row - hb * a.R), i = r / a.G, g = r - i * a.G;
+    const int64_t ro = hb / a.Hkv * a.ost[3] + (hb % a.Hkv * a.G + g) * a.ost[2] + i * a.ost[1];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int d = lane + 64 * x;
         if (d >= a.D) continue;
-        const float o = st.l == 0.f ? 0.f : st.o[t] / st.l;
-        if (a.o16) a.o16[oe + d * a.ost[0]] = (_Float16)o;
-        else a.o[oe + d * a.ost[0]] = o;
+        const float v = l == 0.f ? 0.f : o[x] / l;
+        if (a.o16) a.o16[ro + d * a.ost[0]] = (_Float16)v;
+        else a.o[ro + d * a.ost[0]] = v;
     }
 }
 
 }  // namespace
 
-hipError_t launch_attn_masked(const MaskedAttnArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(k_attn_masked, dim3((unsigned)((a.Sq + 3) / 4), (unsigned)a.H, (unsigned)a.B), dim3(256), 0, s, a);
+hipError_t launch_attn_pack(const PackArgs& p, hipStream_t s) {
+    int64_t most = 0;
+    for (int i = 0; i < p.n; i++) most = std::max(most, (int64_t)p.B * p.v[i].H * p.v[i].S * (p.D / 8));
+    hipLaunchKernelGGL(k_attn_pack, dim3((unsigned)((most + 255) / 256), (unsigned)p.n), dim3(256), 0, s, p);
     return hipGetLastError();
+}
+
+hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+MaskedPlan masked_plan(const MaskedAttnArgs& a) {
+    const int64_t R = (int64_t)a.Sq * (a.H / a.Hkv), heads = (int64_t)a.Hkv * a.B, nch = (a.Sk + kMaskKeys - 1) / kMaskKeys;
+    MaskedPlan p{1, 1, 0};
+    if (heads * ((R + 127) / 128) >= 256) p.qt = 2;
+    const int64_t wgs = heads * ((R + 64 * p.qt - 1) / (64 * p.qt));
+    if (wgs < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, nch / 4));
+    if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.D + 2) * sizeof(float);
+    return p;
+}
+
+hipError_t launch_attn_masked(const MaskedAttnArgs& a, const MaskedPlan& p, hipStream_t s) {
+    const int dc = a.D / 16;
+    const hipError_t e = dc <= 2 ? launch_masked_d<2>(a, p, s) : dc == 3 ? launch_masked_d<3>(a, p, s)
+                       : dc == 4 ? launch_masked_d<4>(a, p, s) : launch_attn_masked_wide(a, p, s);
+    if (e != hipSuccess || p.splits == 1) return e;
+    JoinArgs j{};
+    j.ws = a.ws; j.o = a.o; j.o16 = a.o16;
+    for (int i = 0; i < 4; i++) j.ost[i] = a.ost[i];
+    j.G = a.H / a.Hkv; j.Hkv = a.Hkv; j.D = a.D; j.splits = p.splits;
+    j.R = (int64_t)a.Sq * j.G;
+    j.rows = j.R * a.Hkv * a.B;
+    return launch_attn_join(j, s);
 }
 
 }  // namespace mgh

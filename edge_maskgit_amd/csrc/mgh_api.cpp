@@ -1247,6 +1247,11 @@ int check_scores(mgh_ctx* c, const char* fn, int D, int H, int Hkv, float scale,
 
 bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+// features in order, and rows that start at multiples of `bytes` (`elems` elements)
+bool rows_aligned(const void* p, const int64_t st[4], int elems, size_t bytes) {
+    return st[0] == 1 && st[1] % elems == 0 && st[2] % elems == 0 && st[3] % elems == 0 && aligned_to(p, bytes);
+}
+
 int check_kv8(mgh_ctx* c, const char* fn, const mgh_kv8* kv, mgh::Kv8* out) {
     const std::string f(fn);
     if (!kv) return fail(c, MGH_ERR_ARG, f + ": null cache");
@@ -1300,19 +1305,55 @@ int mgh_attn_masked(mgh_ctx* c, const void* q, const void* k, const void* v, int
     if (!aligned_to(q, eb) || !aligned_to(k, eb) || !aligned_to(v, eb) || !aligned_to(o, 4) || !aligned_to(o16, 2) ||
         !aligned_to(op.d_slopes, 4) || !aligned_to(op.d_prefix, 4) || !aligned_to(op.d_docs, 4))
         return fail(c, MGH_ERR_ARG, "attn_masked: pointers must be aligned to their elements");
-    if (H > 65535 || B > 65535 || Sk > (1 << 24) || (int64_t)Sq * (H / Hkv) > (1 << 24))
-        return fail(c, MGH_ERR_UNSUPPORTED, "attn_masked: at most 65535 heads and sequences, 2^24 keys and rows of a key head");
+    if (H > 65535 || B > 65535 || Sk > (1 << 24) || (int64_t)Sq * (H / Hkv) > (1 << 24) ||
+        (int64_t)Hkv * B * (((int64_t)Sq * (H / Hkv) + 63) / 64) >= (1 << 22))
+        return fail(c, MGH_ERR_UNSUPPORTED, "attn_masked: at most 65535 heads and sequences, 2^24 keys and rows of a key head, "
+                                            "2^22 tiles of 64 rows");
     mgh::MaskedAttnArgs a{};
     a.q = q; a.k = k; a.v = v; a.o = o; a.o16 = (_Float16*)o16;
     for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.kvst[i] = kvst ? kvst[i] : 0;
     const int64_t packed[4] = {1, D, (int64_t)D * Sq, (int64_t)D * Sq * H};
     for (int i = 0; i < 4; i++) a.ost[i] = ost ? ost[i] : packed[i];
     a.D = D; a.Sq = Sq; a.Sk = Sk; a.H = H; a.Hkv = Hkv; a.B = B;
-    a.in16 = in_f16 != 0; a.causal = op.causal != 0;
+    a.causal = op.causal != 0;
     a.mod = mgh::score_mod(scale, op.cap);
     a.slopes = op.d_slopes; a.prefix = op.d_prefix; a.docs = op.d_docs; a.doc_stride = op.doc_stride;
+    a.vec_o = o16 ? rows_aligned(o16, a.ost, 4, 8) : rows_aligned(o, a.ost, 4, 16);
     if (int r = set_dev(c)) return r;
-    MGH_HIP(c, mgh::launch_attn_masked(a, c->stream), "k_attn_masked");
+    // rows that the kernel does not take as they are go through fp16 copies in the scratch
+    mgh::PackArgs p{};
+    p.D = D; p.B = B; p.in16 = in_f16 != 0;
+    const bool pack_q = !in_f16 || !rows_aligned(q, a.qst, 8, 16);
+    const bool pack_kv = Sk && (!in_f16 || !rows_aligned(k, a.kvst, 8, 16) || !rows_aligned(v, a.kvst, 8, 16) ||
+                                a.kvst[1] < 0 || a.kvst[1] >= (1 << 24));
+    const size_t q_b = pack_q ? round256((size_t)B * H * Sq * D * 2) : 0, kv_b = pack_kv ? round256((size_t)B * Hkv * Sk * D * 2) : 0;
+    if (q_b + kv_b) {
+        if ((int64_t)(q_b + kv_b) > ((int64_t)1 << 36)) return fail(c, MGH_ERR_UNSUPPORTED, "attn_masked: too many rows to pack");
+        if (int r = ensure_scratch(c, q_b + 2 * kv_b)) return r;
+        char* at = (char*)c->scratch;
+        auto view = [&](const void* src, int64_t* st, int S, int heads) {
+            auto& w = p.v[p.n++];
+            w.src = src; w.dst = (_Float16*)at; w.S = S; w.H = heads;
+            for (int i = 0; i < 4; i++) w.st[i] = st[i];
+            w.vec = !in_f16 && rows_aligned(src, st, 4, 16);
+            at += round256((size_t)B * heads * S * D * 2);
+            return (const void*)w.dst;
+        };
+        if (pack_q) a.q = view(q, a.qst, Sq, H);
+        if (pack_kv) a.k = view(k, a.kvst, Sk, Hkv), a.v = view(v, a.kvst, Sk, Hkv);
+        MGH_HIP(c, mgh::launch_attn_pack(p, c->stream), "k_attn_pack");
+        const int64_t qs[4] = {1, D, (int64_t)Sq * D, (int64_t)H * Sq * D}, ks[4] = {1, D, (int64_t)Sk * D, (int64_t)Hkv * Sk * D};
+        for (int i = 0; i < 4; i++) {
+            if (pack_q) a.qst[i] = qs[i];
+            if (pack_kv) a.kvst[i] = ks[i];
+        }
+    }
+    const mgh::MaskedPlan plan = mgh::masked_plan(a);
+    if (plan.ws_bytes) {
+        if (int r = ensure_qp_ws(c, plan.ws_bytes)) return r;
+        a.ws = (float*)c->qp_ws;
+    }
+    MGH_HIP(c, mgh::launch_attn_masked(a, plan, c->stream), "k_attn_masked");
     return MGH_OK;
 }
 

@@ -289,21 +289,51 @@ inline ScoreMod score_mod(float scale, float cap) {
     return {scale * kLog2e, cap > 0.f ? (float)(2.0 * scale * 1.4426950408889634 / cap) : 0.f, cap > 0.f ? cap * kLog2e : 0.f};
 }
 struct MaskedAttnArgs {
-    const void* q;         // fp16 (in16) or fp32 views, element strides for d, s, h, b
+    const void* q;         // fp16 rows, 16-byte aligned, features in order; element strides for d, s, h, b
     const void* k;
     const void* v;
     float* o;              // one of o and o16
     _Float16* o16;
+    float* ws;             // MaskedPlan::ws_bytes
     int64_t qst[4], kvst[4], ost[4];
     int D, Sq, Sk, H, Hkv, B;
-    bool in16, causal;
+    bool causal;
+    bool vec_o;            // 4 features of an output row: one aligned store
     ScoreMod mod;
     const float* slopes;   // [H] or null
     const int32_t* prefix; // [B] or null
     const int32_t* docs;   // [B] rows of Sk ids, doc_stride apart, or null
     int64_t doc_stride;
 };
-hipError_t launch_attn_masked(const MaskedAttnArgs& a, hipStream_t s);
+struct MaskedPlan {
+    int qt, splits;        // 16-row tiles per wave, parts that a head's keys are taken in
+    size_t ws_bytes;       // the parts' states
+};
+MaskedPlan masked_plan(const MaskedAttnArgs& a);
+hipError_t launch_attn_masked(const MaskedAttnArgs& a, const MaskedPlan& p, hipStream_t s);
+hipError_t launch_attn_masked_wide(const MaskedAttnArgs& a, const MaskedPlan& p, hipStream_t s);    // D > 64
+// views of any type and strides -> fp16 [B][H][S][D]
+struct PackArgs {
+    struct View {
+        const void* src;
+        _Float16* dst;
+        int64_t st[4];
+        int S, H;
+        bool vec;          // fp32 rows of aligned 16-byte pieces
+    } v[3];
+    int n, D, B;
+    bool in16;
+};
+hipError_t launch_attn_pack(const PackArgs& p, hipStream_t s);
+// partial rows [splits][rows][D], then [splits][rows] (reference, sum); row = ((b Hkv + hk) R + r), r = G i + g
+struct JoinArgs {
+    const float* ws;
+    float* o;
+    _Float16* o16;
+    int64_t ost[4], rows, R;
+    int G, Hkv, D, splits;
+};
+hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s);
 
 // The 8-bit cache (include/mgh.h has the layout)
 constexpr int kKvBlock = 32, kKvRing = 64;
