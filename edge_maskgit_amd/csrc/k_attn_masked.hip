@@ -38,34 +38,51 @@ __global__ __launch_bounds__(256) void k_attn_pack(PackArgs p) {
     *(f16x8*)(v.dst + row * p.D + d) = x;
 }
 
-// one wave per row: the parts' states, joined in their order
+// One workgroup per row: the parts' states joined. The weights 2^(m_s - m) go to LDS, then 8 groups of 32
+// threads, 4 features each, take every eighth part and add up in order.
 __global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
+    __shared__ float w[kMostSplits], red[8];
+    __shared__ __attribute__((aligned(16))) float part[8][128];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int64_t row = blockIdx.x;
     const f32x2* ml = (const f32x2*)(a.ws + a.splits * a.rows * a.D);
+    if (ml[row][1] < 0.f) return;            // not a sequence's row
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; s++) m = fmaxf(m, ml[s * a.rows + row][0]);
-    float l = 0.f, o[2] = {0.f, 0.f};
-    for (int s = 0; s < a.splits; s++) {
-        const f32x2 x = ml[s * a.rows + row];
-        const float w = x[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - m);
-        if (x[1] == 0.f) continue;
-        l = fmaf(w, x[1], l);
+    for (int s = tid; s < a.splits; s += 256) m = fmaxf(m, ml[s * a.rows + row][0]);
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (lane + 64 * i < a.D) o[i] = fmaf(w, a.ws[(s * a.rows + row) * a.D + lane + 64 * i], o[i]);
+    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+    if ((tid & 63) == 0) red[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float l = 0.f;
+    for (int s = tid; s < a.splits; s += 256) {
+        const f32x2 x = ml[s * a.rows + row];
+        w[s] = x[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - m);
+        l = fmaf(w[s], x[1], l);
     }
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i);
+    if ((tid & 63) == 0) red[4 + wave] = l;
+    __syncthreads();
+    l = red[4] + red[5] + red[6] + red[7];
+    const int grp = tid >> 5, d = 4 * (tid & 31);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (d < a.D)
+#pragma unroll 4
+        for (int s = grp; s < a.splits; s += 8)
+            if (w[s] != 0.f) o += *(const f32x4*)(a.ws + (s * a.rows + row) * a.D + d) * w[s];
+    *(f32x4*)&part[grp][d] = o;
+    __syncthreads();
+    if (tid >= 32 || d >= a.D) return;
+    for (int i = 1; i < 8; i++) o += *(const f32x4*)&part[i][d];
     const int64_t hb = row / a.R;
     const int r = (int)(row - hb * a.R), i = r / a.G, g = r - i * a.G;
     const int64_t ro = hb / a.Hkv * a.ost[3] + (hb % a.Hkv * a.G + g) * a.ost[2] + i * a.ost[1];
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int d = lane + 64 * x;
-        if (d >= a.D) continue;
+    for (int x = 0; x < 4; x++) {
         const float v = l == 0.f ? 0.f : o[x] / l;
-        if (a.o16) a.o16[ro + d * a.ost[0]] = (_Float16)v;
-        else a.o[ro + d * a.ost[0]] = v;
+        if (a.o16) a.o16[ro + (d + x) * a.ost[0]] = (_Float16)v;
+        else a.o[ro + (d + x) * a.ost[0]] = v;
     }
 }
 
@@ -79,7 +96,7 @@ hipError_t launch_attn_pack(const PackArgs& p, hipStream_t s) {
 }
 
 hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)a.rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

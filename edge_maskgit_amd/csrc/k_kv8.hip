@@ -1,4 +1,4 @@
-// k_kv8.hip — the 8-bit key / value cache: writing it, reading it back, attention over it (gfx950).
+// k_kv8.hip — the 8-bit key / value cache: writing it and reading it back (gfx950).
 //
 // A sequence's tokens lie in blocks of 32; block i of sequence b is page table[b][i] of the pool. Per
 // block and head K and V have one scale each, d = fp32(max|x| / 127), and every value is the code
@@ -8,33 +8,11 @@
 // codes once its 32 tokens are there, from their fp16 values, which a ring of 64 tokens per sequence and
 // head keeps until then; so the cache does not depend on how tokens were grouped into calls, no code
 // is ever rescaled, and a sequence may be shortened by up to 32 tokens.
-#include "k_attn_row.h"
+#include "k_kv8.h"
 
 namespace mgh {
 
 namespace {
-
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-// tokens of sequence b before and after a call's new ones; false: numbers that the cache cannot hold
-__device__ __forceinline__ bool spans(const Kv8& c, const int32_t* lens, const int32_t* fresh, int S, int b, int& len,
-                                      int& total) {
-    len = lens[b];
-    const int n = fresh ? fresh[b] : S;
-    const int64_t t = (int64_t)len + n;
-    total = (int)t;
-    return len >= 0 && n >= 0 && n <= S && t <= (int64_t)c.max_blocks * kKvBlock;
-}
-
-// the page of a sequence's block, or -1
-__device__ __forceinline__ int64_t page_of(const Kv8& c, int b, int block) {
-    const int64_t p = c.table[b * c.table_stride + block];
-    return p >= 0 && p < c.pages ? p : -1;
-}
-
-// V's codes of a block: the 8 tokens of a matrix instruction's operand of one feature side by side, two
-// features in 16 bytes
-__device__ __forceinline__ int v_at(int t, int d) { return ((d >> 1) * 4 + (t >> 3)) * 16 + (d & 1) * 8 + (t & 7); }
 
 __device__ __forceinline__ uint32_t code_of(_Float16 x, float d, float id) {
     const float a = fabsf((float)x), f = floorf(a * id);
@@ -162,65 +140,6 @@ __global__ void k_kv8_advance(int32_t* lens, const int32_t* fresh, int B, int S)
     if (b < B) lens[b] += fresh ? fresh[b] : S;      // (32-bit wrap-around lands on a length that every call refuses)
 }
 
-struct CacheSrc {
-    const Kv8& c;
-    int b, hk, cut;        // tokens before `cut` are in whole blocks
-    int64_t p;
-    __device__ bool seen(int64_t j) const { return j <= p; }
-    __device__ float dot(int64_t j, const float* qs) const {
-        float s = 0.f;
-        if (j < cut) {
-            const int64_t page = page_of(c, b, (int)(j / kKvBlock));
-            if (page < 0) return __builtin_nanf("");
-            const uint8_t* k = c.k + ((page * c.Hkv + hk) * kKvBlock + j % kKvBlock) * c.D;
-            for (int d = 0; d < c.D; d++) s = fmaf(qs[d], (float)((int)k[d] - 128), s);
-            return s * c.scales[(page * c.Hkv + hk) * 2];
-        }
-        const _Float16* k = c.k_tail + (((int64_t)b * c.Hkv + hk) * kKvRing + j % kKvRing) * c.D;
-        for (int d = 0; d < c.D; d++) s = fmaf(qs[d], (float)k[d], s);
-        return s;
-    }
-    __device__ float value(int64_t j, int d) const {
-        if (j < cut) {
-            const int64_t page = page_of(c, b, (int)(j / kKvBlock));
-            if (page < 0) return __builtin_nanf("");
-            const int64_t at = page * c.Hkv + hk;
-            return (float)((int)c.v[at * kKvBlock * c.D + v_at((int)(j % kKvBlock), d)] - 128) * c.scales[2 * at + 1];
-        }
-        return (float)c.v_tail[(((int64_t)b * c.Hkv + hk) * c.D + d) * kKvRing + j % kKvRing];
-    }
-};
-
-__global__ __launch_bounds__(256) void k_kv8_attn(Kv8AttnArgs a) {
-    __shared__ float qs[4][128], pl[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, D = a.c.D;
-    const int h = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.c.Hkv);
-    const int i = blockIdx.x * 4 + wave;
-    int len, total;
-    const bool fits = spans(a.c, a.lens, a.fresh, a.S, b, len, total);
-    if (i >= (fits ? total - len : a.S)) return;
-    const int64_t qe = b * a.qst[3] + h * a.qst[2] + i * a.qst[1];
-    for (int d = lane; d < D; d += 64) {
-        const int64_t e = qe + d * a.qst[0];
-        qs[wave][d] = a.in16 ? (float)((const _Float16*)a.q)[e] : (float)(_Float16)((const float*)a.q)[e];
-    }
-    __builtin_amdgcn_wave_barrier();
-    const int64_t p = (int64_t)len + i;
-    RowState st{0.f, 1.f, {__builtin_nanf(""), __builtin_nanf("")}};
-    if (fits) {
-        const CacheSrc src{a.c, b, hk, total & ~(kKvBlock - 1), p};
-        st = attn_row(src, a.mod, a.slopes ? a.slopes[h] * kLog2e : 0.f, p, 0, total, D, qs[wave], pl[wave], lane);
-    }
-    const int64_t oe = b * a.ost[3] + h * a.ost[2] + i * a.ost[1];
-    for (int t = 0; t < 2; t++) {
-        const int d = lane + 64 * t;
-        if (d >= D) continue;
-        const float o = st.l == 0.f ? 0.f : st.o[t] / st.l;
-        if (a.o16) a.o16[oe + d * a.ost[0]] = (_Float16)o;
-        else a.o[oe + d * a.ost[0]] = o;
-    }
-}
-
 }  // namespace
 
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t s) {
@@ -238,11 +157,6 @@ hipError_t launch_kv8_read(const Kv8ReadArgs& a, hipStream_t s) {
 
 hipError_t launch_kv8_advance(int32_t* lens, const int32_t* fresh, int B, int S, hipStream_t s) {
     hipLaunchKernelGGL(k_kv8_advance, dim3((unsigned)((B + 255) / 256)), dim3(256), 0, s, lens, fresh, B, S);
-    return hipGetLastError();
-}
-
-hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(k_kv8_attn, dim3((unsigned)((a.S + 3) / 4), (unsigned)a.H, (unsigned)a.c.B), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -1417,8 +1417,16 @@ int mgh_kv8_attn(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const
     a.mod = mgh::score_mod(scale, cap);
     const int64_t packed[4] = {1, kv->D, (int64_t)kv->D * S, (int64_t)kv->D * S * H};
     for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.ost[i] = ost ? ost[i] : packed[i];
+    a.vec_q = in_f16 && rows_aligned(q, qst, 8, 16);
+    const mgh::Kv8Plan plan = mgh::kv8_plan(a);
+    if ((int64_t)plan.tiles * plan.splits * kv->Hkv * kv->B >= (1 << 24))
+        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn: shape too large");
     if (int r = set_dev(c)) return r;
-    MGH_HIP(c, mgh::launch_kv8_attn(a, c->stream), "k_kv8_attn");
+    if (plan.ws_bytes) {
+        if (int r = ensure_qp_ws(c, plan.ws_bytes)) return r;
+        a.ws = (float*)c->qp_ws;
+    }
+    MGH_HIP(c, mgh::launch_kv8_attn(a, plan, c->stream), "k_kv8_attn");
     return MGH_OK;
 }
 

@@ -333,6 +333,7 @@ struct JoinArgs {
     int64_t ost[4], rows, R;
     int G, Hkv, D, splits;
 };
+constexpr int kMostSplits = 1024;
 hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s);
 
 // The 8-bit cache (include/mgh.h has the layout)
@@ -382,8 +383,15 @@ struct Kv8AttnArgs {
     const int32_t* fresh;
     ScoreMod mod;
     const float* slopes;
+    bool vec_q;            // fp16 rows, 16-byte aligned, features in order
+    float* ws;             // Kv8Plan::ws_bytes
 };
-hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t s);
+struct Kv8Plan {
+    int qt, tiles, splits; // 16-row tiles per workgroup, workgroups along a head's rows, parts of a sequence
+    size_t ws_bytes;
+};
+Kv8Plan kv8_plan(const Kv8AttnArgs& a);
+hipError_t launch_kv8_attn(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s);
 
 // Penalties, bias and grammar mask on logits (k_logits.hip)
 struct LogitsArgs {

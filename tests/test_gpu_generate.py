@@ -457,7 +457,11 @@ def test_cache_holds_infinities_as_nan(ctx):
             clean = Cache(dev, 1, 2, 32, 4, np.random.default_rng(0))
             clean.append(k[:, :99], v[:, :99], [0])
             want = clean.attend(q, lens, new)
-            assert np.array_equal(got[0, :2], want[0, :2]) and np.array_equal(got[0, 2, 1], want[0, 2, 1])
+            # rows may be taken by another path there, whose weights are not rounded to fp16: each within its
+            # bound of the 64-bit value, so within twice the bound of one another
+            tol, rel = (2 * x for x in ref.bound(q, k, v, 32 ** -0.5, out16=True))
+            close(got[0, :2], want[0, :2], tol, rel)
+            close(got[0, 2, 1], want[0, 2, 1], tol, rel)
             assert not np.isfinite(got[0, 2, 0, 3]) and np.isfinite(got[0, 2, 0, 4])
             v2 = v.copy()
             v2[0, 40, 1, 3] = bad
@@ -465,7 +469,8 @@ def test_cache_holds_infinities_as_nan(ctx):
             rk, rv = c.read([99], 99)
             assert np.isnan(rv[0, 1, 32:64]).all() and np.isfinite(rv[0, 0]).all() and np.isfinite(rk).all()
             got = c.attend(q, lens, new)
-            assert np.array_equal(got[0, :, 0], want[0, :, 0]) and np.isnan(got[0, :, 1]).all()
+            close(got[0, :, 0], want[0, :, 0], tol, rel)
+            assert np.isnan(got[0, :, 1]).all()
 
 
 def test_cache_refuses_bad_numbers_on_the_device(ctx):
