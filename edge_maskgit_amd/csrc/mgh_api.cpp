@@ -1382,6 +1382,7 @@ int mgh_kv8_append(mgh_ctx* c, const mgh_kv8* kv, const void* k, const void* v, 
         return fail(c, MGH_ERR_ARG, "kv8_append: pointers must be aligned to their elements");
     a.k = k; a.v = v; a.S = S; a.lens = lens; a.fresh = fresh; a.in16 = in_f16 != 0;
     for (int i = 0; i < 4; i++) a.st[i] = st[i];
+    a.vec = rows_aligned(k, st, in_f16 ? 8 : 4, 16) && rows_aligned(v, st, in_f16 ? 8 : 4, 16);
     if (int r = set_dev(c)) return r;
     MGH_HIP(c, mgh::launch_kv8_append(a, c->stream), "k_kv8_append");
     return MGH_OK;
@@ -1443,6 +1444,7 @@ int mgh_kv8_read(mgh_ctx* c, const mgh_kv8* kv, const int32_t* first, int n, con
         return fail(c, MGH_ERR_ARG, "kv8_read: pointers must be aligned to their elements");
     a.first = first; a.lens = lens; a.n = n;
     a.k = k; a.v = v; a.k16 = (_Float16*)k16; a.v16 = (_Float16*)v16;
+    a.vec = aligned16(k) && aligned16(v) && aligned16(k16) && aligned16(v16);
     if (int r = set_dev(c)) return r;
     MGH_HIP(c, mgh::launch_kv8_read(a, c->stream), "k_kv8_read");
     return MGH_OK;
@@ -1458,7 +1460,7 @@ int mgh_logits_process(mgh_ctx* c, const void* x, int f16, int64_t xs, int rows,
     if (op.max_hist < 0 || op.hist_stride < 0 || op.bias_stride < 0 || op.allowed_stride < 0)
         return fail(c, MGH_ERR_ARG, "logits_process: negative history, bias or mask size");
     if (rows == 0 || V == 0) return MGH_OK;
-    if (V > (1 << 30) || (int64_t)rows * ((V + 4095) / 4096) >= (1 << 24))
+    if (V > (1 << 30) || (int64_t)rows * ((V + mgh::kLogitsChunk - 1) / mgh::kLogitsChunk) >= (1 << 24))
         return fail(c, MGH_ERR_UNSUPPORTED, "logits_process: shape too large");
     if (!x || !y) return fail(c, MGH_ERR_ARG, "logits_process: null pointer");
     if (rows > 1 && (xs < V || ys < V)) return fail(c, MGH_ERR_ARG, "logits_process: rows must be at least V apart");

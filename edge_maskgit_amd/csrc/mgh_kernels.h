@@ -357,6 +357,7 @@ struct Kv8AppendArgs {
     const int32_t* fresh;  // [B] new tokens, or null: S
     int S;
     bool in16;
+    bool vec;              // rows of aligned 16-byte pieces, features in order
 };
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t s);
 struct Kv8ReadArgs {
@@ -368,6 +369,7 @@ struct Kv8ReadArgs {
     float* v;
     _Float16* k16;
     _Float16* v16;
+    bool vec;              // 16-byte aligned outputs
 };
 hipError_t launch_kv8_read(const Kv8ReadArgs& a, hipStream_t s);
 hipError_t launch_kv8_advance(int32_t* lens, const int32_t* fresh, int B, int S, hipStream_t s);
@@ -412,6 +414,7 @@ struct LogitsArgs {
     const uint32_t* allowed;
     int64_t allowed_stride;
 };
+constexpr int kLogitsChunk = 2048;      // tokens per workgroup
 hipError_t launch_logits_process(const LogitsArgs& a, hipStream_t s);
 
 size_t noalloc_scratch_bytes();
