@@ -21,6 +21,8 @@
 // A masked key's weight is 0, but 0 times an infinity or NaN of V is not: rows that come out not finite are
 // taken again by attn_row, which reads what a row sees and nothing else.
 #pragma once
+#include <type_traits>
+
 #include "k_attn_row.h"
 
 namespace mgh {
@@ -53,22 +55,31 @@ struct MaskedSrc {
     __device__ float value(int64_t j, int d) const { return (float)v[j * stride + d]; }
 };
 
-// XOR of a 16-byte piece's place in its LDS row: 8 rows of a score operand's pieces, and the 4 rows x 2
-// pieces of a transposing read, fall on different banks
+// XOR of a 16-byte piece's place in its LDS row. 256 bytes of LDS are read at a time: two pieces side by side of
+// 8 rows (a transposing read), or a score operand's pieces of 16 lanes, which are not consecutive lanes: rows
+// 0-3 and 12-15 of one piece with rows 4-11 of the next. With it they fall on different banks, whether 256
+// bytes are one row, two or four. (SQ_LDS_BANK_CONFLICT: 0; by 8 rows of 128 bytes, half of the LDS cycles.)
 template <int PPR>
 __device__ __forceinline__ int piece_swz(int r) {
-    return PPR >= 8 ? 2 * (r & 3) + ((r >> 2) & 1) : 2 * ((r >> 1) & 1) + ((r >> 2) & 1);
+    const int h = (r >> 3) & 1;
+    return 2 * (PPR == 16 ? (r & 7) ^ 4 * h : PPR == 8 ? ((r >> 1) & 3) ^ 2 * h : ((r >> 2) & 1) ^ h) + h;
 }
 
 // DC 16-feature chunks (D <= 16 DC), QT 16-row tiles per wave, PS: weights as hi + lo; MOD 0: scores times a
-// positive scale, 1: any scale and slopes (0: none), 2: capped, then slopes.
+// positive scale, 1: any scale and slopes (0: none), 2: capped, 3: capped, then slopes.
+// The VALU is the busier unit below 128 features and with a cap (per score two exponentials and a reciprocal, at
+// a quarter of its rate), so MOD 0 and 2 keep the raw scores: both maps rise with them, so the maximum is
+// taken raw, and the reference goes into the map's last fma.
+constexpr float kMasked = -3e38f;          // below every raw score (at most 128 65504^2), where -infinity is one
 template <int DC, int QT, bool PS, int MOD>
 __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int tiles, int splits) {
     constexpr int PPR = DC <= 2 ? 4 : DC <= 4 ? 8 : 16;       // 16-byte pieces of an LDS row
     constexpr int KC = (DC + 1) / 2, NT = kMaskKeys / 16, NI = kMaskKeys * PPR / 256;
     constexpr int ROWB = PPR * 16, CH = kMaskKeys * ROWB;     // bytes of an LDS row, of a K or V chunk
     constexpr int WROWS = 16 * QT;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * CH + 2 * kMaskKeys * 4];
+    // two objects, so that the compiler can tell a chunk's reads from the next one's loads (with one it waits for
+    // those before the first read); K, V, the ids of documents
+    __shared__ __attribute__((aligned(1024))) char lds0[2 * CH + kMaskKeys * 4], lds1[2 * CH + kMaskKeys * 4];
     __shared__ uint32_t bits[2][kMaskScan / 32];              // chunks that some row sees; that all rows see all of
     __shared__ int range[3][4];
 
@@ -126,13 +137,25 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
         __syncthreads();
         for (int w = 0; w < 4; w++) lo = min(lo, range[0][w]), hi = max(hi, range[1][w]), all &= range[2][w];
         all = all && lo == hi;
-        for (int c = c0 + wave; c < c1; c += 4) {
-            const int j = c * kMaskKeys + lane;
-            const int x = j < a.Sk ? docs[j] : -1;
-            const bool some = __any(x >= lo && x <= hi), whole = __all(x == hi || j >= a.Sk) && all;
-            if (lane == 0 && some) {
-                atomicOr(&bits[0][(c - c0) >> 5], 1u << ((c - c0) & 31));
-                if (whole) atomicOr(&bits[1][(c - c0) >> 5], 1u << ((c - c0) & 31));
+        // 8 chunks' ids at once; each wave takes 8 of 32 chunks, a byte of the noted bits
+        for (int w0 = c0 + 8 * wave; w0 < c1; w0 += 32) {
+            int x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int j = (w0 + k) * kMaskKeys + lane;
+                x[k] = j < a.Sk ? docs[j] : -1;
+            }
+            uint32_t some = 0, whole = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (w0 + k < c1 && __any(x[k] >= lo && x[k] <= hi)) {
+                    some |= 1u << k;
+                    if (all && __all(x[k] == hi || (w0 + k) * kMaskKeys + lane >= a.Sk)) whole |= 1u << k;
+                }
+            }
+            if (lane == 0) {
+                ((uint8_t*)bits[0])[(w0 - c0) >> 3] = (uint8_t)some;
+                ((uint8_t*)bits[1])[(w0 - c0) >> 3] = (uint8_t)whole;
             }
         }
         __syncthreads();
@@ -157,7 +180,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
         const int n = 256 * u + tid, r = n / PPR, p = (n % PPR) ^ piece_swz<PPR>(r);
         src[u] = 8 * p < a.D ? r * rowb + 16 * p : 0x80000000u;
     }
-    auto stage = [&](int c, int buf) {
+    auto stage = [&](int c, auto bufc) {
+        constexpr int buf = decltype(bufc)::value;
         const int left = a.Sk - c * kMaskKeys;               // rows from this chunk on, >= 1
         const uint32_t ext = (uint32_t)(min(left, kMaskKeys) - 1) * rowb + 2 * a.D;
         const int64_t at = kv0 + (int64_t)c * kMaskKeys * a.kvst[1];
@@ -165,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
             return __builtin_amdgcn_make_buffer_rsrc((void*)((const _Float16*)p + at), (short)0, (int)ext, 0x00020000);
         };
         const __amdgpu_buffer_rsrc_t rk = rsrc(a.k), rv = rsrc(a.v);
-        char* B = lds + buf * 2 * CH + wave * 1024;
+        char* B = (buf ? lds1 : lds0) + wave * 1024;
 #pragma unroll
         for (int u = 0; u < NI; u++) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(B + 4096 * u), 16, (int)src[u], 0, 0, 0);
@@ -174,18 +198,18 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
         if (docs && wave == 0) {
             const __amdgpu_buffer_rsrc_t rd =
                 __builtin_amdgcn_make_buffer_rsrc((void*)(docs + c * kMaskKeys), (short)0, 4 * min(left, kMaskKeys), 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (lds_void*)(lds + 4 * CH + buf * 4 * kMaskKeys), 4, 4 * lane, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (lds_void*)((buf ? lds1 : lds0) + 2 * CH), 4, 4 * lane, 0, 0, 0);
         }
     };
     // where this lane reads: K row l16 of a tile, pieces 4 c + lg; V rows 4 lg + l16 / 4 (of 16), 4 features at
     // 16 c + 4 (l16 % 4)
-    uint32_t ka[2], va[4];
+    uint32_t ka[KC], va[DC];
 #pragma unroll
-    for (int c = 0; c < 2; c++) ka[c] = l16 * ROWB + (((4 * c + lg) ^ piece_swz<PPR>(l16)) & (PPR - 1)) * 16;
+    for (int c = 0; c < KC; c++) ka[c] = l16 * ROWB + ((4 * c + lg) ^ piece_swz<PPR>(l16)) * 16;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
+    for (int c = 0; c < DC; c++) {
         const int r = 4 * lg + (l16 >> 2), p = 2 * c + ((l16 & 3) >> 1);
-        va[c] = r * ROWB + ((p ^ piece_swz<PPR>(r)) & (PPR - 1)) * 16 + 8 * (l16 & 1);
+        va[c] = r * ROWB + (p ^ piece_swz<PPR>(r)) * 16 + 8 * (l16 & 1);
     }
 
     float mref[QT], S1[QT];
@@ -200,16 +224,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
     const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     const float scale2 = a.mod.scale2;
 
-    int buf = 0;
-    int c = find(c0);
-    if (c < c1) stage(c, 0);
-    while (c < c1) {
+    // one chunk, in the buffer that is a constant of the call; returns the next one
+    auto step = [&](auto bufc, int c) {
+        constexpr int buf = decltype(bufc)::value;
         const int cn = find(c + 1);
         stage_sync<0>();                     // this buffer is filled, the other one no longer read
-        if (cn < c1) stage(cn, buf ^ 1);
+        if (cn < c1) stage(cn, std::integral_constant<int, buf ^ 1>{});
         const int k0 = c * kMaskKeys;
         if (k0 <= w_hi) {
-            const char* K = lds + buf * 2 * CH;
+            const char* K = (buf ? lds1 : lds0);
             const char* V = K + CH;
             const bool same = !docs || (scan && (__builtin_amdgcn_readfirstlane(bits[1][(c - c0) >> 5]) >> ((c - c0) & 31) & 1));
             f32x4 sc[QT][NT];
@@ -217,7 +240,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
             for (int n = 0; n < NT; n++) {
                 f16x8 kf[KC];
 #pragma unroll
-                for (int i = 0; i < KC; i++) kf[i] = *(const f16x8*)(K + ka[i & 1] + 128 * (i >> 1) + 16 * n * ROWB);
+                for (int i = 0; i < KC; i++) kf[i] = *(const f16x8*)(K + ka[i] + 16 * n * ROWB);
 #pragma unroll
                 for (int t = 0; t < QT; t++) {
                     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -226,31 +249,33 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     sc[t][n] = acc;
                 }
             }
-            if (MOD) {
+            if (MOD & 1) {
 #pragma unroll
                 for (int t = 0; t < QT; t++)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            const float x = MOD == 2 ? cap_score(sc[t][n][r], a.mod) : sc[t][n][r] * scale2;
+                            const float x = MOD == 3 ? cap_score(sc[t][n][r], a.mod) : sc[t][n][r] * scale2;
                             sc[t][n][r] = fmaf(-slope2[t], fabsf(pos[t] - (float)(k0 + 16 * n + 4 * lg + r)), x);
                         }
             }
             // the results are in their registers before a branch looks at them
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
-            if (k0 + kMaskKeys - 1 > w_lo) {
+            constexpr float kHidden = MOD == 2 ? kMasked : -INFINITY;
+            const bool edge = k0 + kMaskKeys - 1 > w_lo, part = edge || !same;
+            if (edge) {
 #pragma unroll
                 for (int t = 0; t < QT; t++)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int r = 0; r < 4; r++)
-                            if (k0 + 16 * n + 4 * lg + r > lim[t]) sc[t][n][r] = -INFINITY;
+                            if (k0 + 16 * n + 4 * lg + r > lim[t]) sc[t][n][r] = kHidden;
             }
             if (!same) {
-                const int32_t* ids = (const int32_t*)(lds + 4 * CH + buf * 4 * kMaskKeys);
+                const int32_t* ids = (const int32_t*)((buf ? lds1 : lds0) + 2 * CH);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     const i32x4 id = *(const i32x4*)(ids + 16 * n + 4 * lg);
@@ -258,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     for (int t = 0; t < QT; t++)
 #pragma unroll
                         for (int r = 0; r < 4; r++)
-                            if (id[r] != doc[t] || doc[t] < 0) sc[t][n][r] = -INFINITY;
+                            if (id[r] != doc[t] || doc[t] < 0) sc[t][n][r] = kHidden;
                 }
             }
             float mx[QT];
@@ -271,7 +296,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     v = fmaxf(fmaxf(v, sc[t][n][0]), sc[t][n][1]);
                     v = fmaxf(fmaxf(v, sc[t][n][2]), sc[t][n][3]);
                 }
-                mx[t] = MOD ? v : v * scale2;
+                mx[t] = MOD == 2 ? (v == kMasked ? -INFINITY : cap_score(v, a.mod)) : MOD ? v : v * scale2;
                 up[t] = __any(mx[t] > mref[t] + 15.f);
                 any = any || up[t];
             }
@@ -288,9 +313,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     for (int cc = 0; cc < DC; cc++) O[t][cc] *= al;
                 }
             }
+            float top[QT];
             f32x4 s1[QT], oc[QT][DC];
 #pragma unroll
             for (int t = 0; t < QT; t++) {
+                top[t] = a.mod.cap2 - mref[t];
                 s1[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int cc = 0; cc < DC; cc++) oc[t][cc] = PS ? f32x4{0.f, 0.f, 0.f, 0.f} : O[t][cc];
@@ -304,7 +331,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const float s = sc[t][2 * p + j / 4][j % 4];
-                        e[j] = __builtin_amdgcn_exp2f(MOD ? s - mref[t] : fmaf(s, scale2, -mref[t]));
+                        if (MOD == 2) {
+                            const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.mod.cap_in) + 1.f);
+                            e[j] = __builtin_amdgcn_exp2f(fmaf(x, -2.f * a.mod.cap2, top[t]));
+                        } else {
+                            e[j] = __builtin_amdgcn_exp2f(MOD ? s - mref[t] : fmaf(s, scale2, -mref[t]));
+                        }
+                    }
+                    if (MOD == 2 && part) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) e[j] = sc[t][2 * p + j / 4][j % 4] == kMasked ? 0.f : e[j];
                     }
                     u32x4 hi, lo;
 #pragma unroll
@@ -321,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                 }
 #pragma unroll
                 for (int cc = 0; cc < DC; cc++) {
-                    const char* at = V + va[cc & 3] + 128 * (cc >> 2) + 32 * p * ROWB;
+                    const char* at = V + va[cc] + 32 * p * ROWB;
                     const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
                     const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * ROWB));
                     const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -344,13 +380,19 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                 for (int cc = 0; cc < DC; cc++) O[t][cc] = PS ? O[t][cc] + oc[t][cc] : oc[t][cc];
             }
         }
-        c = cn;
-        buf ^= 1;
+        return cn;
+    };
+    int c = find(c0);
+    if (c < c1) stage(c, std::integral_constant<int, 0>{});
+    while (c < c1) {
+        c = step(std::integral_constant<int, 0>{}, c);
+        if (c >= c1) break;
+        c = step(std::integral_constant<int, 1>{}, c);
     }
 
     // rows that are not finite: again, key by key
     __syncthreads();
-    float* qs = (float*)lds + wave * 256;
+    float* qs = (float*)lds0 + wave * 256;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         float z = S1[t];
@@ -426,7 +468,9 @@ template <int DC, int QT, bool PS>
 hipError_t launch_masked_t(const MaskedAttnArgs& a, int splits, hipStream_t s) {
     const int tiles = (int)(((int64_t)a.Sq * (a.H / a.Hkv) + 64 * QT - 1) / (64 * QT));
     const dim3 grid((unsigned)((int64_t)tiles * splits * a.Hkv * a.B));
-    if (a.mod.cap2 != 0.f) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
+    if (a.mod.cap2 != 0.f && (a.slopes || !(a.mod.cap_in > 0.f)))
+        hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 3>), grid, dim3(256), 0, s, a, tiles, splits);
+    else if (a.mod.cap2 != 0.f) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
     else if (a.slopes || !(a.mod.scale2 > 0.f)) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 1>), grid, dim3(256), 0, s, a, tiles, splits);
     else hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 0>), grid, dim3(256), 0, s, a, tiles, splits);
     return hipGetLastError();

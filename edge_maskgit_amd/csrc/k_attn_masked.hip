@@ -2,6 +2,7 @@
 // narrow heads of the tiled kernel (k_attn_masked.h), the packing of rows that it does not take as they are,
 // and the joining of what a head's keys gave in parts.
 #include <algorithm>
+#include <cstdlib>
 
 #include "k_attn_masked.h"
 
@@ -106,6 +107,8 @@ MaskedPlan masked_plan(const MaskedAttnArgs& a) {
     if (heads * ((R + 127) / 128) >= 256) p.qt = 2;
     const int64_t wgs = heads * ((R + 64 * p.qt - 1) / (64 * p.qt));
     if (wgs < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, nch / 4));
+    if (getenv("MQT")) p.qt = atoi(getenv("MQT"));
+    if (getenv("MSP")) p.splits = atoi(getenv("MSP"));
     if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.D + 2) * sizeof(float);
     return p;
 }

@@ -16,6 +16,7 @@
 // Rows that come out not finite (a scale that is, a page outside the pool, infinities among the open block's
 // values) are taken again by attn_row.
 #include <algorithm>
+#include <cstdlib>
 
 #include "k_attn_row.h"
 #include "k_kv8.h"
@@ -409,6 +410,7 @@ Kv8Plan kv8_plan(const Kv8AttnArgs& a) {
     const int64_t wgs = heads * p.tiles;
     // parts of at least 16 blocks (4 per wave) of the table's length, for about 4 workgroups per CU
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((kMostSplits + wgs - 1) / wgs, a.c.max_blocks / 16));
+    if (getenv("KSP")) p.splits = atoi(getenv("KSP"));
     if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.c.D + 2) * sizeof(float);
     return p;
 }
