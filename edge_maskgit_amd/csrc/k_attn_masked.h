@@ -235,18 +235,23 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
             const char* K = (buf ? lds1 : lds0);
             const char* V = K + CH;
             const bool same = !docs || (scan && (__builtin_amdgcn_readfirstlane(bits[1][(c - c0) >> 5]) >> ((c - c0) & 31) & 1));
+            // scores, a tile of 16 keys after the other, K's next operands read into the registers just used; this wave's
+            // products before another's softmax (piece of 512 x 12345, two waves per SIMD: 239 -> 231 us)
             f32x4 sc[QT][NT];
+            f16x8 kf[KC];
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < KC; i++) kf[i] = *(const f16x8*)(K + ka[i]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                f16x8 kf[KC];
 #pragma unroll
-                for (int i = 0; i < KC; i++) kf[i] = *(const f16x8*)(K + ka[i] + 16 * n * ROWB);
+                for (int i = 0; i < KC; i++) {
 #pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < KC; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf[t][i], acc, 0, 0, 0);
-                    sc[t][n] = acc;
+                    for (int t = 0; t < QT; t++)
+                        sc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qf[t][i], i ? sc[t][n] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    if (n + 1 < NT) kf[i] = *(const f16x8*)(K + ka[i] + 16 * (n + 1) * ROWB);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (MOD & 1) {
@@ -260,6 +265,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                             sc[t][n][r] = fmaf(-slope2[t], fabsf(pos[t] - (float)(k0 + 16 * n + 4 * lg + r)), x);
                         }
             }
+            __builtin_amdgcn_s_setprio(0);
             // the results are in their registers before a branch looks at them
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
@@ -313,7 +319,38 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     for (int cc = 0; cc < DC; cc++) O[t][cc] *= al;
                 }
             }
+            // weights of keys 32 p .. 32 p + 31 of row tile t, as the operand of P V
             float top[QT];
+            f16x8 ph[2][QT], pl[2][QT];
+            auto weights = [&](int p, int t) {
+                float e[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float x = sc[t][2 * p + j / 4][j % 4];
+                    if (MOD == 2) {
+                        const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.mod.cap_in) + 1.f);
+                        e[j] = __builtin_amdgcn_exp2f(fmaf(r, -2.f * a.mod.cap2, top[t]));
+                    } else {
+                        e[j] = __builtin_amdgcn_exp2f(MOD ? x - mref[t] : fmaf(x, scale2, -mref[t]));
+                    }
+                }
+                if (MOD == 2 && part) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) e[j] = sc[t][2 * p + j / 4][j % 4] == kMasked ? 0.f : e[j];
+                }
+                u32x4 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const f16x2 h = __builtin_convertvector((f32x2{e[2 * j], e[2 * j + 1]}), f16x2);
+                    hi[j] = __builtin_bit_cast(uint32_t, h);
+                    if (PS) {
+                        const f32x2 d = {e[2 * j] - (float)h[0], e[2 * j + 1] - (float)h[1]};
+                        lo[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, f16x2));
+                    }
+                }
+                ph[p][t] = __builtin_bit_cast(f16x8, hi);
+                if (PS) pl[p][t] = __builtin_bit_cast(f16x8, lo);
+            };
             f32x4 s1[QT], oc[QT][DC];
 #pragma unroll
             for (int t = 0; t < QT; t++) {
@@ -321,56 +358,51 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                 s1[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int cc = 0; cc < DC; cc++) oc[t][cc] = PS ? f32x4{0.f, 0.f, 0.f, 0.f} : O[t][cc];
+                weights(0, t);
             }
+            // V's operands are read AHEAD of their products (else each pair of products waits for its read); the weights
+            // of the second half are made among the products of the first
+            constexpr int AHEAD = DC < 4 ? DC : 4, M = QT * (PS ? 2 : 1);
+            f16x8 vf[AHEAD];
+            auto load_v = [&](int x) {               // operand x: half x / DC, features 16 (x % DC)
+                const char* at = V + va[x % DC] + 32 * (x / DC) * ROWB;
+                const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * ROWB));
+                vf[x % AHEAD] = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
 #pragma unroll
-            for (int p = 0; p < NT / 2; p++) {
-                f16x8 ph[QT], pl[QT];
+            for (int x = 0; x < AHEAD; x++) load_v(x);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    float e[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float s = sc[t][2 * p + j / 4][j % 4];
-                        if (MOD == 2) {
-                            const float x = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.mod.cap_in) + 1.f);
-                            e[j] = __builtin_amdgcn_exp2f(fmaf(x, -2.f * a.mod.cap2, top[t]));
-                        } else {
-                            e[j] = __builtin_amdgcn_exp2f(MOD ? s - mref[t] : fmaf(s, scale2, -mref[t]));
-                        }
-                    }
-                    if (MOD == 2 && part) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) e[j] = sc[t][2 * p + j / 4][j % 4] == kMasked ? 0.f : e[j];
-                    }
-                    u32x4 hi, lo;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const f16x2 h = __builtin_convertvector((f32x2{e[2 * j], e[2 * j + 1]}), f16x2);
-                        hi[j] = __builtin_bit_cast(uint32_t, h);
-                        if (PS) {
-                            const f32x2 d = {e[2 * j] - (float)h[0], e[2 * j + 1] - (float)h[1]};
-                            lo[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, f16x2));
-                        }
-                    }
-                    ph[t] = __builtin_bit_cast(f16x8, hi);
-                    if (PS) pl[t] = __builtin_bit_cast(f16x8, lo);
-                }
+            for (int p = 0; p < 2; p++) {
 #pragma unroll
                 for (int cc = 0; cc < DC; cc++) {
-                    const char* at = V + va[cc] + 32 * p * ROWB;
-                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * ROWB));
-                    const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    const int x = p * DC + cc;
 #pragma unroll
                     for (int t = 0; t < QT; t++) {
-                        if (PS) oc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t], oc[t][cc], 0, 0, 0);
-                        oc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t], oc[t][cc], 0, 0, 0);
+                        if (PS) oc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[x % AHEAD], pl[p][t], oc[t][cc], 0, 0, 0);
+                        oc[t][cc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[x % AHEAD], ph[p][t], oc[t][cc], 0, 0, 0);
                     }
+                    if (x + AHEAD < 2 * DC) load_v(x + AHEAD);
+                    if (p == 0 && cc < QT) weights(1, cc);
+                    if (p) __builtin_amdgcn_sched_barrier(0);
+                }
+                if (p == 0) {                        // a product, vector operations, ..., two reads
+#pragma unroll
+                    for (int i = 0; i < DC; i++) {
+#pragma unroll
+                        for (int m = 0; m < M; m++) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, QT * (MOD == 2 ? 56 : 22) / (DC * M) + 1, 0);
+                        }
+                        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int t = 0; t < QT; t++) {
-                    if (PS) s1[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t], s1[t], 0, 0, 0);
-                    s1[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[t], s1[t], 0, 0, 0);
+                    if (PS) s1[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[p][t], s1[t], 0, 0, 0);
+                    s1[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[p][t], s1[t], 0, 0, 0);
                 }
             }
 #pragma unroll

@@ -2,7 +2,6 @@
 // narrow heads of the tiled kernel (k_attn_masked.h), the packing of rows that it does not take as they are,
 // and the joining of what a head's keys gave in parts.
 #include <algorithm>
-#include <cstdlib>
 
 #include "k_attn_masked.h"
 
@@ -39,7 +38,50 @@ __global__ __launch_bounds__(256) void k_attn_pack(PackArgs p) {
     *(f16x8*)(v.dst + row * p.D + d) = x;
 }
 
-// One workgroup per row: the parts' states joined. The weights 2^(m_s - m) go to LDS, then 8 groups of 32
+// a joined row's features d .. d + N - 1
+template <int N>
+__device__ __forceinline__ void put_row(const JoinArgs& a, int64_t row, int d, const float* o, float l) {
+    const int64_t hb = row / a.R;
+    const int r = (int)(row - hb * a.R), i = r / a.G, g = r - i * a.G;
+    const int64_t ro = hb / a.Hkv * a.ost[3] + (hb % a.Hkv * a.G + g) * a.ost[2] + i * a.ost[1];
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        const float v = l == 0.f ? 0.f : o[x] / l;
+        if (a.o16) a.o16[ro + (d + x) * a.ost[0]] = (_Float16)v;
+        else a.o[ro + (d + x) * a.ost[0]] = v;
+    }
+}
+
+// Few parts: one wave per row, 2 features a lane; nothing waits for another wave.
+__global__ __launch_bounds__(256) void k_attn_join_few(JoinArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const f32x2* ml = (const f32x2*)(a.ws + a.splits * a.rows * a.D);
+    f32x2 st[kFewSplits], part[kFewSplits];
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) st[s] = s < a.splits ? ml[s * a.rows + row] : f32x2{-INFINITY, 0.f};
+    if (st[0][1] < 0.f) return;              // not a sequence's row
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) {   // (a part that saw nothing wrote no values)
+        part[s] = f32x2{0.f, 0.f};
+        if (s < a.splits && st[s][1] != 0.f && 2 * lane < a.D) part[s] = *(const f32x2*)(a.ws + (s * a.rows + row) * a.D + 2 * lane);
+    }
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) m = fmaxf(m, st[s][0]);
+    f32x2 o = {0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) {
+        const float w = st[s][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[s][0] - m);
+        l = fmaf(w, st[s][1], l);
+        o += part[s] * w;
+    }
+    const float v[2] = {o[0], o[1]};
+    if (2 * lane < a.D) put_row<2>(a, row, 2 * lane, v, l);
+}
+
+// Many: one workgroup per row, the parts' states joined. The weights 2^(m_s - m) go to LDS, then 8 groups of 32
 // threads, 4 features each, take every eighth part and add up in order.
 __global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
     __shared__ float w[kMostSplits], red[8];
@@ -76,15 +118,8 @@ __global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
     __syncthreads();
     if (tid >= 32 || d >= a.D) return;
     for (int i = 1; i < 8; i++) o += *(const f32x4*)&part[i][d];
-    const int64_t hb = row / a.R;
-    const int r = (int)(row - hb * a.R), i = r / a.G, g = r - i * a.G;
-    const int64_t ro = hb / a.Hkv * a.ost[3] + (hb % a.Hkv * a.G + g) * a.ost[2] + i * a.ost[1];
-#pragma unroll
-    for (int x = 0; x < 4; x++) {
-        const float v = l == 0.f ? 0.f : o[x] / l;
-        if (a.o16) a.o16[ro + (d + x) * a.ost[0]] = (_Float16)v;
-        else a.o[ro + (d + x) * a.ost[0]] = v;
-    }
+    const float v[4] = {o[0], o[1], o[2], o[3]};
+    put_row<4>(a, row, d, v, l);
 }
 
 }  // namespace
@@ -97,7 +132,8 @@ hipError_t launch_attn_pack(const PackArgs& p, hipStream_t s) {
 }
 
 hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(k_attn_join, dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    if (a.splits <= kFewSplits) hipLaunchKernelGGL(k_attn_join_few, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(k_attn_join, dim3((unsigned)a.rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -106,9 +142,7 @@ MaskedPlan masked_plan(const MaskedAttnArgs& a) {
     MaskedPlan p{1, 1, 0};
     if (heads * ((R + 127) / 128) >= 256) p.qt = 2;
     const int64_t wgs = heads * ((R + 64 * p.qt - 1) / (64 * p.qt));
-    if (wgs < 256) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, nch / 4));
-    if (getenv("MQT")) p.qt = atoi(getenv("MQT"));
-    if (getenv("MSP")) p.splits = atoi(getenv("MSP"));
+    if (wgs < 384) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / wgs, nch / 4));
     if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.D + 2) * sizeof(float);
     return p;
 }

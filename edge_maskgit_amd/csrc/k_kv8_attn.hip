@@ -16,7 +16,6 @@
 // Rows that come out not finite (a scale that is, a page outside the pool, infinities among the open block's
 // values) are taken again by attn_row.
 #include <algorithm>
-#include <cstdlib>
 
 #include "k_attn_row.h"
 #include "k_kv8.h"
@@ -71,7 +70,7 @@ __device__ __forceinline__ f16x8 widen(uint32_t a, uint32_t b) {
 
 // DG 32-feature groups (D <= 32 DG), QT 16-row tiles, PS: weights as hi + lo, MOD: capped or sloped
 template <int DG, int QT, bool PS, bool MOD>
-__global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a, int tiles, int splits) {
+__global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a, int tiles, int splits, int least) {
     constexpr int DK = (DG + 1) / 2, ROWS = 16 * QT, OLD = 32 * DG + 4;
     __shared__ __attribute__((aligned(16))) float so[4][ROWS][OLD];
     __shared__ float sm[4][ROWS][2];
@@ -79,8 +78,9 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
     const Kv8& cache = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lg = lane >> 4, D = cache.D;
-    const int hb = blockIdx.x / (tiles * splits), in_h = blockIdx.x - hb * (tiles * splits);
-    const int tile = in_h / splits, sp = in_h - tile * splits;
+    // heads innermost, so that each XCD (blockIdx % 8) gets as many of the first parts, which every sequence has
+    const int heads = cache.Hkv * cache.B, hb = blockIdx.x % heads, in_h = blockIdx.x / heads;
+    const int sp = in_h / tiles, tile = in_h - sp * tiles;
     const int hk = hb % cache.Hkv, b = hb / cache.Hkv, G = a.H / cache.Hkv;
     int len, total;
     const bool fits = spans(cache, a.lens, a.fresh, a.S, b, len, total);
@@ -92,7 +92,12 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
     const int whole = fits ? total / kKvBlock : 0, cut = whole * kKvBlock;
     const int last = r0 < R ? len + (min(r0 + ROWS, R) - 1) / G : -1;       // the last row's position
     const int nb = fits && r0 < R ? min((total + kKvBlock - 1) / kKvBlock, last / kKvBlock + 1) : 0;
-    const int per = (nb + splits - 1) / splits, b0 = min(sp * per, nb), b1 = min(b0 + per, nb);
+    const int per = max((nb + splits - 1) / splits, least), b0 = min(sp * per, nb), b1 = min(b0 + per, nb);
+
+    // rows past the sequence's own: marked for the joining kernel, which leaves them alone; a part without blocks: 0
+    if (splits > 1 && tid < ROWS && r0 + tid < RS && (r0 + tid >= R || b0 >= b1))
+        *(f32x2*)(ml + 2 * (sp * rows + row0 + r0 + tid)) = f32x2{-1e30f, r0 + tid >= R ? -1.f : 0.f};
+    if (splits > 1 && b0 >= b1 && fits) return;
 
     // rows of Q as the B operand: features 64 g + 16 lg + 8 j + e
     f16x8 qf[QT][2 * DK];
@@ -228,25 +233,26 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         }
     };
 
-    // this wave's whole blocks b0 + wave, + 4, ..., two sets of registers in turn. ids: the pages of 64 of them
+    // this wave's whole blocks b0 + wave, + 4, ..., two sets of registers in turn. Every load is made, past the last
+    // block that one's again and for a page outside the pool page 0's: behind a branch around them the compiler
+    // could not count the loads and would wait for all. ids: the pages of 64 of the blocks
     struct Set {
         u32x4 k[2 * DK], v[DG];
         f32x2 s;
-        bool ok;
     };
-    const int w1 = min(b1, whole);
-    bool lost = false;                   // a page outside the pool
+    const int w1 = min(b1, whole), w0 = b0 + wave;
+    bool lost = w0 < w1 && cache.pages == 0;         // a page outside the pool
     int ids = 0, id0 = 0;
     auto load = [&](int blk, Set& x) {
-        if (blk >= w1) return;
-        if (blk == b0 + wave || blk - id0 >= 256) {
+        blk = min(blk, w0 + (w1 - 1 - w0) / 4 * 4);
+        if (blk == w0 || blk - id0 >= 256) {
             id0 = blk;
             ids = blk + 4 * lane < w1 ? cache.table[b * cache.table_stride + blk + 4 * lane] : 0;
         }
-        const int64_t page = __builtin_amdgcn_readlane(ids, (blk - id0) >> 2);
-        x.ok = page >= 0 && page < cache.pages;
-        if (!x.ok) return;
-        const int64_t at = page * cache.Hkv + hk;
+        const int id = __builtin_amdgcn_readlane(ids, (blk - id0) >> 2);
+        const bool in = id >= 0 && id < cache.pages;
+        lost = lost || !in;
+        const int64_t at = (int64_t)(in ? id : 0) * cache.Hkv + hk;
         const uint8_t* K = cache.k + at * kKvBlock * D;
         const uint8_t* V = cache.v + at * kKvBlock * D;
 #pragma unroll
@@ -259,22 +265,20 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         x.s = *(const f32x2*)(cache.scales + 2 * at);
     };
     auto use = [&](int blk, const Set& x) {
-        if (!x.ok) {
-            lost = true;
-            return;
-        }
         block(blk, x.s[0], x.s[1],
               [&](int n, int c) { const u32x4 w = x.k[2 * (c >> 1) + n]; return c & 1 ? widen(w[2], w[3]) : widen(w[0], w[1]); },
               [&](int c) { const u32x4 w = x.v[c >> 1]; return c & 1 ? widen(w[2], w[3]) : widen(w[0], w[1]); });
     };
-    Set A, B;
-    load(b0 + wave, A);
-    for (int blk = b0 + wave; blk < w1; blk += 8) {
-        load(blk + 4, B);
-        use(blk, A);
-        if (blk + 4 >= w1) break;
-        load(blk + 8, A);
-        use(blk + 4, B);
+    if (w0 < w1 && cache.pages) {
+        Set A, B;
+        load(w0, A);
+        for (int blk = w0; blk < w1; blk += 8) {
+            load(blk + 4, B);
+            use(blk, A);
+            if (blk + 4 >= w1) break;
+            load(blk + 8, A);
+            use(blk + 4, B);
+        }
     }
     // the open block
     if (b1 > whole && b0 <= whole && ((whole - b0) & 3) == wave) {
@@ -378,25 +382,23 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         if (4 * lane < D) put(r0 + r, 4 * lane, *(const f32x4*)&qs[4 * lane], st.m == -INFINITY ? -1e30f : st.m, st.l);
         __builtin_amdgcn_wave_barrier();
     }
-    // rows past the sequence's own: marked for the joining kernel, which leaves them alone
-    if (splits > 1 && tid < ROWS && r0 + tid >= R && r0 + tid < RS) ml[2 * (sp * rows + row0 + r0 + tid) + 1] = -1.f;
 }
 
 template <int DG, int QT, bool PS>
-void launch_cache_t(const Kv8AttnArgs& a, int tiles, int splits, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)tiles * splits * a.c.Hkv * a.c.B));
-    if (a.mod.cap2 != 0.f || a.slopes) hipLaunchKernelGGL((k_kv8_attn<DG, QT, PS, true>), grid, dim3(256), 0, s, a, tiles, splits);
-    else hipLaunchKernelGGL((k_kv8_attn<DG, QT, PS, false>), grid, dim3(256), 0, s, a, tiles, splits);
+void launch_cache_t(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)p.tiles * p.splits * a.c.Hkv * a.c.B));
+    if (a.mod.cap2 != 0.f || a.slopes) hipLaunchKernelGGL((k_kv8_attn<DG, QT, PS, true>), grid, dim3(256), 0, s, a, p.tiles, p.splits, p.least);
+    else hipLaunchKernelGGL((k_kv8_attn<DG, QT, PS, false>), grid, dim3(256), 0, s, a, p.tiles, p.splits, p.least);
 }
 
 template <int DG>
 void launch_cache_d(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s) {
     if (p.qt == 2) {
-        if (a.o16) launch_cache_t<DG, 2, false>(a, p.tiles, p.splits, s);
-        else launch_cache_t<DG, 2, true>(a, p.tiles, p.splits, s);
+        if (a.o16) launch_cache_t<DG, 2, false>(a, p, s);
+        else launch_cache_t<DG, 2, true>(a, p, s);
     } else {
-        if (a.o16) launch_cache_t<DG, 1, false>(a, p.tiles, p.splits, s);
-        else launch_cache_t<DG, 1, true>(a, p.tiles, p.splits, s);
+        if (a.o16) launch_cache_t<DG, 1, false>(a, p, s);
+        else launch_cache_t<DG, 1, true>(a, p, s);
     }
 }
 
@@ -408,9 +410,16 @@ Kv8Plan kv8_plan(const Kv8AttnArgs& a) {
     p.qt = R > 16 ? 2 : 1;
     p.tiles = (int)((R + 16 * p.qt - 1) / (16 * p.qt));
     const int64_t wgs = heads * p.tiles;
-    // parts of at least 16 blocks (4 per wave) of the table's length, for about 4 workgroups per CU
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((kMostSplits + wgs - 1) / wgs, a.c.max_blocks / 16));
-    if (getenv("KSP")) p.splits = atoi(getenv("KSP"));
+    // Few workgroups: parts until every CU has one, of at least 8 blocks (2 per wave). Enough of them: parts only of
+    // sequences past 96 blocks, for the balance of ragged batches (the table's width is all that the host knows of
+    // their lengths): a second launch costs 5-8 us. Measured (32 heads on 8 of 128 features, one token), parts
+    // 1 / 2 / 3 / 4 / 8 / 32: one sequence of 100000 tokens 631 / 323 / 221 / 169 / 92 / 45 us, one of 9000 68 / 42 / 31 / 27 /
+    // 19 / 14, 16 of 9000 78 / 61 / 68 / 62 / 65 / 74, 64 of 2700 69 / 77 / 74 / 79 / 86 / 105, 64 of up to 8000 98 / 104 / 93 / 93 /
+    // 92 / 114, 64 of up to 500 14 / 22 / 19 / 25 / 20 / 40.
+    const int fill = (int)std::max<int64_t>(1, (256 + wgs - 1) / wgs), least = fill > 1 ? 192 * fill : 96;
+    p.least = fill > 1 ? 8 : 96;
+    p.splits = (int)std::min<int64_t>(kMostSplits, (int64_t)fill * std::max(1, (a.c.max_blocks + least - 1) / least));
+    p.splits = std::max(1, std::min(p.splits, (a.c.max_blocks + p.least - 1) / p.least));
     if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.c.D + 2) * sizeof(float);
     return p;
 }

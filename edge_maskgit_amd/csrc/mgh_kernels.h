@@ -333,7 +333,7 @@ struct JoinArgs {
     int64_t ost[4], rows, R;
     int G, Hkv, D, splits;
 };
-constexpr int kMostSplits = 1024;
+constexpr int kMostSplits = 1024, kFewSplits = 8;
 hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s);
 
 // The 8-bit cache (include/mgh.h has the layout)
@@ -390,6 +390,7 @@ struct Kv8AttnArgs {
 };
 struct Kv8Plan {
     int qt, tiles, splits; // 16-row tiles per workgroup, workgroups along a head's rows, parts of a sequence
+    int least;             // blocks that a part holds before another one is used
     size_t ws_bytes;
 };
 Kv8Plan kv8_plan(const Kv8AttnArgs& a);
