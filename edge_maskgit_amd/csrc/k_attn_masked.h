@@ -160,13 +160,25 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
         }
         __syncthreads();
     }
-    // the next chunk from c on that some row sees, or c1
-    auto find = [&](int c) {
+    // the next chunk from c on that some row sees, or c1; `same`: whether all rows see all of it, as far as documents
+    // go. The bits of 32 chunks at a time stay in scalar registers.
+    uint32_t seen = 0, full = 0;
+    int word = -1;
+    auto find = [&](int c, bool& same) {
+        same = !docs;
         if (!scan) return c;
-        while (c < c1) {
-            const uint32_t w = __builtin_amdgcn_readfirstlane(bits[0][(c - c0) >> 5]) >> ((c - c0) & 31);
-            if (w) return min(c1, c + __builtin_ctz(w));
-            c = c0 + (((c - c0) >> 5) + 1) * 32;
+        for (; c < c1; c = c0 + 32 * (word + 1)) {
+            const int at = (c - c0) >> 5, bit = (c - c0) & 31;
+            if (at != word) {
+                word = at;
+                seen = __builtin_amdgcn_readfirstlane(bits[0][at]);
+                full = __builtin_amdgcn_readfirstlane(bits[1][at]);
+            }
+            if (seen >> bit) {
+                const int n = bit + __builtin_ctz(seen >> bit);
+                same = full >> n & 1;
+                return c0 + 32 * word + n;       // (no bits past c1)
+            }
         }
         return c1;
     };
@@ -225,16 +237,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
     const float scale2 = a.mod.scale2;
 
     // one chunk, in the buffer that is a constant of the call; returns the next one
-    auto step = [&](auto bufc, int c) {
+    auto step = [&](auto bufc, int c, bool& same) {
         constexpr int buf = decltype(bufc)::value;
-        const int cn = find(c + 1);
+        bool next_same;
+        const int cn = find(c + 1, next_same);
         stage_sync<0>();                     // this buffer is filled, the other one no longer read
         if (cn < c1) stage(cn, std::integral_constant<int, buf ^ 1>{});
         const int k0 = c * kMaskKeys;
         if (k0 <= w_hi) {
             const char* K = (buf ? lds1 : lds0);
             const char* V = K + CH;
-            const bool same = !docs || (scan && (__builtin_amdgcn_readfirstlane(bits[1][(c - c0) >> 5]) >> ((c - c0) & 31) & 1));
             // scores, a tile of 16 keys after the other, K's next operands read into the registers just used; this wave's
             // products before another's softmax (piece of 512 x 12345, two waves per SIMD: 239 -> 231 us)
             f32x4 sc[QT][NT];
@@ -412,14 +424,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                 for (int cc = 0; cc < DC; cc++) O[t][cc] = PS ? O[t][cc] + oc[t][cc] : oc[t][cc];
             }
         }
+        same = next_same;
         return cn;
     };
-    int c = find(c0);
+    bool same;
+    int c = find(c0, same);
     if (c < c1) stage(c, std::integral_constant<int, 0>{});
     while (c < c1) {
-        c = step(std::integral_constant<int, 0>{}, c);
+        c = step(std::integral_constant<int, 0>{}, c, same);
         if (c >= c1) break;
-        c = step(std::integral_constant<int, 1>{}, c);
+        c = step(std::integral_constant<int, 1>{}, c, same);
     }
 
     // rows that are not finite: again, key by key

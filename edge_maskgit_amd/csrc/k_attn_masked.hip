@@ -137,10 +137,18 @@ hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Two row tiles per wave (each operand read from LDS serves both) where they still give a workgroup per CU: 128
+// features, 32 heads of 4097 tokens 334 against 374 us for one. Up to 64 features the LDS is no bound and the gain is
+// small (unmasked 184 / 197 us), while rows that see unlike numbers of keys are better shared out in smaller
+// pieces (causal 117 / 108, nine documents 85 / 78) and capped scores wait for the VALU anyway (280 / 274): one.
+// Too few workgroups for two per CU: the keys in parts (512 x 12345, 256 workgroups: one part 243 us, two 214; one
+// token over 8000 keys, 64 workgroups: 1 / 2 / 4 / 8 parts 253 / 136 / 78 / 56 us), of at least 4 chunks (257 tokens, 80
+// workgroups of 5 chunks: 12 us whole, 19 in two parts).
 MaskedPlan masked_plan(const MaskedAttnArgs& a) {
     const int64_t R = (int64_t)a.Sq * (a.H / a.Hkv), heads = (int64_t)a.Hkv * a.B, nch = (a.Sk + kMaskKeys - 1) / kMaskKeys;
     MaskedPlan p{1, 1, 0};
-    if (heads * ((R + 127) / 128) >= 256) p.qt = 2;
+    const bool even = !a.causal && !a.docs && a.mod.cap2 == 0.f;
+    if (heads * ((R + 127) / 128) >= 256 && (a.D > 64 || even)) p.qt = 2;
     const int64_t wgs = heads * ((R + 64 * p.qt - 1) / (64 * p.qt));
     if (wgs < 384) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / wgs, nch / 4));
     if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.D + 2) * sizeof(float);
