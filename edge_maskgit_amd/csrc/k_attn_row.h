@@ -13,10 +13,17 @@ namespace mgh {
 
 // The score in log2 units from q . k. tanh(x) = 1 - 2 / (exp(2x) + 1): exp2 of an overflowing argument
 // is inf (its reciprocal 0: +cap), of an underflowing one 0 (-cap). The hardware's exp2 and reciprocal
-// are 1 ulp off; near zero the difference costs an absolute 1.2e-7 cap.
+// are 1 ulp off; near zero the difference costs an absolute 1.2e-7 cap, so with large caps |x| < 1/4 takes
+// tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 (what is left out: 8e-9 of it).
 __device__ __forceinline__ float cap_score(float s, const ScoreMod& m) {
     const float e = __builtin_amdgcn_exp2f(s * m.cap_in);
-    return fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * m.cap2, m.cap2);
+    float y = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * m.cap2, m.cap2);
+    if (m.cap_x != 0.f) {
+        const float x = s * m.cap_x, z = x * x;
+        const float p = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+        y = fabsf(x) < 0.25f ? m.cap2 * x * p : y;
+    }
+    return y;
 }
 
 // A row's partial result: weights relative to 2^m

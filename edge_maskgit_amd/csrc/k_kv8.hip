@@ -50,8 +50,8 @@ __device__ __forceinline__ void load_row(const void* p, int64_t e, int64_t st, _
 // NaN above infinity: a block that holds either has that scale, and all its values come out NaN.
 // The ring: each workgroup stores the new ones of its tokens, unless the call touches more than two blocks and the
 // first one's earlier tokens are still in the ring, where the third block's slots are theirs: then the first
-// workgroup stores all, after its reads. Four prompts of 2050 tokens, 8 heads of 128, 50 MB: 16.9 us without the ring, 17.1 with
-// it, 22.8 by the first workgroup alone.
+// workgroup stores all, after its reads. Four prompts of 2050 tokens, 8 heads of 128, 50 MB: 17.6 us, 22.8 where
+// the first workgroup stores all (16.9 without a ring).
 template <bool IN16, bool VEC>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
     __shared__ uint32_t mx[2][4];

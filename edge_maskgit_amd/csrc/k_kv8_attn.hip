@@ -101,13 +101,12 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
 
     // rows of Q as the B operand: features 64 g + 16 lg + 8 j + e
     f16x8 qf[QT][2 * DK];
-    float pos[QT], slope2[QT];
+    float slope2[QT];
     int lim[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const int r = min(r0 + 16 * t + l16, RS - 1), i = r / G, g = r - i * G;
         lim[t] = r0 + 16 * t + l16 < R ? len + i : -1;
-        pos[t] = (float)lim[t];
         slope2[t] = MOD && a.slopes ? a.slopes[hk * G + g] * kLog2e : 0.f;
         const int64_t e = b * a.qst[3] + (int64_t)(hk * G + g) * a.qst[2] + i * a.qst[1];
 #pragma unroll
@@ -176,7 +175,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
                     float s = sc[t][n][r] * scale;
                     if (MOD) {
                         if (a.mod.cap2 != 0.f) s = cap_score(s, a.mod);
-                        s = fmaf(-slope2[t], fabsf(pos[t] - (float)(j0 + 4 * n + r)), s);
+                        s = fmaf(-slope2[t], (float)(lim[t] - (j0 + 4 * n + r)), s);     // (of the keys that it sees)
                     }
                     s = j0 + 4 * n + r > lim[t] ? -INFINITY : s;
                     sc[t][n][r] = s;
@@ -419,6 +418,8 @@ Kv8Plan kv8_plan(const Kv8AttnArgs& a) {
     const int fill = (int)std::max<int64_t>(1, (256 + wgs - 1) / wgs), least = fill > 1 ? 192 * fill : 96;
     p.least = fill > 1 ? 8 : 96;
     p.splits = (int)std::min<int64_t>(kMostSplits, (int64_t)fill * std::max(1, (a.c.max_blocks + least - 1) / least));
+    // (a table far wider than its sequences: no more than 8 workgroups per CU, most of them without blocks)
+    p.splits = (int)std::min<int64_t>(p.splits, std::max<int64_t>(1, 2048 / wgs));
     p.splits = std::max(1, std::min(p.splits, (a.c.max_blocks + p.least - 1) / p.least));
     if (p.splits > 1) p.ws_bytes = (size_t)p.splits * heads * R * (a.c.D + 2) * sizeof(float);
     return p;

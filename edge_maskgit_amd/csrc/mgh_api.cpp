@@ -1241,6 +1241,9 @@ int check_scores(mgh_ctx* c, const char* fn, int D, int H, int Hkv, float scale,
     if (D <= 0 || D % 16 || D > 128) return fail(c, MGH_ERR_UNSUPPORTED, f + ": D must be a multiple of 16 up to 128");
     if (!(scale - scale == 0.f)) return fail(c, MGH_ERR_ARG, f + ": scale must be finite");
     if (!(cap >= 0.f) || cap - cap != 0.f) return fail(c, MGH_ERR_ARG, f + ": cap must be finite and >= 0");
+    const mgh::ScoreMod m = mgh::score_mod(scale, cap);
+    if (m.scale2 - m.scale2 != 0.f || m.cap_in - m.cap_in != 0.f || m.cap2 - m.cap2 != 0.f)
+        return fail(c, MGH_ERR_ARG, f + ": scale or cap is past what fp32 scores can hold");
     if ((o != nullptr) == (o16 != nullptr)) return fail(c, MGH_ERR_ARG, f + ": exactly one of d_o and d_o16 is needed");
     return MGH_OK;
 }
@@ -1276,7 +1279,7 @@ int check_kv8(mgh_ctx* c, const char* fn, const mgh_kv8* kv, mgh::Kv8* out) {
 int check_step(mgh_ctx* c, const char* fn, int S, const int32_t* lens, const int32_t* fresh) {
     const std::string f(fn);
     if (S < 0) return fail(c, MGH_ERR_ARG, f + ": negative number of tokens");
-    if (S > (1 << 29)) return fail(c, MGH_ERR_UNSUPPORTED, f + ": at most 2^29 tokens");
+    if (S > (1 << 28)) return fail(c, MGH_ERR_UNSUPPORTED, f + ": at most 2^28 tokens");
     if (!lens) return fail(c, MGH_ERR_ARG, f + ": null lengths");
     if (!aligned_to(lens, 4) || !aligned_to(fresh, 4)) return fail(c, MGH_ERR_ARG, f + ": lengths must be 4-byte aligned");
     return MGH_OK;
@@ -1328,7 +1331,7 @@ int mgh_attn_masked(mgh_ctx* c, const void* q, const void* k, const void* v, int
                                 a.kvst[1] < 0 || a.kvst[1] >= (1 << 24));
     const size_t q_b = pack_q ? round256((size_t)B * H * Sq * D * 2) : 0, kv_b = pack_kv ? round256((size_t)B * Hkv * Sk * D * 2) : 0;
     if (q_b + kv_b) {
-        if ((int64_t)(q_b + kv_b) > ((int64_t)1 << 36)) return fail(c, MGH_ERR_UNSUPPORTED, "attn_masked: too many rows to pack");
+        if (q_b > ((size_t)1 << 35) || kv_b > ((size_t)1 << 35)) return fail(c, MGH_ERR_UNSUPPORTED, "attn_masked: too many rows to pack");
         if (int r = ensure_scratch(c, q_b + 2 * kv_b)) return r;
         char* at = (char*)c->scratch;
         auto view = [&](const void* src, int64_t* st, int S, int heads) {

@@ -277,16 +277,21 @@ hipError_t launch_group_norm(const float* x, int64_t W, int64_t H, int C, int N,
                              const float* gamma, const float* beta, float* y, void* ws, hipStream_t s);
 hipError_t launch_upscale(const float* x, int IW, int IH, int64_t CN, int f, float* y, hipStream_t s);
 
-// Attention under masks and over the 8-bit cache (k_attn_masked.hip, k_kv8.hip). Scores become log2
+// Attention under masks and over the 8-bit cache (k_attn_masked.hip, k_kv8_attn.hip). Scores become log2
 // units: s scale2, or cap2 tanh(s scale / cap) = cap2 (1 - 2 / (exp2(s cap_in) + 1)).
 constexpr float kLog2e = 1.4426950408889634f;
 struct ScoreMod {
     float scale2;          // scale log2(e)
     float cap_in;          // 2 scale log2(e) / cap
     float cap2;            // cap log2(e); 0: not capped
+    float cap_x;           // scale / cap where small arguments of the tanh need their own form, else 0
 };
+// Near zero the quotient's form is off by an absolute 1.2e-7 of the cap, which a cap past 64 no longer hides: from
+// there on small arguments take the series.
+constexpr float kFineCap = 64.f;
 inline ScoreMod score_mod(float scale, float cap) {
-    return {scale * kLog2e, cap > 0.f ? (float)(2.0 * scale * 1.4426950408889634 / cap) : 0.f, cap > 0.f ? cap * kLog2e : 0.f};
+    if (!(cap > 0.f)) return {scale * kLog2e, 0.f, 0.f, 0.f};
+    return {scale * kLog2e, (float)(2.0 * scale * 1.4426950408889634 / cap), cap * kLog2e, cap > kFineCap ? scale / cap : 0.f};
 }
 struct MaskedAttnArgs {
     const void* q;         // fp16 rows, 16-byte aligned, features in order; element strides for d, s, h, b

@@ -436,7 +436,7 @@ int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* 
  *      pool among the blocks a call reads; nothing outside the buffers is touched. Two sequences may
  *      share pages that are whole. A block that holds an infinity or NaN reads as NaN.
  *      D a multiple of 16 up to 128; d_k, d_v and the tails 16-byte, d_scales 8-byte aligned;
- *      max_blocks * 32 and S up to 2^29. */
+ *      max_blocks * 32 up to 2^29, S and n up to 2^28. */
 typedef struct mgh_kv8 {
     void* d_k;
     void* d_v;

@@ -50,7 +50,7 @@ def bound(q, k, v, scale, cap=0.0, slopes=None, out16=False):
 
     Scores: a dot product of D terms in fp32 is off by at most (D + 8) 2^-24 of the sum of its terms'
     magnitudes (the products of fp16 values are exact), the cap's tanh by 8 2^-24 cap (exp2, reciprocal
-    and fma, 1-2 ulp each), and each of the few operations on a score of magnitude S by 2^-24 S. That
+    and fma, 1-2 ulp each; from a cap of 64 on small arguments by their series, 8 2^-24 of the score), and each of the few operations on a score of magnitude S by 2^-24 S. That
     difference is the relative error of a weight, with 2^-20 for its exponential and the 22 bits of it
     that meet v. Sums of n weights and products add n 2^-24. An output is a ratio of such sums: twice
     that, of the largest |v|. With fp16 outputs the weights are rounded to fp16 (2^-11) and the output is
@@ -61,7 +61,7 @@ def bound(q, k, v, scale, cap=0.0, slopes=None, out16=False):
     mag = abs(scale) * (q.reshape(-1, D).max(0) * k.reshape(-1, D).max(0)).sum() if k.size and q.size else 0.0
     far = 0.0 if slopes is None else float(np.abs(slopes).max()) * max(n, q.shape[1])
     top = (min(mag, cap) if cap else mag) + far
-    eps = 2.0 ** -24 * ((D + 8) * mag + 8 * cap + 6 * top + n) + 2.0 ** -20
+    eps = 2.0 ** -24 * ((D + 8) * mag + 8 * (cap if cap <= 64 else min(4 * cap, 4 * mag)) + 6 * top + n) + 2.0 ** -20
     vmax = v.max() if v.size else 0.0
     # (2^-30: outputs below fp16's normal numbers are rounded to multiples of 2^-24)
     return 2 * (eps + (2.0 ** -11 if out16 else 0)) * vmax + (2.0 ** -25 if out16 else 1e-30), 2.0 ** -11 if out16 else 2.0 ** -24

@@ -34,7 +34,7 @@ assert kernels()
 nan = float("nan")
 for kw, what in (({"D": 24}, "D must"), ({"D": 144}, "D must"), ({"D": 0}, "D must"), ({"H": 3, "Hkv": 2}, "H % Hkv"),
                  ({"Hkv": 0}, "H % Hkv"), ({"H": -4}, "H % Hkv"), ({"scale": nan}, "scale"), ({"scale": float("inf")}, "scale"),
-                 ({"cap": -1.0}, "cap"), ({"cap": nan}, "cap"), ({"cap": float("inf")}, "cap"), ({"o16": None}, "exactly one"),
+                 ({"cap": -1.0}, "cap"), ({"cap": nan}, "cap"), ({"cap": float("inf")}, "cap"), ({"cap": 1e-45}, "fp32"), ({"cap": 3e38}, "fp32"), ({"scale": 3e38}, "fp32"), ({"o16": None}, "exactly one"),
                  ({"o": G}, "exactly one"), ({"Sq": -1}, "negative"), ({"Sk": -1}, "negative"), ({"Bn": -1}, "negative"),
                  ({"prefix": R}, "needs causal"), ({"docs": R, "doc_stride": 8}, "doc_stride"), ({"docs": R, "doc_stride": -9}, "doc_stride"),
                  ({"q": None}, "null"), ({"k": None}, "null"), ({"v": None}, "null"), ({"q": W + 1}, "aligned"), ({"o16": Y + 1}, "aligned"),
@@ -74,7 +74,7 @@ for name, f in calls.items():
                      ({"vt": Y + 2}, "aligned"), ({"scales": B + 4}, "aligned"), ({"table": G + 2}, "aligned")):
         refused(f, kv(**kw), what=what)
     refused(f, kv(), S=-1, what="negative")
-    refused(f, kv(), S=2 ** 29 + 1, what="2^29")
+    refused(f, kv(), S=2 ** 28 + 1, what="2^28")
     refused(f, kv(), lens=None, what="null")
     refused(f, kv(), lens=N + 2, what="aligned")
 refused(calls["append"], kv(), k=None, what="null")

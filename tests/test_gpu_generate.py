@@ -177,6 +177,107 @@ def test_masked_attention_scores_of_any_size(ctx):
                 check_masked(ctx, np.abs(q), kk, v, scale=scale, cap=30.0, out16=out16)
 
 
+@pytest.mark.parametrize("cap", [60.0, 70.0, 1e4, 1e8])
+def test_caps_of_any_size(ctx, cap):
+    """scores far below the cap keep their relative accuracy"""
+    rng = np.random.default_rng(14)
+    q, k, v = qkv(rng, 1, 20, 150, 2, 1, 32)
+    for slopes in (None, np.full(2, 0.05, F32)):
+        check_masked(ctx, q, k, v, cap=cap, out16=False, causal=True, slopes=slopes)
+        check_masked(ctx, q, k, v, cap=cap, scale=-0.3, slopes=slopes)
+    with Dev(ctx) as dev:
+        c, q, k, v, have = cache_case(dev, rng, [150], [2], 2, 1, 32)
+        check_cache(c, q, k, v, [150], [2], have, cap=cap, out16=False)
+
+
+@pytest.mark.parametrize("D,G", [(48, 1), (64, 4), (128, 1), (128, 2)])
+@pytest.mark.parametrize("kind", ["full", "docs", "causal", "cap", "slopes"])
+def test_masked_attention_many_rows(ctx, D, G, kind):
+    """enough rows for every plan (two row tiles per wave, several workgroups per CU): some rows against 64 bits"""
+    print(f"many rows {D} {G} {kind}", flush=True)
+    rng = np.random.default_rng(D + G)
+    B, S, Hkv = 4, 1100, 8
+    q, k, v = qkv(rng, B, S, S, Hkv * G, Hkv, D)
+    docs = docs_of(rng, B, S, 4, pad=70)
+    kw = {"docs": {"docs": docs}, "causal": {"causal": True, "prefix": np.array([0, 5, 700, 1100], I32)}, "cap": {"cap": 9.0},
+          "slopes": {"slopes": (0.5 ** np.arange(Hkv * G)).astype(F32)}}.get(kind, {})
+    for out16 in (True, False):
+        got = run_masked(ctx, q, k, v, out16=out16, **kw)
+        assert np.isfinite(got).all()
+        tol, rel = ref.bound(q, k, v, D ** -0.5, kw.get("cap", 0.0), kw.get("slopes"), out16)
+        for i in (0, 63, 64, 127, 128, 500, 1029, 1030, 1099):
+            b, h = int(rng.integers(B)), int(rng.integers(Hkv * G))
+            j = np.arange(S)
+            seen = np.ones(S, bool)
+            if kind == "causal":
+                seen = (j <= i) | (j < kw["prefix"][b])
+            if kind == "docs":
+                seen = (docs[b] == docs[b, i]) & (docs[b] >= 0)
+            sl = kw.get("slopes")
+            want = ref.attention_row(q[b, i, h].astype(F64), k[b, :, h // G].astype(F64), v[b, :, h // G].astype(F64), D ** -0.5,
+                                     kw.get("cap", 0.0), None if sl is None else float(sl[h]), i, seen)
+            close(got[b, i, h], want, tol, rel)
+
+
+def test_masked_attention_a_million_keys(ctx):
+    """more keys than a workgroup notes documents of, and rows in parts of a long sequence"""
+    rng = np.random.default_rng(15)
+    Sq, Sk, D = 26000, 1100000, 16
+    q, k, v = (rng.standard_normal((1, n, 1, D)).astype(F16) for n in (Sq, Sk, Sk))
+    docs = np.sort(rng.integers(0, 30, (1, Sk)).astype(I32), 1)
+    docs[0, -50:] = -1
+    got = run_masked(ctx, q, k, v, docs=docs, causal=True)
+    few = run_masked(ctx, q[:, -60:], k, v, docs=docs, causal=True)
+    tol, rel = ref.bound(q, k, v, D ** -0.5, out16=True)
+    j = np.arange(Sk)
+    for i in (0, 1, 12345, Sq - 60, Sq - 51, Sq - 50, Sq - 1):
+        p = Sk - Sq + i
+        seen = (j <= p) & (docs[0] == docs[0, p]) & (docs[0] >= 0)
+        want = ref.attention_row(q[0, i, 0].astype(F64), k[0, :, 0].astype(F64), v[0, :, 0].astype(F64), D ** -0.5, 0.0, None, p, seen)
+        close(got[0, i, 0], want, tol, rel)
+        if i >= Sq - 60:
+            close(few[0, i - (Sq - 60), 0], want, tol, rel)
+
+
+def _put(ctx, ptr, x):
+    x = np.ascontiguousarray(x)
+    ctx._check(ema.lib().mgh_h2d(ctx.h, ptr, x.ctypes.data, x.nbytes))
+
+
+def test_offsets_past_32_bits(ctx):
+    """rows, sequences and pages whose byte offsets do not fit 32 bits"""
+    rng = np.random.default_rng(16)
+    B, S, H, D = 2, 300, 2, 64
+    q, k, v = qkv(rng, B, S, S, H, H, D)
+    want = run_masked(ctx, q, k, v, causal=True)
+    token, seq = 1 << 22, (1 << 22) * 300 + 64                # 8 MiB between rows, 2.5 GB per sequence
+    with Dev(ctx) as dev:
+        big = ctx.alloc(2 * (seq * B + (1 << 20)))
+        dev.bufs.append(big)
+        for b in range(B):
+            for i in range(S):
+                _put(ctx, big.ptr + 2 * (b * seq + i * token), np.concatenate([q[b, i].ravel(), k[b, i].ravel(), v[b, i].ravel()]))
+        st = (1, token, D, seq)
+        o = dev.up(np.zeros_like(q))
+        ctx.attn_masked(big, big.ptr + 2 * H * D, big.ptr + 4 * H * D, st, st, D, S, S, H, H, B, D ** -0.5, causal=True, o16=o,
+                        o_strides=(1, H * D, D, S * H * D))
+        assert np.array_equal(dev.get(o, q.shape, F16), want)
+    with Dev(ctx) as dev:
+        lens, new, Hkv = [70, 40], [2, 1], 8
+        c, q, k, v, have = cache_case(dev, rng, lens, new, 8, Hkv, 128)
+        want = c.attend(q, lens, new)
+        pages = 80000                                          # 2.6 GB of codes each
+        per = Hkv * 32 * 128
+        dk, dv, ds = ctx.alloc(pages * per), ctx.alloc(pages * per), ctx.alloc(pages * Hkv * 8)
+        dev.bufs += [dk, dv, ds]
+        c.k, c.v, c.scales, c.pages = dk, dv, ds, pages
+        c.set_table((79990 + np.arange(2 * c.nb).reshape(2, c.nb) * 3 % 10).astype(I32))
+        c.append(k[:, :max(have)], v[:, :max(have)], [0, 0], have)
+        assert np.array_equal(c.attend(q, lens, new), want)
+        rk, _ = c.read(have, 72)
+        assert np.array_equal(rk[0, :, :64], ref.cache_values(k[0, :64]).astype(F32).transpose(1, 0, 2))
+
+
 def test_masked_attention_strides(ctx):
     """any strides and alignments give what contiguous rows give: views of a fused row, heads outside
     the tokens, features apart, odd offsets, one row for all sequences, separate output layouts"""
@@ -501,6 +602,55 @@ def test_cache_refuses_bad_numbers_on_the_device(ctx):
             assert np.array_equal(x, y, equal_nan=x.dtype != np.uint8)
         assert np.isnan(c.read([-1, 32 * c.nb + 1, 71, 71], 5)[0][:2]).all()
         assert np.array_equal(c.attend(q, lens, new), want)
+
+
+def test_cache_table_wider_than_the_sequences(ctx):
+    """parts that most sequences have no blocks for, short and long ones in a batch, more rows than a workgroup's"""
+    rng = np.random.default_rng(17)
+    with Dev(ctx) as dev:
+        lens, new = [5, 300, 0, 1700], [1, 1, 1, 1]
+        c, q, k, v, have = cache_case(dev, rng, lens, new, 8, 2, 64, spare=900)
+        check_cache(c, q, k, v, lens, new, have)
+        c, q, k, v, have = cache_case(dev, rng, [400, 90], [40, 30], 8, 2, 128, spare=200)
+        check_cache(c, q, k, v, [400, 90], [40, 30], have, cap=5.0)
+        check_cache(c, q, k, v, [400, 90], [40, 30], have, out16=False, slopes=np.full(8, 0.2, F32))
+
+
+@pytest.mark.parametrize("B,nb", [(64, 8), (64, 300)])
+def test_cache_attention_large_batches(ctx, B, nb):
+    """a workgroup per CU and more, sequences past and below the length that is taken in parts"""
+    rng = np.random.default_rng(nb)
+    Hkv, D, H = 4, 48, 4
+    with Dev(ctx) as dev:
+        lens = rng.integers(0, 32 * nb - 1, B)
+        lens[:2] = 32 * nb - 1, 0
+        pages = B * nb
+        k, v = rng.standard_normal((2, 1, 32 * nb, Hkv, D)).astype(F16)
+        c = Cache(dev, 1, Hkv, D, nb, rng, spare=0)
+        c.append(k, v, [0])
+        # every sequence reads the same pages; its open block is its own
+        table = np.repeat(c.table, B, 0)
+        one = c
+        c = Cache(dev, B, Hkv, D, nb, rng, spare=0)
+        c.k, c.v, c.scales, c.pages = one.k, one.v, one.scales, one.pages
+        tk, tv = np.full((B, Hkv, 64, D), np.nan, F16), np.full((B, Hkv, D, 64), np.nan, F16)
+        for b, n in enumerate(lens):
+            t = np.arange((n + 1) // 32 * 32, n + 1)
+            tk[b][:, t % 64], tv[b][:, :, t % 64] = k[0, t].transpose(1, 0, 2), v[0, t].transpose(1, 2, 0)
+        c.kt, c.vt = dev.up(tk), dev.up(tv)
+        c.set_table(table)
+        q = rng.standard_normal((B, 1, H, D)).astype(F16)
+        got = c.attend(q, lens)
+        whole = ref.cache_values(k[0]), ref.cache_values(v[0])
+        tol, rel = ref.bound(q, whole[0][None], whole[1][None], D ** -0.5, out16=True)
+        for b in list(range(6)) + [B - 1]:
+            n = int(lens[b]) + 1
+            cut = n // 32 * 32
+            kk = np.concatenate([whole[0][:cut], k[0, cut:n].astype(F64)])
+            vv = np.concatenate([whole[1][:cut], v[0, cut:n].astype(F64)])
+            for h in range(H):
+                want = ref.attention_row(q[b, 0, h].astype(F64), kk[:, h], vv[:, h], D ** -0.5, 0.0, None, n - 1, np.ones(n, bool))
+                close(got[b, 0, h], want, tol, rel)
 
 
 def test_cache_pages_shared(ctx):
