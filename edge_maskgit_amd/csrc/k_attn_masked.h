@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
     f32x4 O[QT][DC];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        mref[t] = -1e30f;
+        mref[t] = kNoScore;
         S1[t] = 0.f;
 #pragma unroll
         for (int c = 0; c < DC; c++) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
             qs[lane] = st.o[0], qs[lane + 64] = st.o[1];
             __builtin_amdgcn_wave_barrier();
             if (l16 == l) {
-                mref[t] = st.m == -INFINITY ? -1e30f : st.m;
+                mref[t] = st.m == -INFINITY ? kNoScore : st.m;
                 S1[t] = st.l;
 #pragma unroll
                 for (int cc = 0; cc < DC; cc++)

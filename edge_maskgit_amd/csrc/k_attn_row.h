@@ -26,6 +26,9 @@ __device__ __forceinline__ float cap_score(float s, const ScoreMod& m) {
     return y;
 }
 
+// The reference of a row that has seen nothing: below every finite score in sight, and finite
+constexpr float kNoScore = -3e38f;
+
 // A row's partial result: weights relative to 2^m
 struct RowState {
     float m, l;

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
 
     // rows past the sequence's own: marked for the joining kernel, which leaves them alone; a part without blocks: 0
     if (splits > 1 && tid < ROWS && r0 + tid < RS && (r0 + tid >= R || b0 >= b1))
-        *(f32x2*)(ml + 2 * (sp * rows + row0 + r0 + tid)) = f32x2{-1e30f, r0 + tid >= R ? -1.f : 0.f};
+        *(f32x2*)(ml + 2 * (sp * rows + row0 + r0 + tid)) = f32x2{kNoScore, r0 + tid >= R ? -1.f : 0.f};
     if (splits > 1 && b0 >= b1 && fits) return;
 
     // rows of Q as the B operand: features 64 g + 16 lg + 8 j + e
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
     f32x4 O[QT][2 * DG];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        mref[t] = -1e30f;
+        mref[t] = kNoScore;
         S1[t] = 0.f;
 #pragma unroll
         for (int c = 0; c < 2 * DG; c++) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         }
         qs[lane] = st.o[0], qs[lane + 64] = st.o[1];
         __builtin_amdgcn_wave_barrier();
-        if (4 * lane < D) put(r0 + r, 4 * lane, *(const f32x4*)&qs[4 * lane], st.m == -INFINITY ? -1e30f : st.m, st.l);
+        if (4 * lane < D) put(r0 + r, 4 * lane, *(const f32x4*)&qs[4 * lane], st.m == -INFINITY ? kNoScore : st.m, st.l);
         __builtin_amdgcn_wave_barrier();
     }
 }

@@ -396,7 +396,8 @@ int mgh_decode_step(mgh_ctx* ctx, void* d_state, void* d_work, const float* d_lo
  *      What masked keys hold, infinities and NaN included, does not matter, nor does the value of a key
  *      whose weight is zero. Sums and softmax in fp32; with an fp16 output the weights are rounded to
  *      fp16 before they meet v, with an fp32 output they keep 22 bits.
- *      D a multiple of 16 up to 128. Rows that are not fp16, 16-byte aligned (pointers and all
+ *      D a multiple of 16 up to 128; Sk and Sq H / Hkv up to 2^24, H and B up to 65535, and Hkv B ceil(Sq
+ *      (H / Hkv) / 64) below 2^22. The output overlaps no input. Rows that are not fp16, 16-byte aligned (pointers and all
  *      strides but the first) with unit feature stride are first packed into the context's scratch,
  *      and calls with few rows keep partial results in its workspace: run a shape once before it is
  *      captured. */
@@ -426,7 +427,7 @@ int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* 
  *                 t at t % 64. The tokens behind the last whole block are read from here; a block gets
  *                 its codes from here once its 32 tokens are there. So the cache does not depend on how
  *                 tokens were grouped into calls, and a sequence may be shortened (its length lowered)
- *                 by up to 32 tokens.
+ *                 to 32 tokens below the longest that it has been.
  *      d_lens [B] holds each sequence's length before the step, d_new [B] its new tokens, 0 .. S (NULL:
  *      S each): append writes them at positions lens[b] + i, attention takes them as queries at those
  *      positions (each sees the cache up to its own position), and after the last layer mgh_kv8_advance
@@ -434,7 +435,8 @@ int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* 
  *      A sequence whose numbers do not fit (negative, more than S new tokens, past max_blocks * 32) is
  *      left alone by append and gives NaN rows in attention and read, as does a page number outside the
  *      pool among the blocks a call reads; nothing outside the buffers is touched. Two sequences may
- *      share pages that are whole. A block that holds an infinity or NaN reads as NaN.
+ *      share pages that are whole and that neither writes again (a sequence put on shared pages starts
+ *      at a multiple of 32 tokens). A block that holds an infinity or NaN reads as NaN.
  *      D a multiple of 16 up to 128; d_k, d_v and the tails 16-byte, d_scales 8-byte aligned;
  *      max_blocks * 32 up to 2^29, S and n up to 2^28. */
 typedef struct mgh_kv8 {

@@ -177,6 +177,34 @@ def test_masked_attention_scores_of_any_size(ctx):
                 check_masked(ctx, np.abs(q), kk, v, scale=scale, cap=30.0, out16=out16)
 
 
+@pytest.mark.parametrize("scale", [-1e30, 1e30, -1e36])
+def test_scores_far_from_zero(ctx, scale):
+    """every score of a row below -1e31 (or above): a row that sees keys is no row that sees nothing. Dot products
+    are 32 or 64, so weights are 0 or equal whatever the rounding; all keys of a block have one scale of codes."""
+    rng = np.random.default_rng(15)
+    q = np.ones((1, 3, 2, 32), F16)
+    k = np.ones((1, 96, 1, 32), F16)
+    k[0, ::3] = 2
+    v = (rng.standard_normal((1, 96, 1, 32)) + 0.3).astype(F16)
+    some = np.arange(96) % 3 == 0 if scale > 0 else np.arange(96) % 3 != 0
+    for sk in (96, 70):
+        for out16 in (False, True):
+            for kw in ({}, {"causal": True}, {"slopes": np.zeros(2, F32)}):
+                got = run_masked(ctx, q, k[:, :sk], v[:, :sk], out16=out16, scale=scale, **kw)
+                for i in range(3):
+                    n = sk - 2 + i if kw.get("causal") else sk
+                    want = v[0, :n, 0].astype(F64)[some[:n]].mean(0)
+                    close(got[0, i], np.stack([want] * 2), *ref.bound(q, k, v, 0.0, out16=out16))
+    with Dev(ctx) as dev:
+        c = Cache(dev, 1, 1, 32, 3, rng)
+        c.append(k, v, [0])
+        for out16 in (False, True):
+            got = c.attend(q, [93], [3], out16=out16, scale=scale)
+            for i in range(3):
+                want = ref.cache_values(v[0])[:94 + i, 0][some[:94 + i]].mean(0)
+                close(got[0, i], np.stack([want] * 2), *ref.bound(q, k, v, 0.0, out16=out16))
+
+
 @pytest.mark.parametrize("cap", [60.0, 70.0, 1e4, 1e8])
 def test_caps_of_any_size(ctx, cap):
     """scores far below the cap keep their relative accuracy"""
