@@ -38,47 +38,62 @@ __global__ __launch_bounds__(256) void k_attn_pack(PackArgs p) {
     *(f16x8*)(v.dst + row * p.D + d) = x;
 }
 
-// a joined row's features d .. d + N - 1
-template <int N>
-__device__ __forceinline__ void put_row(const JoinArgs& a, int64_t row, int d, const float* o, float l) {
-    const int64_t hb = row / a.R;
-    const int r = (int)(row - hb * a.R), i = r / a.G, g = r - i * a.G;
-    const int64_t ro = hb / a.Hkv * a.ost[3] + (hb % a.Hkv * a.G + g) * a.ost[2] + i * a.ost[1];
+// a joined row's features d .. d + 3
+__device__ __forceinline__ void put_row(const JoinArgs& a, int row, int d, const float* o, float l) {
+    const int hb = row / a.R, r = row - hb * a.R, i = r / a.G, g = r - i * a.G, b = hb / a.Hkv;
+    const int64_t ro = (int64_t)b * a.ost[3] + (int64_t)((hb - b * a.Hkv) * a.G + g) * a.ost[2] + (int64_t)i * a.ost[1];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    f32x4 v;
 #pragma unroll
-    for (int x = 0; x < N; x++) {
-        const float v = l == 0.f ? 0.f : o[x] / l;
-        if (a.o16) a.o16[ro + (d + x) * a.ost[0]] = (_Float16)v;
-        else a.o[ro + (d + x) * a.ost[0]] = v;
+    for (int x = 0; x < 4; x++) v[x] = l == 0.f ? 0.f : o[x] * inv;
+    if (a.vec_o) {
+        if (a.o16) *(f16x4*)(a.o16 + ro + d) = __builtin_convertvector(v, f16x4);
+        else *(f32x4*)(a.o + ro + d) = v;
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        if (a.o16) a.o16[ro + (d + x) * a.ost[0]] = (_Float16)v[x];
+        else a.o[ro + (d + x) * a.ost[0]] = v[x];
     }
 }
 
-// Few parts: one wave per row, 2 features a lane; nothing waits for another wave.
+// Few parts (at most P): half a wave per row, 4 features a lane, no wait for another wave. Bound by bytes where rows are
+// many (32768 of 128 features in two parts, 42 MB: 8.9 us, 4.7 TB/s; a wave per row, 2 features a lane, 13.4), else by
+// one round trip to memory (32 rows 2.8 us).
+template <int P>
 __global__ __launch_bounds__(256) void k_attn_join_few(JoinArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int d = 4 * (threadIdx.x & 31), row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= a.rows) return;
-    const f32x2* ml = (const f32x2*)(a.ws + a.splits * a.rows * a.D);
-    f32x2 st[kFewSplits], part[kFewSplits];
+    const f32x2* ml = (const f32x2*)(a.ws + (int64_t)a.splits * a.rows * a.D);
+    const float* ws = a.ws + (int64_t)row * a.D + (d < a.D ? d : 0);
+    // all loads at once: a part that saw nothing wrote no values, whatever lies there is read and not used
+    f32x2 st[P];
+    f32x4 part[P];
 #pragma unroll
-    for (int s = 0; s < kFewSplits; s++) st[s] = s < a.splits ? ml[s * a.rows + row] : f32x2{-INFINITY, 0.f};
+    for (int s = 0; s < P; s++) {
+        const int64_t at = (int64_t)min(s, a.splits - 1) * a.rows;
+        st[s] = ml[at + row];
+        part[s] = *(const f32x4*)(ws + at * a.D);
+    }
     if (st[0][1] < 0.f) return;              // not a sequence's row
 #pragma unroll
-    for (int s = 0; s < kFewSplits; s++) {   // (a part that saw nothing wrote no values)
-        part[s] = f32x2{0.f, 0.f};
-        if (s < a.splits && st[s][1] != 0.f && 2 * lane < a.D) part[s] = *(const f32x2*)(a.ws + (s * a.rows + row) * a.D + 2 * lane);
+    for (int s = 0; s < P; s++) {
+        if (s >= a.splits) st[s] = f32x2{kNoScore, 0.f};
+        if (st[s][1] == 0.f) part[s] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    float m = -INFINITY, l = 0.f;
+    float m = st[0][0], l = 0.f;
 #pragma unroll
-    for (int s = 0; s < kFewSplits; s++) m = fmaxf(m, st[s][0]);
-    f32x2 o = {0.f, 0.f};
+    for (int s = 1; s < P; s++) m = fmaxf(m, st[s][0]);
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < kFewSplits; s++) {
+    for (int s = 0; s < P; s++) {
         const float w = st[s][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[s][0] - m);
         l = fmaf(w, st[s][1], l);
-        o += part[s] * w;
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[x] = fmaf(part[s][x], w, o[x]);
     }
-    const float v[2] = {o[0], o[1]};
-    if (2 * lane < a.D) put_row<2>(a, row, 2 * lane, v, l);
+    if (d < a.D) put_row(a, row, d, o, l);
 }
 
 // Many: one workgroup per row, the parts' states joined. The weights 2^(m_s - m) go to LDS, then 8 groups of 32
@@ -87,11 +102,11 @@ __global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
     __shared__ float w[kMostSplits], red[8];
     __shared__ __attribute__((aligned(16))) float part[8][128];
     const int tid = threadIdx.x, wave = tid >> 6;
-    const int64_t row = blockIdx.x;
-    const f32x2* ml = (const f32x2*)(a.ws + a.splits * a.rows * a.D);
+    const int row = blockIdx.x;
+    const f32x2* ml = (const f32x2*)(a.ws + (int64_t)a.splits * a.rows * a.D);
     if (ml[row][1] < 0.f) return;            // not a sequence's row
     float m = -INFINITY;
-    for (int s = tid; s < a.splits; s += 256) m = fmaxf(m, ml[s * a.rows + row][0]);
+    for (int s = tid; s < a.splits; s += 256) m = fmaxf(m, ml[(int64_t)s * a.rows + row][0]);
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
     if ((tid & 63) == 0) red[wave] = m;
@@ -99,7 +114,7 @@ __global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float l = 0.f;
     for (int s = tid; s < a.splits; s += 256) {
-        const f32x2 x = ml[s * a.rows + row];
+        const f32x2 x = ml[(int64_t)s * a.rows + row];
         w[s] = x[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - m);
         l = fmaf(w[s], x[1], l);
     }
@@ -113,13 +128,13 @@ __global__ __launch_bounds__(256) void k_attn_join(JoinArgs a) {
     if (d < a.D)
 #pragma unroll 4
         for (int s = grp; s < a.splits; s += 8)
-            if (w[s] != 0.f) o += *(const f32x4*)(a.ws + (s * a.rows + row) * a.D + d) * w[s];
+            if (w[s] != 0.f) o += *(const f32x4*)(a.ws + ((int64_t)s * a.rows + row) * a.D + d) * w[s];
     *(f32x4*)&part[grp][d] = o;
     __syncthreads();
     if (tid >= 32 || d >= a.D) return;
     for (int i = 1; i < 8; i++) o += *(const f32x4*)&part[i][d];
     const float v[4] = {o[0], o[1], o[2], o[3]};
-    put_row<4>(a, row, d, v, l);
+    put_row(a, row, d, v, l);
 }
 
 }  // namespace
@@ -132,7 +147,10 @@ hipError_t launch_attn_pack(const PackArgs& p, hipStream_t s) {
 }
 
 hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s) {
-    if (a.splits <= kFewSplits) hipLaunchKernelGGL(k_attn_join_few, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+    const dim3 waves((unsigned)((a.rows + 7) / 8));
+    if (a.splits <= 2) hipLaunchKernelGGL(k_attn_join_few<2>, waves, dim3(256), 0, s, a);
+    else if (a.splits <= 4) hipLaunchKernelGGL(k_attn_join_few<4>, waves, dim3(256), 0, s, a);
+    else if (a.splits <= 8) hipLaunchKernelGGL(k_attn_join_few<8>, waves, dim3(256), 0, s, a);
     else hipLaunchKernelGGL(k_attn_join, dim3((unsigned)a.rows), dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -164,7 +182,8 @@ hipError_t launch_attn_masked(const MaskedAttnArgs& a, const MaskedPlan& p, hipS
     j.ws = a.ws; j.o = a.o; j.o16 = a.o16;
     for (int i = 0; i < 4; i++) j.ost[i] = a.ost[i];
     j.G = a.H / a.Hkv; j.Hkv = a.Hkv; j.D = a.D; j.splits = p.splits;
-    j.R = (int64_t)a.Sq * j.G;
+    j.vec_o = a.vec_o;
+    j.R = a.Sq * j.G;
     j.rows = j.R * a.Hkv * a.B;
     return launch_attn_join(j, s);
 }

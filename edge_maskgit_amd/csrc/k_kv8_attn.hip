@@ -438,7 +438,8 @@ hipError_t launch_kv8_attn(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s
     j.ws = a.ws; j.o = a.o; j.o16 = a.o16;
     for (int i = 0; i < 4; i++) j.ost[i] = a.ost[i];
     j.G = a.H / a.c.Hkv; j.Hkv = a.c.Hkv; j.D = a.c.D; j.splits = p.splits;
-    j.R = (int64_t)a.S * j.G;
+    j.vec_o = a.vec_o;
+    j.R = a.S * j.G;
     j.rows = j.R * a.c.Hkv * a.c.B;
     return launch_attn_join(j, s);
 }

@@ -1422,6 +1422,7 @@ int mgh_kv8_attn(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const
     const int64_t packed[4] = {1, kv->D, (int64_t)kv->D * S, (int64_t)kv->D * S * H};
     for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.ost[i] = ost ? ost[i] : packed[i];
     a.vec_q = in_f16 && rows_aligned(q, qst, 8, 16);
+    a.vec_o = o16 ? rows_aligned(o16, a.ost, 4, 8) : rows_aligned(o, a.ost, 4, 16);
     const mgh::Kv8Plan plan = mgh::kv8_plan(a);
     if ((int64_t)plan.tiles * plan.splits * kv->Hkv * kv->B >= (1 << 24))
         return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn: shape too large");

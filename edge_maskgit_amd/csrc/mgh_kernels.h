@@ -335,10 +335,11 @@ struct JoinArgs {
     const float* ws;
     float* o;
     _Float16* o16;
-    int64_t ost[4], rows, R;
-    int G, Hkv, D, splits;
+    int64_t ost[4];
+    int rows, R, G, Hkv, D, splits;
+    bool vec_o;            // 4 features of an output row: one aligned store
 };
-constexpr int kMostSplits = 1024, kFewSplits = 8;
+constexpr int kMostSplits = 1024;
 hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s);
 
 // The 8-bit cache (include/mgh.h has the layout)
@@ -391,6 +392,7 @@ struct Kv8AttnArgs {
     ScoreMod mod;
     const float* slopes;
     bool vec_q;            // fp16 rows, 16-byte aligned, features in order
+    bool vec_o;            // 4 features of an output row: one aligned store
     float* ws;             // Kv8Plan::ws_bytes
 };
 struct Kv8Plan {
