@@ -85,11 +85,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lg = lane >> 4;
-    // each XCD takes contiguous runs of (sequence, key head); of a head the last rows, which see most, first
+    // each XCD takes contiguous runs of (key head, sequence), sequences innermost, whose masks may leave unlike work; of
+    // a head the last rows, which see most, first
     const int lid = xcd_remap(blockIdx.x, gridDim.x);
-    const int hb = lid / (tiles * splits), in_h = lid - hb * (tiles * splits);
+    const int at = lid / (tiles * splits), in_h = lid - at * (tiles * splits);
     const int tile = tiles - 1 - in_h / splits, sp = in_h % splits;
-    const int hk = hb % a.Hkv, b = hb / a.Hkv, G = a.H / a.Hkv, R = a.Sq * G, off = a.Sk - a.Sq;
+    const int hk = at / a.B, b = at - hk * a.B, hb = b * a.Hkv + hk, G = a.H / a.Hkv, R = a.Sq * G, off = a.Sk - a.Sq;
     const int prefix = a.prefix ? min(a.prefix[b], a.Sk) : 0;
     auto bound_of = [&](int i) { return a.causal ? min(max(off + i, prefix - 1), a.Sk - 1) : a.Sk - 1; };
     const int r0 = tile * 4 * WROWS, rw = r0 + wave * WROWS;
@@ -120,8 +121,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
     // this split's chunks
     const int nch = wg_hi / kMaskKeys + 1, per = (nch + splits - 1) / splits;
     const int c0 = wg_hi < 0 ? 0 : sp * per, c1 = wg_hi < 0 ? 0 : min(nch, c0 + per);
-    const bool scan = docs && c1 - c0 <= kMaskScan;
+    const bool scan = docs && c1 > c0 && c1 - c0 <= kMaskScan;
     if (scan) {
+        // 8 chunks' ids at once, the first ones with the rows' own; each wave takes 8 of 32 chunks, a byte of the noted bits
+        int x[8];
+        auto load_ids = [&](int c) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = docs[min((c + k) * kMaskKeys + lane, a.Sk - 1)];
+        };
+        load_ids(c0 + 8 * wave);
         // the workgroup's ids: smallest, largest, and whether every row has one
         const int i0 = r0 / G, i1 = (min(r0 + 4 * WROWS, R) - 1) / G;
         int lo = INT32_MAX, hi = -1, all = 1;
@@ -137,20 +145,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
         __syncthreads();
         for (int w = 0; w < 4; w++) lo = min(lo, range[0][w]), hi = max(hi, range[1][w]), all &= range[2][w];
         all = all && lo == hi;
-        // 8 chunks' ids at once; each wave takes 8 of 32 chunks, a byte of the noted bits
         for (int w0 = c0 + 8 * wave; w0 < c1; w0 += 32) {
-            int x[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int j = (w0 + k) * kMaskKeys + lane;
-                x[k] = j < a.Sk ? docs[j] : -1;
-            }
+            if (w0 != c0 + 8 * wave) load_ids(w0);
             uint32_t some = 0, whole = 0;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                if (w0 + k < c1 && __any(x[k] >= lo && x[k] <= hi)) {
+                if (w0 + k < c1 && __any(x[k] >= lo && x[k] <= hi)) {     // (past the last key: its id again)
                     some |= 1u << k;
-                    if (all && __all(x[k] == hi || (w0 + k) * kMaskKeys + lane >= a.Sk)) whole |= 1u << k;
+                    if (all && __all(x[k] == hi)) whole |= 1u << k;
                 }
             }
             if (lane == 0) {
