@@ -151,3 +151,86 @@ def test_oracle_matches_a_plain_softmax(cap):
     s = s - 0.1 * np.abs(19 - np.arange(20))
     w = np.exp(s) / np.exp(s).sum()
     assert np.allclose(ref.attention_row(q, k, v, 0.3, cap, 0.1, 19, np.ones(20, bool)), w @ v, atol=1e-12)
+
+
+def test_which_kernels_masked_attention_takes():
+    """tiles per wave, parts of the keys, packing and joining, as the rules say"""
+    run(BODY + """
+def call(Sq, Sk, H, Hkv, D, Bn=1, in16=True, out16=True, q=W, st=None, **kw):
+    q_st = st or (1, H * D, D, Sq * H * D)
+    launches()
+    c.attn_masked(q, X, B, q_st, (1, Hkv * D, D, Sk * Hkv * D), D, Sq, Sk, H, Hkv, Bn, D ** -0.5, in16=in16,
+                  **{"o16" if out16 else "o": Y}, **kw)
+    return launches()
+
+def tile(l):
+    m = re.search(r"k_attn_maskedILi(\\d)ELi(\\d)ELb(\\d)ELi(\\d)E", l[1])
+    return tuple(map(int, m.groups())), l[2][0]
+
+def one(*a, **kw):
+    l = call(*a, **kw)
+    assert [k for k, _, _ in l] == ["k_attn_masked"], l
+    return tile(l[0])
+
+# many rows: two 16-row tiles per wave for wide heads, and for narrow ones whose rows all see the same keys
+assert one(4097, 4097, 32, 32, 128) == ((8, 2, 0, 0), 33 * 32)
+assert one(4097, 4097, 32, 32, 128, causal=True) == ((8, 2, 0, 0), 33 * 32)
+assert one(4097, 4097, 32, 32, 64) == ((4, 2, 0, 0), 33 * 32)
+assert one(4097, 4097, 32, 32, 64, causal=True) == ((4, 1, 0, 0), 65 * 32)
+assert one(4097, 4097, 32, 32, 64, docs=G, doc_stride=0) == ((4, 1, 0, 0), 65 * 32)
+assert one(4097, 4097, 32, 32, 64, cap=30.0) == ((4, 1, 0, 2), 65 * 32)
+# the heads of a group are rows of one tile
+assert one(4096, 4096, 32, 8, 128) == ((8, 2, 0, 0), 128 * 8)
+# scores: scaled, sloped or of any scale, capped, both or with caps past 64
+assert one(257, 257, 16, 16, 48) == ((3, 1, 0, 0), 5 * 16)
+assert one(257, 257, 16, 16, 48, slopes=R) == ((3, 1, 0, 1), 5 * 16)
+assert one(257, 257, 16, 16, 48, cap=30.0) == ((3, 1, 0, 2), 5 * 16)
+assert one(257, 257, 16, 16, 48, cap=70.0) == ((3, 1, 0, 3), 5 * 16)
+assert one(257, 257, 16, 16, 48, cap=30.0, slopes=R) == ((3, 1, 0, 3), 5 * 16)
+assert one(257, 257, 16, 16, 48, out16=False) == ((3, 1, 1, 0), 5 * 16)
+for D, dc in ((16, 2), (32, 2), (80, 6), (96, 6), (112, 8)):
+    assert one(64, 64, 2, 2, D) == ((dc, 1, 0, 0), 2)
+# few workgroups: the keys in parts of at least four chunks, joined
+for sk, parts, join in ((448, 1, None), (511, 2, "ILi2E"), (512, 2, "ILi2E"), (1000, 4, "ILi4E"), (2048, 8, "ILi8E"), (8192, 32, "k_attn_joinE")):
+    l = call(1, sk, 8, 2, 128)
+    assert tile(l[0]) == ((8, 1, 0, 0), 2 * parts), (sk, l)
+    assert len(l) == (1 if join is None else 2) and (join is None or join in l[1][1]), (sk, l)
+assert [k for k, _, _ in call(1, 8000, 32, 8, 128, Bn=8)] == ["k_attn_masked", "k_attn_join_few"]
+assert len(call(512, 12345, 32, 8, 128, Bn=2)) == 2
+# rows that are not fp16, not 16-byte aligned or without unit stride are packed first
+p = ["k_attn_pack", "k_attn_masked"]
+assert [k for k, _, _ in call(64, 64, 2, 2, 64, in16=False, out16=False)] == p
+assert [k for k, _, _ in call(64, 64, 2, 2, 64, q=W + 2)] == p
+assert [k for k, _, _ in call(64, 64, 2, 2, 64, st=(1, 132, 64, 64 * 132))] == p
+assert call(64, 64, 2, 2, 64, q=W + 2)[0][2][1] == 1 and call(64, 64, 2, 2, 64, in16=False)[0][2][1] == 3
+assert one(64, 64, 2, 2, 64, st=(1, 136, 64, 64 * 136)) == ((4, 1, 0, 0), 2)
+""")
+
+
+def test_which_kernels_cache_attention_takes():
+    run(BODY + """
+def call(S, H, Hkv, D, Bn, nb, **kw):
+    kv = ema.Kv8(W, X, B, R, Y, G, nb, 1 << 20, Hkv, D, Bn)
+    launches()
+    c.kv8_attn(kv, 0x1200000, (1, H * D, D, S * H * D), S, 0x1300000, None, H, D ** -0.5, o16=0x1400000, **kw)
+    l = launches()
+    m = re.search(r"k_kv8_attnILi(\\d)ELi(\\d)ELb(\\d)ELb(\\d)E", l[0][1])
+    return tuple(map(int, m.groups())), l[0][2][0], [k for k, _, _ in l[1:]]
+
+few, many = ["k_attn_join_few"], ["k_attn_join"]
+assert call(1, 32, 8, 128, 1, 8) == ((4, 1, 0, 0), 8, [])                     # eight blocks: one part
+assert call(1, 32, 8, 128, 1, 9) == ((4, 1, 0, 0), 16, few)
+assert call(1, 32, 8, 128, 1, 64) == ((4, 1, 0, 0), 8 * 8, few)
+assert call(1, 32, 8, 128, 1, 4096) == ((4, 1, 0, 0), 8 * 32, many)           # a workgroup per CU
+assert call(1, 32, 8, 128, 1, 16384) == ((4, 1, 0, 0), 8 * 96, many)
+assert call(1, 32, 8, 128, 1, 1 << 24) == ((4, 1, 0, 0), 2048, many)          # no more than eight per CU
+assert call(1, 32, 8, 128, 64, 96) == ((4, 1, 0, 0), 512, [])                 # enough workgroups: parts of long sequences only
+assert call(1, 32, 8, 128, 64, 97) == ((4, 1, 0, 0), 1024, few)
+assert call(1, 32, 8, 128, 64, 1 << 20) == ((4, 1, 0, 0), 2048, few)
+assert call(4, 32, 8, 128, 64, 8) == ((4, 1, 0, 0), 512, [])                  # 16 rows of a key head: one tile
+assert call(5, 32, 8, 128, 64, 8) == ((4, 2, 0, 0), 512, [])
+assert call(9, 32, 8, 128, 64, 8) == ((4, 2, 0, 0), 1024, [])
+for D, dg in ((16, 1), (32, 1), (48, 2), (64, 2), (80, 3), (96, 3), (112, 4)):
+    assert call(1, 8, 8, D, 64, 8) == ((dg, 1, 0, 0), 512, [])
+assert call(1, 8, 8, 64, 64, 8, cap=3.0)[0] == call(1, 8, 8, 64, 64, 8, slopes=0x1500000)[0] == (2, 1, 0, 1)
+""")
