@@ -14,10 +14,10 @@ namespace mgh {
 
 namespace {
 
-__device__ __forceinline__ uint32_t code_of(_Float16 x, float d, float id) {
-    const float a = fabsf((float)x), f = floorf(a * id);
-    const int q = (int)f + (fmaf(-(f + 0.5f), d, a) >= 0.f ? 1 : 0);
-    return (uint32_t)(128 + ((float)x < 0.f ? -q : q));
+// code + 128, a whole number (a conversion to a byte takes it as it is)
+__device__ __forceinline__ float code_of(_Float16 x, float d, float id) {
+    const float a = fabsf((float)x), h = floorf(a * id) + 0.5f;
+    return 128.f + copysignf(h + (fmaf(-h, d, a) >= 0.f ? 0.5f : -0.5f), (float)x);
 }
 
 // N consecutive features of a row: 16-byte loads where rows are aligned for them (VEC), else one by one
@@ -83,13 +83,20 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
         }
     };
     auto load_v8 = [&](int t, int d, int from, _Float16* x) {            // the input's from token `from` on
+        const int64_t e = at(t, d);
+        auto one = [&](int i) {
+            _Float16 two[2];
+            load_row<2, IN16, VEC>(a.v, e + i * a.st[1], a.st[0], two);
+            x[i] = two[0], x[8 + i] = two[1];
+        };
+        if (t >= from && t + 8 <= total) {                               // no branch between the loads
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (t + i >= from && t + i < total) {
-                _Float16 two[2];
-                load_row<2, IN16, VEC>(a.v, at(t + i, d), a.st[0], two);
-                x[i] = two[0], x[8 + i] = two[1];
-            }
+            for (int i = 0; i < 8; i++) one(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (t + i >= from && t + i < total) one(i);
+        }
     };
 
     const bool has = tid < 2 * D;                                        // 32 D / 16 units of K, as many of V
@@ -143,9 +150,10 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
             const float top = h2f(u), d = top / 127.f, id = u && u < 0x7c00u ? 127.f / top : 0.f;
             if (page < 0 || !has) continue;
             const _Float16* x = w ? xv : xk;
-            u32x4 q = {0, 0, 0, 0};
+            u32x4 q = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+            if (id > 0.f)
 #pragma unroll
-            for (int i = 0; i < 16; i++) q[i >> 2] |= (id > 0.f ? code_of(x[i], d, id) : 128u) << (8 * (i & 3));
+                for (int i = 0; i < 16; i++) q[i >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(code_of(x[i], d, id), i & 3, q[i >> 2]);
             const int64_t to = (page * c.Hkv + hk) * kKvBlock * D + (int64_t)16 * tid;
             *(u32x4*)((w ? c.v : c.k) + to) = q;
             if (tid == 0) c.scales[(page * c.Hkv + hk) * 2 + w] = d;
