@@ -2,7 +2,7 @@
 //
 // s_j = scale q . k_j; capped: s <- cap tanh(s / cap); sloped: s <- s - slope |p - j|; over the keys
 // that the row sees, o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with a running m (fp32 throughout).
-// A masked key is not read, and a key whose weight is zero adds nothing whatever its value holds, so
+// A masked key's score is not computed, and a key whose weight is zero adds nothing whatever its value holds, so
 // neither infinities nor NaN there reach the row. The tiled kernels, whose matrix products multiply a
 // masked key's value by a zero weight, take this path for the rows that came out not finite.
 #pragma once
@@ -65,13 +65,24 @@ __device__ __forceinline__ RowState attn_row(const Src& src, const ScoreMod& mod
         st.o[1] *= al;
         pl[lane] = w;
         __builtin_amdgcn_wave_barrier();
-        const int n = (int)(hi - j0 < 64 ? hi - j0 : 64);
-        for (int k = 0; k < n; k++) {
-            const float pk = pl[k];
-            if (pk == 0.f) continue;
+        // 8 keys' values on their way at once; those of weight zero are read and left out
+        for (int k = 0; k < 64 && j0 + k < hi; k += 8) {
+            float x[2][8];
 #pragma unroll
             for (int i = 0; i < 2; i++)
-                if (lane + 64 * i < D) st.o[i] = fmaf(pk, src.value(j0 + k, lane + 64 * i), st.o[i]);
+                if (64 * i < D)
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const int64_t j = j0 + k + u < hi ? j0 + k + u : hi - 1;
+                        x[i][u] = src.value(j, lane + 64 * i < D ? lane + 64 * i : D - 1);
+                    }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float pk = pl[k + u];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    if (64 * i < D) st.o[i] = pk == 0.f ? st.o[i] : fmaf(pk, x[i][u], st.o[i]);
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }

@@ -13,8 +13,8 @@
 //  * Codes stay whole numbers in the products; K's scale multiplies a block's scores, V's its share of the
 //    output, both in fp32. Weights are fp16 (hi + lo for an fp32 output, PS).
 //  * The tokens behind the last whole block are one more block, of fp16 rows.
-// Rows that come out not finite (a scale that is, a page outside the pool, infinities among the open block's
-// values) are taken again by attn_row.
+// Rows whose sum is finite and whose values are not (a scale of V that is not, infinities among the open block's
+// values), and all rows of a part with a page outside the pool, are taken again by attn_row.
 #include <algorithm>
 
 #include "k_attn_row.h"
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
     constexpr int DK = (DG + 1) / 2, ROWS = 16 * QT, OLD = 32 * DG + 4;
     __shared__ __attribute__((aligned(16))) float so[4][ROWS][OLD];
     __shared__ float sm[4][ROWS][2];
-    __shared__ int odd[ROWS];
+    __shared__ int odd[ROWS], gone[4];
     const Kv8& cache = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lg = lane >> 4, D = cache.D;
@@ -302,7 +302,6 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
     // the waves' states, joined by the threads: row, 4 features
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        if (lost) S1[t] = __builtin_nanf("");
 #pragma unroll
         for (int g = 0; g < DG; g++)
 #pragma unroll
@@ -314,7 +313,9 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         if (lg == 0) sm[wave][16 * t + l16][0] = mref[t], sm[wave][16 * t + l16][1] = S1[t];
     }
     if (tid < ROWS) odd[tid] = 0;
+    if (lane == 0) gone[wave] = lost;
     __syncthreads();
+    const bool again = !fits || gone[0] || gone[1] || gone[2] || gone[3];
     auto put = [&](int r, int d, f32x4 o, float m, float l) {
         if (splits > 1) {
             *(f32x4*)(a.ws + (sp * rows + row0 + r) * D + d) = o;
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         float m, l;
         const f32x4 o = join(x, m, l);
         const float z = (o[0] + o[1] + o[2] + o[3]) * 0.f + l;
-        if (!fits || !(z - z == 0.f)) odd[x / (D / 4)] = 1;
+        if (again || (!(z - z == 0.f) && l == l)) odd[x / (D / 4)] = 1;
     }
     __syncthreads();
     for (int x = tid; x < nr * (D / 4); x += 256) {

@@ -164,6 +164,24 @@ def test_masked_places_may_hold_anything(ctx, bad, out16, S):
     assert np.isfinite(got[0, :at].astype(F64)).all()
 
 
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("D", [48, 128])
+def test_padded_batch_of_anything(ctx, bad, D):
+    """documents and padding behind them whose keys and values are never written; rows that see an infinity or
+    NaN come out NaN, the rest as if it were not there"""
+    rng = np.random.default_rng(16)
+    q, k, v = qkv(rng, 2, 260, 260, 4, 2, D)
+    docs = docs_of(rng, 2, 260, 3, pad=77)
+    k[:, 183:] = bad
+    v[:, 183:] = bad
+    for kw in ({}, {"causal": True}, {"cap": 5.0}, {"slopes": np.full(4, 0.1, F32)}):
+        for out16 in (False, True):
+            got = check_masked(ctx, q, k, v, out16=out16, docs=docs, **kw)
+            assert np.isfinite(got.astype(F64)).all() and not got[:, 183:].any()
+    got = run_masked(ctx, q, k, v, causal=True)
+    assert np.isfinite(got[:, :183].astype(F64)).all() and np.isnan(got[:, 183:].astype(F64)).all()
+
+
 def test_masked_attention_scores_of_any_size(ctx):
     """a row whose scores climb, fall, or stand far above or below zero; a negative scale; scale 0"""
     rng = np.random.default_rng(8)
