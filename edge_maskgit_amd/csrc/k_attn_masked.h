@@ -23,9 +23,9 @@
 // finite has seen such a score.) Two rows of 4097 tokens in documents, NaN behind them: 1.1 ms against 0.06. Values
 // that no row of the workgroup sees zeroed in LDS would make that 0.06 too, but cost every call 4-5%.
 //
-// Measured: 16 heads of 64, 2 x 4097 tokens 184 us (749 TFLOP/s); 32 heads on 8 of 128, 512 rows of each of two
-// prompts of 12345 in 201 us (1.0 PFLOP/s; MFMA busy 44%, VALU 36% of the peak clock's cycles), 8191 tokens capped 646
-// (864 TFLOP/s: two exponentials and a reciprocal per score); one row of 8000 keys, 8 sequences: 53 us, 4.9 TB/s.
+// Measured: 16 heads of 64, 2 x 4097 tokens 177 us (780 TFLOP/s); 32 heads on 8 of 128, 512 rows of each of two
+// prompts of 12345 in 199 us (1.0 PFLOP/s; MFMA busy 44%, VALU 36% of the peak clock's cycles), 8191 tokens capped 640
+// (870 TFLOP/s: two exponentials and a reciprocal per score); one row of 8000 keys, 8 sequences: 53 us, 4.9 TB/s.
 // Tiles of 32 rows on v_mfma_f32_32x32x16_f16 (half the softmax state) ran 3-11% longer.
 #pragma once
 #include <type_traits>
@@ -282,14 +282,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
             }
             if (MOD & 1) {
 #pragma unroll
-                for (int t = 0; t < QT; t++)
+                for (int t = 0; t < QT; t++) {
+                    const float d0 = pos[t] - (float)(k0 + 4 * lg);      // (whole numbers below 2^24 throughout)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            const float x = MOD == 3 ? cap_score(sc[t][n][r], a.mod) : sc[t][n][r] * scale2;
-                            sc[t][n][r] = fmaf(-slope2[t], fabsf(pos[t] - (float)(k0 + 16 * n + 4 * lg + r)), x);
+                            const float d = fabsf(d0 - (float)(16 * n + r));
+                            sc[t][n][r] = MOD == 3 ? fmaf(-slope2[t], d, cap_score(sc[t][n][r], a.mod)) : fmaf(sc[t][n][r], scale2, -slope2[t] * d);
                         }
+                }
             }
             __builtin_amdgcn_s_setprio(0);
             // the results are in their registers before a branch looks at them

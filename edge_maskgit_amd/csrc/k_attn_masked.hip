@@ -156,10 +156,11 @@ hipError_t launch_attn_join(const JoinArgs& a, hipStream_t s) {
 }
 
 // Two row tiles per wave (each operand read from LDS serves both) where they still give a workgroup per CU: 128
-// features, 32 heads of 4097 tokens 334 against 374 us for one. Up to 64 features the LDS is no bound and the gain is
-// small (unmasked 184 / 197 us), while rows that see unlike numbers of keys are better shared out in smaller
-// pieces (causal 117 / 108, nine documents 85 / 78) and capped scores wait for the VALU anyway (280 / 274): one.
-// Too few workgroups for two per CU: the keys in parts (512 x 12345, 256 workgroups: one part 243 us, two 214; one
+// features, 32 heads of 4097 tokens 332 against 372 us for one, a prefix of 1000 in 8191 capped 638 / 795. Up to 64
+// features the LDS is no bound and the gain is small (unmasked 177 / 193 us), while rows that see unlike numbers of
+// keys are better shared out in smaller pieces (nine documents 78 / 69, causal 105 / 107) and capped scores wait for
+// the VALU anyway (276 / 270): one.
+// Too few workgroups for two per CU: the keys in parts (512 x 12345, 256 workgroups: one part 248 us, two 199; one
 // token over 8000 keys, 64 workgroups: 1 / 2 / 4 / 8 parts 253 / 136 / 78 / 56 us), of at least 4 chunks (257 tokens, 80
 // workgroups of 5 chunks: 12 us whole, 19 in two parts).
 MaskedPlan masked_plan(const MaskedAttnArgs& a) {

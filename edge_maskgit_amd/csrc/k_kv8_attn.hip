@@ -15,6 +15,10 @@
 //  * The tokens behind the last whole block are one more block, of fp16 rows.
 // Rows whose sum is finite and whose values are not (a scale of V that is not, infinities among the open block's
 // values), and all rows of a part with a page outside the pool, are taken again by attn_row.
+//
+// Measured (32 heads on 8 of 128): one sequence of 100000 tokens, 205 MB, 39.5 us (5.2 TB/s) and the join 4.8; 64 of 2700
+// tokens 69 us (5.2 TB/s), of up to 8000 with capped scores 90 (4.1 TB/s: long sequences' parts at the end). A block takes
+// a wave 0.88 us, so short sequences are latency: 4 of 1030, 16 heads of 48, five rows: 7.3 us and the join 2.8.
 #include <algorithm>
 
 #include "k_attn_row.h"
@@ -168,6 +172,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             mx[t] = -INFINITY;
+            const float d0 = (float)(lim[t] - j0);
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
                     float s = sc[t][n][r] * scale;
                     if (MOD) {
                         if (a.mod.cap2 != 0.f) s = cap_score(s, a.mod);
-                        s = fmaf(-slope2[t], (float)(lim[t] - (j0 + 4 * n + r)), s);     // (of the keys that it sees)
+                        s = fmaf(-slope2[t], d0 - (float)(4 * n + r), s);     // (of the keys that it sees)
                     }
                     s = j0 + 4 * n + r > lim[t] ? -INFINITY : s;
                     sc[t][n][r] = s;
