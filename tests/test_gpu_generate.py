@@ -914,3 +914,45 @@ def test_capture_and_replay(ctx):
             other.sync()
             assert np.array_equal(dev.get(o2, q.shape, F16), want)
         g.destroy()
+
+
+def test_replay_after_the_workspaces_grew(ctx):
+    """a graph captured in a context of its own keeps the buffers that it was captured with when later calls need
+    larger ones, and two graphs of one context may take turns"""
+    rng = np.random.default_rng(32)
+    q, k, v = qkv(rng, 1, 2, 600, 4, 2, 64)
+    Q, K, V = qkv(rng, 2, 40, 3000, 8, 4, 64)
+    with ema.Context(0) as own, Dev(own) as dev:
+        def call(x, in16):
+            _, Sq, H, D = x[0].shape
+            Sk, Hkv = x[1].shape[1:3]
+            ins = [dev.up(a, F16 if in16 else F32) for a in x]
+            o = dev.up(np.zeros(x[0].shape, F16))
+            st, kst = (1, H * D, D, Sq * H * D), (1, Hkv * D, D, Sk * Hkv * D)
+
+            def run():
+                own.attn_masked(*ins, st, kst, D, Sq, Sk, H, Hkv, len(x[0]), D ** -0.5, o16=o, in16=in16, o_strides=st)
+            return run, o, x[0].shape
+
+        def capture(run):
+            run()
+            own.graph_begin()
+            run()
+            return own.graph_end()
+
+        small, o1, s1 = call((q, k, v), False)                  # packed, in parts
+        g1 = capture(small)
+        want1 = dev.get(o1, s1, F16)
+        large, o2, s2 = call((Q, K, V), False)
+        g2 = capture(large)                                     # both buffers grow
+        want2 = dev.get(o2, s2, F16)
+        close(want1, ref.masked(q, k, v, 0.125), *ref.bound(q, k, v, 0.125, out16=True))
+        for rep in range(3):
+            for g, o, s, want in ((g1, o1, s1, want1), (g2, o2, s2, want2)):
+                own.write(o, np.zeros(s, F16))
+                g.launch()
+                if rep == 1:
+                    (small if g is g2 else large)()
+                assert np.array_equal(dev.get(o, s, F16), want)
+        g1.destroy()
+        g2.destroy()
