@@ -412,12 +412,15 @@ void launch_cache_d(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s) {
 Kv8Plan kv8_plan(const Kv8AttnArgs& a) {
     const int64_t R = (int64_t)a.S * (a.H / a.c.Hkv), heads = (int64_t)a.c.Hkv * a.c.B;
     Kv8Plan p{};
+    // Past 16 rows two tiles share the codes' way to operands: 32 rows over 100000 tokens 51 against 59 us with one, 20 rows
+    // 48 / 55, 32 rows over 16 sequences of up to 5000 35 / 38, 64 rows 46 / 58.
     p.qt = R > 16 ? 2 : 1;
     p.tiles = (int)((R + 16 * p.qt - 1) / (16 * p.qt));
     const int64_t wgs = heads * p.tiles;
     // Few workgroups: parts until every CU has one, of at least 8 blocks (2 per wave). Enough of them: parts only of
     // sequences past 96 blocks, for the balance of ragged batches (the table's width is all that the host knows of
-    // their lengths): a second launch costs 5-8 us. Measured (32 heads on 8 of 128 features, one token), parts
+    // their lengths): a second launch costs 3-6 us. (Of 48, 64 or 96 blocks: 64 of 2700 80 / 78 / 71 us, 64 of up
+    // to 8000 92 / 90 / 95.) Measured (32 heads on 8 of 128 features, one token), parts
     // 1 / 2 / 3 / 4 / 8 / 32: one sequence of 100000 tokens 631 / 323 / 221 / 169 / 92 / 45 us, one of 9000 68 / 42 / 31 / 27 /
     // 19 / 14, 16 of 9000 78 / 61 / 68 / 62 / 65 / 74, 64 of 2700 69 / 77 / 74 / 79 / 86 / 105, 64 of up to 8000 98 / 104 / 93 / 93 /
     // 92 / 114, 64 of up to 500 14 / 22 / 19 / 25 / 20 / 40.
