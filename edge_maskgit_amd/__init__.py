@@ -560,7 +560,7 @@ class Context:
                                          (ctypes.c_int64 * 4)(*strides), S, P(lens), P(new)))
 
     def kv8_advance(self, lens, new, B, S):
-        """lens[b] += new[b] (S where new is None)"""
+        """lens[b] += new[b] (S where new is None); numbers that append refuses leave lens[b] as it is"""
         self._check(lib().mgh_kv8_advance(self.h, self._ptr(lens), self._ptr(new), B, S))
 
     def kv8_attn(self, cache, q, q_strides, S, lens, new, H, scale, o=None, o16=None, o_strides=None, in16=True, cap=0.0,

@@ -255,9 +255,14 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8ReadArgs a, T* out_k, T* ou
     }
 }
 
+// Lengths after a step. Numbers that append and attention refuse (spans) leave the length as it is, so that the next
+// step refuses it too instead of taking ring slots that were never written for tokens. Past the table, whose width is
+// not at hand here, the length grows: no later call takes it either.
 __global__ void k_kv8_advance(int32_t* lens, const int32_t* fresh, int B, int S) {
     const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b < B) lens[b] += fresh ? fresh[b] : S;      // (32-bit wrap-around lands on a length that every call refuses)
+    if (b >= B) return;
+    const int len = lens[b], n = fresh ? fresh[b] : S;
+    if (len >= 0 && n >= 0 && n <= S && n <= INT32_MAX - len) lens[b] = len + n;
 }
 
 }  // namespace

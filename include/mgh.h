@@ -457,6 +457,9 @@ size_t mgh_kv8_tail_bytes(int B, int Hkv, int D);            /* of d_k_tail, and
 /* k, v: {D, S, Hkv, B} views (element strides d, token, head, sequence), fp16 or fp32 (rounded to fp16) */
 int mgh_kv8_append(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_k, const void* d_v, int in_f16,
                    const int64_t strides[4], int S, const int32_t* d_lens, const int32_t* d_new);
+/* lens[b] += new[b] (S where d_new is NULL). A negative length, new tokens outside 0 .. S and a sum past 2^31 - 1
+ * leave lens[b] as it is, so a sequence that append left alone stays refused; one that ran past its table gets a
+ * length past it: set that back before the table is made wider. */
 int mgh_kv8_advance(mgh_ctx* ctx, int32_t* d_lens, const int32_t* d_new, int B, int S);
 /* q, o: {D, S, H, B} views, scores as mgh_attn_masked (cap, d_slopes [H] or NULL); calls with few rows keep
  * partial results in the context's workspace: run a shape once before it is captured */

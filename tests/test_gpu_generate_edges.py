@@ -1,0 +1,41 @@
+"""Token-by-token generation where it can go wrong: infinities that a row sees, rows whose sums leave fp16,
+keys whose weight is zero, sequences that a call refuses among good ones with few and many parts. Against the
+definitions in 64 bits (tests/gen_oracle.py)."""
+import numpy as np
+import pytest
+
+from tests import gen_oracle as ref
+from tests.test_gpu_generate import Dev, cache_case, ctx  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+F16, F32, F64, I32 = np.float16, np.float32, np.float64, np.int32
+
+
+# ---- the cache's lengths ------------------------------------------------------------------
+
+
+def test_cache_advance_leaves_refused_sequences_refused(ctx):
+    """numbers that append and attention refuse do not become a length that they take"""
+    rng = np.random.default_rng(1)
+    bad, new, S = [70, 70, -1, -1, 2 ** 31 - 1, 5], [2, -1, 0, 1, 1, 1], 1
+    with Dev(ctx) as dev:
+        c, q, k, v, have = cache_case(dev, rng, [70] * 6, [1] * 6, 2, 1, 32)
+        before = c.state()
+        lens = dev.up(bad, I32)
+        ctx.kv8_advance(lens, dev.up(new, I32), 6, S)
+        assert dev.get(lens, 6, I32).tolist() == [70, 70, -1, -1, 2 ** 31 - 1, 6]
+        idle = dev.up([-1, -5, 70], I32)
+        ctx.kv8_advance(idle, None, 3, 4)                                   # idle slots stay idle
+        assert dev.get(idle, 3, I32).tolist() == [-1, -5, 74]
+        # four refused steps in a row: no byte of the pages and rings changes, every row is NaN
+        lens = dev.up([70, 70, -1, -1, 2 ** 31 - 1, 32 * c.nb], I32)
+        fresh = dev.up([2, -1, 1, 1, 1, 1], I32)
+        st, w = (1, 32, 32, 32), dev.up(rng.standard_normal((6, 1, 1, 32)), F16)
+        o, qst, dq = dev.up(np.zeros((6, 1, 2, 32), F32)), (1, 64, 32, 64), dev.up(q)
+        for _ in range(4):
+            ctx.kv8_append(c.h, w, w, st, S, lens, fresh)
+            ctx.kv8_attn(c.h, dq, qst, S, lens, fresh, 2, 0.2, o=o, o_strides=qst)
+            assert np.isnan(dev.get(o, (6, 2, 32), F32)).all()
+            ctx.kv8_advance(lens, fresh, 6, S)
+        for x, y in zip(c.state(), before):
+            assert np.array_equal(x, y, equal_nan=x.dtype != np.uint8)
