@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
     }
 
     // where this lane reads in a block: K's key and features of tile t (+ 4 keys), V's feature pair and keys;
-    // lanes past D read some code of the block, which meets a zero of Q or is not stored
+    // lanes past D read some code of the block, which is finite and meets a zero of Q or is not stored
     const int key = 8 * (l16 >> 2) + (l16 & 3);
     uint32_t ka[DK], va[DG];
 #pragma unroll
@@ -293,7 +293,9 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         block(whole, 1.f, 1.f,
               [&](int n, int c) {
                   const int d = 64 * (c >> 1) + 16 * lg + 8 * (c & 1);
-                  return *(const f16x8*)(K + (slot + key + 4 * n) * D + (d < D ? d : 0));
+                  const f16x8 k = *(const f16x8*)(K + (slot + key + 4 * n) * D + (d < D ? d : 0));
+                  // (past D zeros: the key's own values may be infinite, and Q's zeros would make NaN of them)
+                  return d < D ? k : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
               },
               [&](int c) {
                   const int d = 32 * (c >> 1) + 2 * l16 + (c & 1);

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from tests import gen_oracle as ref
-from tests.test_gpu_generate import Dev, cache_case, ctx  # noqa: F401
+from tests.test_gpu_generate import Dev, cache_case, check_cache, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 F16, F32, F64, I32 = np.float16, np.float32, np.float64, np.int32
@@ -39,3 +39,29 @@ def test_cache_advance_leaves_refused_sequences_refused(ctx):
             ctx.kv8_advance(lens, fresh, 6, S)
         for x, y in zip(c.state(), before):
             assert np.array_equal(x, y, equal_nan=x.dtype != np.uint8)
+
+
+# ---- infinities that a row sees -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("D", [16, 48, 64, 80, 112, 128])
+@pytest.mark.parametrize("in16", [True, False])
+def test_open_block_with_infinite_keys(ctx, D, in16):
+    """a key behind the last whole block with an infinite feature (fp32 ones from 65520 on are): its score is an
+    infinity, so it weighs nothing where that is the negative one, whatever the width of the heads"""
+    rng = np.random.default_rng(D)
+    lens, new, H, Hkv = [40, 3], [4, 2], 4, 2
+    big = F32(np.inf) if in16 else F32(65520)
+    with Dev(ctx) as dev:
+        c, q, k, v, have = cache_case(dev, rng, lens, new, H, Hkv, D)
+        q[..., 0], q[..., 7] = np.abs(q[..., 0]) + F16(0.1), -np.abs(q[..., 7]) - F16(0.1)
+        k = k.astype(F32)
+        k[0, 36, 0, 0], k[0, 41, :, 7], k[1, 1, 1, 0], k[1, 3, 0, 7] = -big, big, -big, big
+        c.append(k[:, :max(have)], v[:, :max(have)], [0, 0], have, in16)
+        with np.errstate(over="ignore"):
+            k = k.astype(F16)
+        assert np.isinf(k).sum() == 5
+        for out16 in (True, False):
+            for kw in ({}, {"slopes": np.full(H, 0.1, F32)}, {"cap": 30.0}):
+                got = check_cache(c, q, k, v, lens, new, have, out16=out16, **kw)
+                assert all(np.isfinite(got[b, :new[b]].astype(F64)).all() for b in range(2))
