@@ -473,8 +473,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
             const MaskedSrc s{a, (const _Float16*)a.k + kv0, (const _Float16*)a.v + kv0, a.kvst[1], bound_of(i), docs,
                               docs && off + i >= 0 ? docs[off + i] : -1};
             const float sl = a.slopes ? a.slopes[hk * G + g] * kLog2e : 0.f;
-            const RowState st = attn_row(s, a.mod, sl, off + i, (int64_t)c0 * kMaskKeys, min((int64_t)c1 * kMaskKeys, (int64_t)a.Sk), a.D, qs,
-                                         qs + 128, lane);
+            const RowState st = attn_row(s, a.mod, sl, off + i, s.lim + 1, (int64_t)c0 * kMaskKeys,
+                                         min((int64_t)c1 * kMaskKeys, (int64_t)s.lim + 1), a.D, qs, qs + 128, lane);
             __builtin_amdgcn_wave_barrier();
             qs[lane] = st.o[0], qs[lane + 64] = st.o[1];
             __builtin_amdgcn_wave_barrier();

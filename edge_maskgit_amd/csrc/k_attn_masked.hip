@@ -78,10 +78,8 @@ __global__ __launch_bounds__(256) void k_attn_join_few(JoinArgs a) {
     }
     if (st[0][1] < 0.f) return;              // not a sequence's row
 #pragma unroll
-    for (int s = 0; s < P; s++) {
+    for (int s = 0; s < P; s++)
         if (s >= a.splits) st[s] = f32x2{kNoScore, 0.f};
-        if (st[s][1] == 0.f) part[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
     float m = st[0][0], l = 0.f;
 #pragma unroll
     for (int s = 1; s < P; s++) m = fmaxf(m, st[s][0]);
@@ -91,7 +89,7 @@ __global__ __launch_bounds__(256) void k_attn_join_few(JoinArgs a) {
         const float w = st[s][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(st[s][0] - m);
         l = fmaf(w, st[s][1], l);
 #pragma unroll
-        for (int x = 0; x < 4; x++) o[x] = fmaf(part[s][x], w, o[x]);
+        for (int x = 0; x < 4; x++) o[x] = w == 0.f ? o[x] : fmaf(part[s][x], w, o[x]);
     }
     if (d < a.D) put_row(a, row, d, o, l);
 }

@@ -1,9 +1,11 @@
 // k_attn_row.h — one query row of the masked and the 8-bit-cache attention, by one wave.
 //
 // s_j = scale q . k_j; capped: s <- cap tanh(s / cap); sloped: s <- s - slope |p - j|; over the keys
-// that the row sees, o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) with a running m (fp32 throughout).
-// A masked key's score is not computed, and a key whose weight is zero adds nothing whatever its value holds, so
-// neither infinities nor NaN there reach the row. The tiled kernels, whose matrix products multiply a
+// that the row sees, o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), m the largest score of all keys that the
+// row sees (fp32 throughout). A masked key's score is not computed, and a key whose weight is zero (below 2^-126
+// of the largest) adds nothing whatever its value holds, so neither infinities nor NaN there reach the row. For
+// that m is found first: against a running maximum a far key's value would have entered the sum before its weight
+// went to zero, and a part's own maximum is not the row's. The tiled kernels, whose matrix products multiply a
 // masked key's value by a zero weight, take this path for the rows that came out not finite.
 #pragma once
 #include "mgh_common.h"
@@ -35,34 +37,34 @@ struct RowState {
     float o[2];        // features lane and lane + 64
 };
 
-// keys [lo, hi) of one row. qs: the row's q in LDS (fp32, D values), pl: 64 floats of LDS; both this
-// wave's own. src.seen(j), src.dot(j, qs), src.value(j, d).
+// keys [lo, hi) of one row that sees keys of [0, end) and no others. qs: the row's q in LDS (fp32, D values), pl: 64
+// floats of LDS; both this wave's own. src.seen(j), src.dot(j, qs), src.value(j, d).
 template <class Src>
-__device__ __forceinline__ RowState attn_row(const Src& src, const ScoreMod& mod, float slope2, int64_t p, int64_t lo,
+__device__ __forceinline__ RowState attn_row(const Src& src, const ScoreMod& mod, float slope2, int64_t p, int64_t end, int64_t lo,
                                              int64_t hi, int D, const float* qs, float* pl, int lane) {
-    RowState st{-INFINITY, 0.f, {0.f, 0.f}};
-    for (int64_t j0 = lo; j0 < hi; j0 += 64) {
-        const int64_t j = j0 + lane;
-        float s = -INFINITY;
-        if (j < hi && src.seen(j)) {
-            const float x = src.dot(j, qs);
-            s = mod.cap2 != 0.f ? cap_score(x, mod) : x * mod.scale2;
-            s -= slope2 * fabsf((float)(p - j));
+    auto score = [&](int64_t j, int64_t to) {
+        if (j >= to || !src.seen(j)) return -INFINITY;
+        const float x = src.dot(j, qs);
+        return (mod.cap2 != 0.f ? cap_score(x, mod) : x * mod.scale2) - slope2 * fabsf((float)(p - j));
+    };
+    float m = -INFINITY;
+    for (int64_t j0 = 0; j0 < end; j0 += 64) {
+        const float s = score(j0 + lane, end);
+        // a NaN is the whole row's, and so is an infinite score: infinity minus itself
+        if (__any(!(s < INFINITY))) {
+            const float nan = __builtin_nanf("");
+            return RowState{nan, nan, {nan, nan}};
         }
-        float mx = s;
+        m = fmaxf(m, s);
+    }
 #pragma unroll
-        for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
-        if (__all(s == -INFINITY)) continue;
-        const float m = fmaxf(st.m, mx);
-        const float al = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
-        const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - m);
-        float sum = w;
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
-        st.l = st.l * al + sum;
-        st.m = m;
-        st.o[0] *= al;
-        st.o[1] *= al;
+    for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+    RowState st{m, 0.f, {0.f, 0.f}};
+    if (m == -INFINITY) return st;
+    for (int64_t j0 = lo; j0 < hi; j0 += 64) {
+        const float w = __builtin_amdgcn_exp2f(score(j0 + lane, hi) - m);
+        if (__all(w == 0.f)) continue;
+        st.l += w;
         pl[lane] = w;
         __builtin_amdgcn_wave_barrier();
         // 8 keys' values on their way at once; those of weight zero are read and left out
@@ -86,6 +88,8 @@ __device__ __forceinline__ RowState attn_row(const Src& src, const ScoreMod& mod
         }
         __builtin_amdgcn_wave_barrier();
     }
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) st.l += __shfl_xor(st.l, i);
     return st;
 }
 

@@ -35,8 +35,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 struct CacheSrc {
     const Kv8& c;
     int b, hk, cut;        // tokens before `cut` are in whole blocks
-    int64_t p;
-    __device__ bool seen(int64_t j) const { return j <= p; }
+    __device__ bool seen(int64_t) const { return true; }
     __device__ float dot(int64_t j, const float* qs) const {
         float s = 0.f;
         if (j < cut) {
@@ -380,8 +379,8 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
             }
             __builtin_amdgcn_wave_barrier();
             const int64_t p = (int64_t)len + i;
-            st = attn_row(CacheSrc{cache, b, hk, cut, p}, a.mod, a.slopes ? a.slopes[hk * G + g] * kLog2e : 0.f, p,
-                          (int64_t)b0 * kKvBlock, min((int64_t)b1 * kKvBlock, (int64_t)total), D, qs, qs + 128, lane);
+            st = attn_row(CacheSrc{cache, b, hk, cut}, a.mod, a.slopes ? a.slopes[hk * G + g] * kLog2e : 0.f, p, p + 1,
+                          (int64_t)b0 * kKvBlock, min((int64_t)b1 * kKvBlock, p + 1), D, qs, qs + 128, lane);
             __builtin_amdgcn_wave_barrier();
         }
         qs[lane] = st.o[0], qs[lane + 64] = st.o[1];

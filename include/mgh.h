@@ -394,7 +394,7 @@ int mgh_decode_step(mgh_ctx* ctx, void* d_state, void* d_work, const float* d_lo
  *        apart, 0: one row for all; negative: padding; a query before position 0 has none).
  *      o = softmax over the seen keys, times v; a row that sees none, or only scores of -infinity, is 0.
  *      What masked keys hold, infinities and NaN included, does not matter, nor does the value of a key
- *      whose weight is zero. Sums and softmax in fp32; with an fp16 output the weights are rounded to
+ *      whose weight is zero (below 2^-126 of the row's largest). Sums and softmax in fp32; with an fp16 output the weights are rounded to
  *      fp16 before they meet v, with an fp32 output they keep 22 bits.
  *      D a multiple of 16 up to 128; Sk and Sq H / Hkv up to 2^24, H and B up to 65535, and Hkv B ceil(Sq
  *      (H / Hkv) / 64) below 2^22. The output overlaps no input. Rows that are not fp16, 16-byte aligned (pointers and all

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from tests import gen_oracle as ref
-from tests.test_gpu_generate import Dev, cache_case, check_cache, ctx  # noqa: F401
+from tests.test_gpu_generate import Dev, cache_case, check_cache, check_masked, ctx, qkv  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 F16, F32, F64, I32 = np.float16, np.float32, np.float64, np.int32
@@ -65,3 +65,42 @@ def test_open_block_with_infinite_keys(ctx, D, in16):
             for kw in ({}, {"slopes": np.full(H, 0.1, F32)}, {"cap": 30.0}):
                 got = check_cache(c, q, k, v, lens, new, have, out16=out16, **kw)
                 assert all(np.isfinite(got[b, :new[b]].astype(F64)).all() for b in range(2))
+
+
+# ---- keys whose weight is zero ------------------------------------------------------------
+
+# keys, heads, key heads: one part, a few, more than eight
+FAR = [(300, 4, 2), (700, 4, 2), (2500, 4, 2), (8000, 2, 1)]
+
+
+@pytest.mark.parametrize("S,H,Hkv", FAR)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("out16", [True, False])
+def test_values_of_weightless_keys(ctx, S, H, Hkv, bad, out16):
+    """a slope takes far keys' weights to zero: what their values hold does not reach the row, neither within the part
+    that holds them nor where parts are joined, and a near one's does"""
+    print(f"weightless {S} {bad} {out16}", flush=True)
+    rng = np.random.default_rng(S)
+    q, k, v = qkv(rng, 1, 3, S, H, Hkv, 48)
+    v[0, 0], v[0, 5, 0, 3], v[0, 50:S - 150:50, :, 7] = bad, bad, bad
+    slopes = np.full(H, 8.0, F32)
+    got = check_masked(ctx, q, k, v, out16=out16, causal=True, slopes=slopes)
+    assert np.isfinite(got.astype(F64)).all()
+    v[0, S - 3, 0, 9] = bad
+    check_masked(ctx, q, k, v, out16=out16, causal=True, slopes=slopes)
+
+
+@pytest.mark.parametrize("S,spare", [(240, 0), (700, 10), (2500, 900)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("out16", [True, False])
+def test_cached_values_of_weightless_keys(ctx, S, spare, bad, out16):
+    """the same over the cache, whole blocks that read as NaN among them, in one part, a few and many"""
+    print(f"weightless cached {S} {spare} {bad} {out16}", flush=True)
+    rng = np.random.default_rng(S + spare)
+    H, Hkv, D = 4, 2, 48
+    with Dev(ctx) as dev:
+        c, q, k, v, have = cache_case(dev, rng, [S - 3], [3], H, Hkv, D, spare=spare)
+        v[0, 0], v[0, 5, 0, 3], v[0, 50:S - 170:50, :, 7] = bad, bad, bad
+        c.append(k[:, :S], v[:, :S], [0])
+        got = check_cache(c, q, k, v, [S - 3], [3], have, out16=out16, slopes=np.full(H, 8.0, F32))
+        assert np.isfinite(got.astype(F64)).all()
