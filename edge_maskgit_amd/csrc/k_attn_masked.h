@@ -18,9 +18,11 @@
 //    chunks need no test; ids of documents are compared only in chunks where they can differ: a first
 //    pass over the ids notes for each chunk whether any row of the workgroup can see it and whether all
 //    see all of it.
-// A masked key's weight is 0, but 0 times an infinity or NaN of V is not: rows that come out not finite although
-// their sum is are taken again by attn_row, which uses what a row sees and nothing else. (A sum that is not
-// finite has seen such a score.) Two rows of 4097 tokens in documents, NaN behind them: 1.1 ms against 0.06. Values
+// A masked key's weight is 0, but 0 times an infinity or NaN of V is not: rows that come out not finite are taken
+// again by attn_row, which uses what a row sees and nothing else. Rows whose sum of weights is not finite too: they may
+// have seen no NaN, but weights past fp16, which a moving reference then multiplied by 0: all that a row saw of a
+// chunk were infinite products at the lower end of a cap, or scores past 1e8 lie farther apart than the
+// reference's distance. Two rows of 4097 tokens in documents, NaN behind them: 1.1 ms against 0.06. Values
 // that no row of the workgroup sees zeroed in LDS would make that 0.06 too, but cost every call 4-5%.
 //
 // Measured: 16 heads of 64, 2 x 4097 tokens 177 us (780 TFLOP/s); 32 heads on 8 of 128, 512 rows of each of two
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
         for (int cc = 0; cc < DC; cc++)
 #pragma unroll
             for (int r = 0; r < 4; r++) z += O[t][cc][r] * 0.f;
-        uint64_t m = __ballot(!(z - z == 0.f) && S1[t] == S1[t] && rw + 16 * t + l16 < R);
+        uint64_t m = __ballot(!(z - z == 0.f) && rw + 16 * t + l16 < R);
         m = (m | m >> 16 | m >> 32 | m >> 48) & 0xffff;
         while (m) {
             const int l = __builtin_ctzll(m), r = rw + 16 * t + l, i = r / G, g = r - i * G;

@@ -13,8 +13,9 @@
 //  * Codes stay whole numbers in the products; K's scale multiplies a block's scores, V's its share of the
 //    output, both in fp32. Weights are fp16 (hi + lo for an fp32 output, PS).
 //  * The tokens behind the last whole block are one more block, of fp16 rows.
-// Rows whose sum is finite and whose values are not (a scale of V that is not, infinities among the open block's
-// values), and all rows of a part with a page outside the pool, are taken again by attn_row.
+// Rows that are not finite (a scale of V that is not, infinities among the open block's values, weights past fp16
+// where scores lie farther apart than the reference's distance), and all rows of a part with a page outside the pool, are
+// taken again by attn_row.
 //
 // Measured (32 heads on 8 of 128): one sequence of 100000 tokens, 205 MB, 39.5 us (5.2 TB/s) and the join 4.8; 64 of 2700
 // tokens 69 us (5.2 TB/s), of up to 8000 with capped scores 90 (4.1 TB/s: long sequences' parts at the end). A block takes
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         float m, l;
         const f32x4 o = join(x, m, l);
         const float z = (o[0] + o[1] + o[2] + o[3]) * 0.f + l;
-        if (again || (!(z - z == 0.f) && l == l)) odd[x / (D / 4)] = 1;
+        if (again || !(z - z == 0.f)) odd[x / (D / 4)] = 1;
     }
     __syncthreads();
     for (int x = tid; x < nr * (D / 4); x += 256) {

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from tests import gen_oracle as ref
-from tests.test_gpu_generate import Dev, cache_case, check_cache, check_masked, ctx, qkv  # noqa: F401
+from tests.test_gpu_generate import Cache, Dev, cache_case, check_cache, check_masked, close, ctx, qkv, run_masked  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 F16, F32, F64, I32 = np.float16, np.float32, np.float64, np.int32
@@ -65,6 +65,46 @@ def test_open_block_with_infinite_keys(ctx, D, in16):
             for kw in ({}, {"slopes": np.full(H, 0.1, F32)}, {"cap": 30.0}):
                 got = check_cache(c, q, k, v, lens, new, have, out16=out16, **kw)
                 assert all(np.isfinite(got[b, :new[b]].astype(F64)).all() for b in range(2))
+
+
+@pytest.mark.parametrize("out16", [True, False])
+def test_capped_scores_of_infinite_keys(ctx, out16):
+    """the cap of an infinite product is -cap, also for a row that sees nothing else in a chunk of 64 keys"""
+    rng = np.random.default_rng(3)
+    q, k, v = qkv(rng, 1, 200, 200, 2, 1, 48)
+    q[..., 3] = np.abs(q[..., 3]) + F16(0.1)
+    docs = np.zeros((1, 200), I32)
+    for first in (63, 127, 61):                       # a document begins with the last keys of a chunk
+        docs[:, first:] += 1
+        k[0, first:(first // 64 + 1) * 64, 0, 3] = -np.inf
+    for cap in (5.0, 30.0):
+        check_masked(ctx, q, k, v, out16=out16, cap=cap, docs=docs)
+        check_masked(ctx, q, k, v, out16=out16, cap=cap, docs=docs, causal=True)
+
+
+@pytest.mark.parametrize("out16", [True, False])
+def test_scores_past_the_reach_of_the_reference(ctx, out16):
+    """scores of 2e8, where fp32 numbers lie 16 apart: weights against a reference that could not be set closer leave
+    fp16, and a later chunk far above takes the whole weight"""
+    rng = np.random.default_rng(4)
+    D = 16
+    q, k = np.zeros((1, 2, 2, D), F16), np.zeros((1, 320, 1, D), F16)
+    q[..., 0], q[..., 1] = 32768, 0.25
+    v = (rng.standard_normal((1, 320, 1, D)) + 0.3).astype(F16)
+    for i, n in ((0, 2), (1, 4), (2, 127)):
+        k[0, 64 * i:64 * i + 64, 0, :2] = 127, n
+    got = run_masked(ctx, q, k[:, :192], v[:, :192], out16=out16, scale=32.0)
+    close(got[0], np.broadcast_to(v[0, 128:192, 0].astype(F64).mean(0), got[0].shape), *ref.bound(q, k, v, 0.0, out16=out16))
+    k[:] = 0
+    for i, n in ((0, 2), (4, 4), (8, 127)):           # blocks of one wave, in a batch of whole sequences; codes are the values
+        k[0, 32 * i:32 * i + 32, 0, :2] = 127, n
+    B = 256
+    with Dev(ctx) as dev:
+        c = Cache(dev, B, 1, D, 10, rng)
+        c.append(k.repeat(B, 0), v.repeat(B, 0), [0] * B)
+        want = ref.cache_values(v[0])[256:288, 0].mean(0)
+        got = c.attend(q.repeat(B, 0), [318] * B, [2] * B, out16=out16, scale=32.0)
+        close(got, np.broadcast_to(want, got.shape), *ref.bound(q, k, v, 0.0, out16=out16))
 
 
 # ---- keys whose weight is zero ------------------------------------------------------------
