@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
     const int at = lid / (tiles * splits), in_h = lid - at * (tiles * splits);
     const int tile = tiles - 1 - in_h / splits, sp = in_h % splits;
     const int hk = at / a.B, b = at - hk * a.B, hb = b * a.Hkv + hk, G = a.H / a.Hkv, R = a.Sq * G, off = a.Sk - a.Sq;
-    const int prefix = a.prefix ? min(a.prefix[b], a.Sk) : 0;
+    const int prefix = a.prefix ? max(min(a.prefix[b], a.Sk), 0) : 0;
     auto bound_of = [&](int i) { return a.causal ? min(max(off + i, prefix - 1), a.Sk - 1) : a.Sk - 1; };
     const int r0 = tile * 4 * WROWS, rw = r0 + wave * WROWS;
     const int wg_hi = bound_of((min(r0 + 4 * WROWS, R) - 1) / G);

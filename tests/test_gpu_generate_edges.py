@@ -144,3 +144,10 @@ def test_cached_values_of_weightless_keys(ctx, S, spare, bad, out16):
         c.append(k[:, :S], v[:, :S], [0])
         got = check_cache(c, q, k, v, [S - 3], [3], have, out16=out16, slopes=np.full(H, 8.0, F32))
         assert np.isfinite(got.astype(F64)).all()
+
+
+def test_prefixes_of_any_number(ctx):
+    """a prefix below zero is none, one past the keys is all of them"""
+    rng = np.random.default_rng(7)
+    q, k, v = qkv(rng, 5, 30, 70, 2, 1, 32)
+    check_masked(ctx, q, k, v, causal=True, prefix=np.array([-2 ** 31, -1, 0, 2 ** 31 - 1, 71], I32))
