@@ -80,7 +80,8 @@ __device__ __forceinline__ int piece_swz(int r) {
 }
 
 // DC 16-feature chunks (D <= 16 DC), QT 16-row tiles per wave, PS: weights as hi + lo; MOD 0: scores times a
-// positive scale, 1: any scale and slopes (0: none), 2: capped, 3: capped with any scale and cap, then slopes.
+// positive scale, 1: any scale and slopes (0: none), 2: capped, weights in fp16, 3: capped with any scale and cap, then
+// slopes.
 // The VALU is the busier unit below 128 features and with a cap (per score two exponentials and a reciprocal, at
 // a quarter of its rate), so MOD 0 and 2 keep the raw scores: both maps rise with them, so the maximum is
 // taken raw, and the reference goes into the map's last fma.
@@ -532,10 +533,12 @@ template <int DC, int QT, bool PS>
 hipError_t launch_masked_t(const MaskedAttnArgs& a, int splits, hipStream_t s) {
     const int tiles = (int)(((int64_t)a.Sq * (a.H / a.Hkv) + 64 * QT - 1) / (64 * QT));
     const dim3 grid((unsigned)((int64_t)tiles * splits * a.Hkv * a.B));
-    if (a.mod.cap2 != 0.f && (a.slopes || !(a.mod.cap_in > 0.f) || a.mod.cap_x != 0.f))
+    const bool capped = a.mod.cap2 != 0.f;
+    if (capped && (PS || a.slopes || !(a.mod.cap_in > 0.f) || a.mod.cap_x != 0.f))
         hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 3>), grid, dim3(256), 0, s, a, tiles, splits);
-    else if (a.mod.cap2 != 0.f) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
-    else if (a.slopes || !(a.mod.scale2 > 0.f)) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 1>), grid, dim3(256), 0, s, a, tiles, splits);
+    else if (capped) {
+        if constexpr (!PS) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
+    } else if (a.slopes || !(a.mod.scale2 > 0.f)) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 1>), grid, dim3(256), 0, s, a, tiles, splits);
     else hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 0>), grid, dim3(256), 0, s, a, tiles, splits);
     return hipGetLastError();
 }

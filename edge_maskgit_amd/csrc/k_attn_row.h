@@ -14,9 +14,9 @@
 namespace mgh {
 
 // The score in log2 units from q . k. tanh(x) = 1 - 2 / (exp(2x) + 1): exp2 of an overflowing argument
-// is inf (its reciprocal 0: +cap), of an underflowing one 0 (-cap). The hardware's exp2 and reciprocal
-// are 1 ulp off; near zero the difference costs an absolute 1.2e-7 cap, so with large caps |x| < 1/4 takes
-// tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 (what is left out: 8e-9 of it).
+// is inf (its reciprocal 0: +cap), of an underflowing one 0 (-cap). Argument, exp2, sum, reciprocal and fma, a step
+// or half of one each, leave an absolute 6 2^-24 cap. Where that shows (score_mod) |x| < 1/4 takes
+// tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 (what is left out: 8e-9 of it), off by 10 2^-24 of the score.
 __device__ __forceinline__ float cap_score(float s, const ScoreMod& m) {
     const float e = __builtin_amdgcn_exp2f(s * m.cap_in);
     float y = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * m.cap2, m.cap2);

@@ -1241,7 +1241,7 @@ int check_scores(mgh_ctx* c, const char* fn, int D, int H, int Hkv, float scale,
     if (D <= 0 || D % 16 || D > 128) return fail(c, MGH_ERR_UNSUPPORTED, f + ": D must be a multiple of 16 up to 128");
     if (!(scale - scale == 0.f)) return fail(c, MGH_ERR_ARG, f + ": scale must be finite");
     if (!(cap >= 0.f) || cap - cap != 0.f) return fail(c, MGH_ERR_ARG, f + ": cap must be finite and >= 0");
-    const mgh::ScoreMod m = mgh::score_mod(scale, cap);
+    const mgh::ScoreMod m = mgh::score_mod(scale, cap, o16 != nullptr);
     if (m.scale2 - m.scale2 != 0.f || m.cap_in - m.cap_in != 0.f || m.cap2 - m.cap2 != 0.f)
         return fail(c, MGH_ERR_ARG, f + ": scale or cap is past what fp32 scores can hold");
     if ((o != nullptr) == (o16 != nullptr)) return fail(c, MGH_ERR_ARG, f + ": exactly one of d_o and d_o16 is needed");
@@ -1319,7 +1319,7 @@ int mgh_attn_masked(mgh_ctx* c, const void* q, const void* k, const void* v, int
     for (int i = 0; i < 4; i++) a.ost[i] = ost ? ost[i] : packed[i];
     a.D = D; a.Sq = Sq; a.Sk = Sk; a.H = H; a.Hkv = Hkv; a.B = B;
     a.causal = op.causal != 0;
-    a.mod = mgh::score_mod(scale, op.cap);
+    a.mod = mgh::score_mod(scale, op.cap, o16 != nullptr);
     a.slopes = op.d_slopes; a.prefix = op.d_prefix; a.docs = op.d_docs; a.doc_stride = op.doc_stride;
     a.vec_o = o16 ? rows_aligned(o16, a.ost, 4, 8) : rows_aligned(o, a.ost, 4, 16);
     if (int r = set_dev(c)) return r;
@@ -1418,7 +1418,7 @@ int mgh_kv8_attn(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const
         return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn: at most 65535 heads and 2^24 rows of a key head");
     a.q = q; a.o = o; a.o16 = (_Float16*)o16; a.S = S; a.H = H; a.in16 = in_f16 != 0;
     a.lens = lens; a.fresh = fresh; a.slopes = slopes;
-    a.mod = mgh::score_mod(scale, cap);
+    a.mod = mgh::score_mod(scale, cap, o16 != nullptr);
     const int64_t packed[4] = {1, kv->D, (int64_t)kv->D * S, (int64_t)kv->D * S * H};
     for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.ost[i] = ost ? ost[i] : packed[i];
     a.vec_q = in_f16 && rows_aligned(q, qst, 8, 16);

@@ -286,12 +286,14 @@ struct ScoreMod {
     float cap2;            // cap log2(e); 0: not capped
     float cap_x;           // scale / cap where small arguments of the tanh need their own form, else 0
 };
-// Near zero the quotient's form is off by an absolute 1.2e-7 of the cap, which a cap past 64 no longer hides: from
-// there on small arguments take the series.
+// Near zero the quotient's form is off by an absolute 6 2^-24 of the cap, however small the score: 1.8e-5 of a score
+// below a cap of 50. Weights that are rounded to 11 bits (an fp16 output) hide that up to a cap of 64. Past it, and
+// wherever weights keep 22 bits (an fp32 output), small arguments take the series, at twice the vector operations.
 constexpr float kFineCap = 64.f;
-inline ScoreMod score_mod(float scale, float cap) {
+inline ScoreMod score_mod(float scale, float cap, bool out16) {
     if (!(cap > 0.f)) return {scale * kLog2e, 0.f, 0.f, 0.f};
-    return {scale * kLog2e, (float)(2.0 * scale * 1.4426950408889634 / cap), cap * kLog2e, cap > kFineCap ? scale / cap : 0.f};
+    const bool fine = !out16 || cap > kFineCap;
+    return {scale * kLog2e, (float)(2.0 * scale * 1.4426950408889634 / cap), cap * kLog2e, fine ? scale / cap : 0.f};
 }
 struct MaskedAttnArgs {
     const void* q;         // fp16 rows, 16-byte aligned, features in order; element strides for d, s, h, b

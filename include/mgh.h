@@ -395,7 +395,8 @@ int mgh_decode_step(mgh_ctx* ctx, void* d_state, void* d_work, const float* d_lo
  *      o = softmax over the seen keys, times v; a row that sees none, or only scores of -infinity, is 0.
  *      What masked keys hold, infinities and NaN included, does not matter, nor does the value of a key
  *      whose weight is zero (below 2^-126 of the row's largest). Sums and softmax in fp32; with an fp16 output the weights are rounded to
- *      fp16 before they meet v, with an fp32 output they keep 22 bits.
+ *      fp16 before they meet v, with an fp32 output they keep 22 bits. A capped score is off by at most 6 2^-24 cap, and with
+ *      an fp32 output or a cap past 64 by 10 2^-24 of itself where it lies below a quarter of the cap.
  *      D a multiple of 16 up to 128; Sk and Sq H / Hkv up to 2^24, H and B up to 65535, and Hkv B ceil(Sq
  *      (H / Hkv) / 64) below 2^22. The output overlaps no input. Rows that are not fp16, 16-byte aligned (pointers and all
  *      strides but the first) with unit feature stride are first packed into the context's scratch,
