@@ -297,9 +297,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                 }
             }
             __builtin_amdgcn_s_setprio(0);
-            // the results are in their registers before a branch looks at them
             __builtin_amdgcn_sched_barrier(0);
-            asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
             constexpr float kHidden = MOD == 2 ? kMasked : -INFINITY;
             const bool edge = k0 + kMaskKeys - 1 > w_lo, part = edge || !same;
             if (edge) {
