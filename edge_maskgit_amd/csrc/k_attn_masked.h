@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (MOD & 1) {
+            auto mapped = [&](auto map) {            // scores of the map, then slopes
 #pragma unroll
                 for (int t = 0; t < QT; t++) {
                     const float d0 = pos[t] - (float)(k0 + 4 * lg);      // (whole numbers below 2^24 throughout)
@@ -292,9 +292,23 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const float d = fabsf(d0 - (float)(16 * n + r));
-                            sc[t][n][r] = MOD == 3 ? fmaf(-slope2[t], d, cap_score(sc[t][n][r], a.mod)) : fmaf(sc[t][n][r], scale2, -slope2[t] * d);
+                            sc[t][n][r] = MOD == 3 ? fmaf(-slope2[t], d, map(sc[t][n][r])) : fmaf(sc[t][n][r], scale2, -slope2[t] * d);
                         }
                 }
+            };
+            if (MOD == 3) {                          // the series alone where the whole tile's scores are small
+                float big = 0.f;
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        big = fmaxf(fmaxf(big, fabsf(sc[t][n][0])), fabsf(sc[t][n][1]));
+                        big = fmaxf(fmaxf(big, fabsf(sc[t][n][2])), fabsf(sc[t][n][3]));
+                    }
+                if (all_small(big, a.mod)) mapped([&](float x) { return cap_small(x, a.mod); });
+                else mapped([&](float x) { return cap_score(x, a.mod); });
+            } else if (MOD == 1) {
+                mapped([](float x) { return x; });
             }
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
