@@ -43,11 +43,19 @@ struct CacheSrc {
             const int64_t page = page_of(c, b, (int)(j / kKvBlock));
             if (page < 0) return __builtin_nanf("");
             const uint8_t* k = c.k + ((page * c.Hkv + hk) * kKvBlock + j % kKvBlock) * c.D;
-            for (int d = 0; d < c.D; d++) s = fmaf(qs[d], (float)((int)k[d] - 128), s);
+            for (int d = 0; d < c.D; d += 16) {
+                const u32x4 x = *(const u32x4*)(k + d);
+#pragma unroll
+                for (int i = 0; i < 16; i++) s = fmaf(qs[d + i], (float)((int)(x[i >> 2] >> (8 * (i & 3)) & 255) - 128), s);
+            }
             return s * c.scales[(page * c.Hkv + hk) * 2];
         }
         const _Float16* k = c.k_tail + (((int64_t)b * c.Hkv + hk) * kKvRing + j % kKvRing) * c.D;
-        for (int d = 0; d < c.D; d++) s = fmaf(qs[d], (float)k[d], s);
+        for (int d = 0; d < c.D; d += 8) {
+            const f16x8 x = *(const f16x8*)(k + d);
+#pragma unroll
+            for (int i = 0; i < 8; i++) s = fmaf(qs[d + i], (float)x[i], s);
+        }
         return s;
     }
     __device__ float value(int64_t j, int d) const {
@@ -167,22 +175,43 @@ __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a
         }
         const int j0 = blk * kKvBlock + 8 * lg;              // this lane's keys: j0 + 4 n + r
         const float scale = ks * (MOD && a.mod.cap2 != 0.f ? 1.f : a.mod.scale2);
+        auto mapped = [&](auto map) {                        // scores of the map, then slopes (of the keys that a row sees)
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                const float d0 = (float)(lim[t] - j0);
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float s = map(sc[t][n][r] * scale);
+                        sc[t][n][r] = MOD ? fmaf(-slope2[t], d0 - (float)(4 * n + r), s) : s;
+                    }
+            }
+        };
+        if (MOD && a.mod.cap2 != 0.f) {
+            float big = 0.f;
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    big = fmaxf(fmaxf(big, fabsf(sc[t][n][0])), fabsf(sc[t][n][1]));
+                    big = fmaxf(fmaxf(big, fabsf(sc[t][n][2])), fabsf(sc[t][n][3]));
+                }
+            if (all_small(big * scale, a.mod)) mapped([&](float x) { return cap_small(x, a.mod); });
+            else mapped([&](float x) { return cap_score(x, a.mod); });
+        } else {
+            mapped([](float x) { return x; });
+        }
         float mx[QT];
         bool any = false;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             mx[t] = -INFINITY;
-            const float d0 = (float)(lim[t] - j0);
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    float s = sc[t][n][r] * scale;
-                    if (MOD) {
-                        if (a.mod.cap2 != 0.f) s = cap_score(s, a.mod);
-                        s = fmaf(-slope2[t], d0 - (float)(4 * n + r), s);     // (of the keys that it sees)
-                    }
-                    s = j0 + 4 * n + r > lim[t] ? -INFINITY : s;
+                    const float s = j0 + 4 * n + r > lim[t] ? -INFINITY : sc[t][n][r];
                     sc[t][n][r] = s;
                     mx[t] = fmaxf(mx[t], s);
                 }
