@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from tests import gen_oracle as ref
-from tests.test_gpu_generate import Cache, Dev, cache_case, check_cache, check_masked, close, ctx, qkv, run_masked  # noqa: F401
+from tests.test_gpu_generate import Cache, Dev, cache_case, check_cache, check_masked, close, ctx, qkv, run_masked, tokens  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 F16, F32, F64, I32 = np.float16, np.float32, np.float64, np.int32
@@ -151,3 +151,97 @@ def test_prefixes_of_any_number(ctx):
     rng = np.random.default_rng(7)
     q, k, v = qkv(rng, 5, 30, 70, 2, 1, 32)
     check_masked(ctx, q, k, v, causal=True, prefix=np.array([-2 ** 31, -1, 0, 2 ** 31 - 1, 71], I32))
+
+
+# ---- sequences that a call refuses, in parts ----------------------------------------------
+
+
+@pytest.mark.parametrize("spare", [10, 900])
+@pytest.mark.parametrize("S", [1, 4])
+def test_cache_refuses_bad_numbers_in_parts(ctx, spare, S):
+    """refused, ragged and good sequences, and pages outside the pool in an early and in a late part"""
+    print(f"refused in parts {spare} {S}", flush=True)
+    rng = np.random.default_rng(spare + S)
+    H, Hkv, D = 4, 2, 48
+    lens, new = [1500, 1500, 1200, 40, 900, 7], [S, S, S, max(S - 2, 0), S, S]
+    with Dev(ctx) as dev:
+        c, q, k, v, have = cache_case(dev, rng, lens, new, H, Hkv, D, spare=spare)
+        for out16 in (True, False):
+            want = check_cache(c, q, k, v, lens, new, have, out16=out16)
+            before = c.state()
+            good = c.table
+            table = good.copy()
+            table[0, 45], table[1, 0], table[2, 20], table[4, 29:], table[3, 2:] = c.pages, -1, -2 ** 31, -7, -7
+            c.set_table(table)
+            got = c.attend(q, lens, new, out16=out16)
+            # sequence 4's last whole block is number 27, sequence 3's 0: what lies behind is not read
+            assert np.isnan(got[:3]).all() and np.array_equal(got[3:], want[3:])
+            c.set_table(good)
+            bad = [lens[0], -1, 32 * c.nb, lens[3], 2 ** 31 - 1, lens[5]]
+            n = [S + 1, S, S, new[3], S, -1]
+            for cap in (0.0, 9.0):
+                got = c.attend(q, bad, n, out16=out16, cap=cap)
+                assert np.isnan(got[[0, 1, 2, 4, 5]]).all()
+                assert (got[3, new[3]:] == 7).all() and np.isfinite(got[3].astype(F64)).all()
+            assert np.array_equal(c.attend(q, bad, n, out16=out16)[3], want[3])
+            c.append(k[:, :S], v[:, :S], bad, [n[0], n[1], n[2], 0, n[4], n[5]])
+            for x, y in zip(c.state(), before):
+                assert np.array_equal(x, y, equal_nan=x.dtype != np.uint8)
+
+
+# ---- together -----------------------------------------------------------------------------
+
+
+def test_drafted_tokens_are_taken_back(ctx):
+    """a prompt, then drafted tokens of which some are kept, again and again, eager and replayed: the cache and the
+    rows are those of the tokens kept"""
+    rng = np.random.default_rng(9)
+    B, H, Hkv, D, S, P = 2, 4, 2, 48, 5, 37
+    n = 150
+    k, v = tokens(rng, B, n, Hkv, D)
+    with Dev(ctx) as dev:
+        c = Cache(dev, B, Hkv, D, 6, rng)
+        c.append(k[:, :P], v[:, :P], [0, 0])
+        have = np.array([P, P])
+        lens = dev.up(have, I32)
+        dk, dv, dq = (dev.up(np.zeros((B, S, h, D), F16)) for h in (Hkv, Hkv, H))
+        o, st, kst = dev.up(np.zeros((B, S, H, D), F32)), (1, H * D, D, S * H * D), (1, Hkv * D, D, S * Hkv * D)
+
+        def step():
+            ctx.kv8_append(c.h, dk, dv, kst, S, lens)
+            ctx.kv8_attn(c.h, dq, st, S, lens, None, H, 0.2, o=o, o_strides=st)
+
+        graph = None
+        for t in range(18):
+            keep = rng.integers(0, S + 1, B)
+            rows = [np.stack([x[b, have[b]:have[b] + S] for b in range(B)]) for x in (k, v)]
+            for x in rows:                                                # the tokens not kept are other ones
+                for b in range(B):
+                    x[b, keep[b]:] = rng.standard_normal((S - keep[b], Hkv, D))
+            q = rng.standard_normal((B, S, H, D)).astype(F16)
+            for d, x in ((dk, rows[0]), (dv, rows[1]), (dq, q)):
+                ctx.write(d, x)
+            if t == 1:
+                ctx.graph_begin()
+                step()
+                graph = ctx.graph_end()
+            graph.launch() if graph else step()
+            got = dev.get(o, (B, S, H, D), F32)
+            for b in range(B):
+                kk = np.concatenate([k[b, :have[b]], rows[0][b]])
+                vv = np.concatenate([v[b, :have[b]], rows[1][b]])
+                kk, vv, m = ref.cache_values(kk), ref.cache_values(vv), have[b] + S
+                tol, rel = ref.bound(q[b:b + 1], kk[None], vv[None], 0.2)
+                for i in range(S):
+                    for h in range(H):
+                        want = ref.attention_row(q[b, i, h].astype(F64), kk[:, h // 2], vv[:, h // 2], 0.2, 0.0, None, have[b] + i,
+                                                 np.arange(m) <= have[b] + i)
+                        close(got[b, i, h], want, tol, rel)
+            ctx.kv8_advance(lens, dev.up(keep, I32), B, S)
+            have = have + keep
+        assert dev.get(lens, B, I32).tolist() == have.tolist()
+        rk, rv = c.read(have, n)
+        for b in range(B):
+            for got, x in ((rk, k), (rv, v)):
+                assert np.array_equal(got[b, :, :have[b]], ref.cache_values(x[b, :have[b]]).astype(F32).transpose(1, 0, 2))
+        graph.destroy()
