@@ -13,7 +13,10 @@
 //  * The softmax reference of a row stays within [-7, 15] (log2 units) of its maximum: it moves, and O is
 //    rescaled, only when a score passes it by 15, a wave-uniform branch. Weights lie in fp16's normal
 //    range up to 2^15; with an fp32 output (PS) a weight is hi + lo in fp16, both to nearest, and a
-//    chunk's products are summed apart from O.
+//    chunk's products are summed apart from O. With an fp16 output a weight is fp16: over thousands of keys the
+//    outputs are then 2.3-2.8e-4 off (relative, root mean square) where their own rounding alone makes 2.1e-4, and
+//    lo would take 40-50% longer (two rows of 4097 tokens, 16 heads of 64, 283 us against 189; 4097 tokens, 32
+//    heads on 8 of 128, 452 against 330).
 //  * Which keys a row sees is one bound per row (causal and prefix together), known per wave, so that whole
 //    chunks need no test; ids of documents are compared only in chunks where they can differ: a first
 //    pass over the ids notes for each chunk whether any row of the workgroup can see it and whether all
@@ -22,12 +25,14 @@
 // again by attn_row, which uses what a row sees and nothing else. Rows whose sum of weights is not finite too: they may
 // have seen no NaN, but weights past fp16, which a moving reference then multiplied by 0: all that a row saw of a
 // chunk were infinite products at the lower end of a cap, or scores past 1e8 lie farther apart than the
-// reference's distance. Two rows of 4097 tokens in documents, NaN behind them: 1.1 ms against 0.06. Values
-// that no row of the workgroup sees zeroed in LDS would make that 0.06 too, but cost every call 4-5%.
+// reference's distance. Two rows of 4097 tokens in nine documents each, 197 places of NaN behind them: 3.5 ms against
+// 0.075, the time of the last documents' rows, whose keys end in a chunk with NaN. Values that no row of the workgroup
+// sees zeroed in LDS would make that 0.075 too, but cost every call 4-5%.
 //
-// Measured: 16 heads of 64, 2 x 4097 tokens 177 us (780 TFLOP/s); 32 heads on 8 of 128, 512 rows of each of two
-// prompts of 12345 in 199 us (1.0 PFLOP/s; MFMA busy 44%, VALU 36% of the peak clock's cycles), 8191 tokens capped 640
-// (870 TFLOP/s: two exponentials and a reciprocal per score); one row of 8000 keys, 8 sequences: 53 us, 4.9 TB/s.
+// Measured: 16 heads of 64, 2 x 4096 tokens 173 us (794 TFLOP/s), 2 x 4097 189: the last row's workgroups are a
+// round of their own (32 heads of 128: 266, 333); 32 heads on 8 of 128, 512 rows of each of two
+// prompts of 12345 in 207 us (980 TFLOP/s), 8191 tokens causal with a prefix of 1000 530, capped 660
+// (840 TFLOP/s: two exponentials and a reciprocal per score); one row of 8000 keys, 8 sequences: 53 us, 4.9 TB/s.
 // Tiles of 32 rows on v_mfma_f32_32x32x16_f16 (half the softmax state) ran 3-11% longer.
 #pragma once
 #include <type_traits>
@@ -81,7 +86,7 @@ __device__ __forceinline__ int piece_swz(int r) {
 
 // DC 16-feature chunks (D <= 16 DC), QT 16-row tiles per wave, PS: weights as hi + lo; MOD 0: scores times a
 // positive scale, 1: any scale and slopes (0: none), 2: capped, weights in fp16, 3: capped with any scale and cap, then
-// slopes.
+// slopes; small scores by the series (4097 tokens, cap 50, fp32 output 610 us; the quotient for all 550, both for all 722).
 // The VALU is the busier unit below 128 features and with a cap (per score two exponentials and a reciprocal, at
 // a quarter of its rate), so MOD 0 and 2 keep the raw scores: both maps rise with them, so the maximum is
 // taken raw, and the reference goes into the map's last fma.

@@ -288,7 +288,7 @@ struct ScoreMod {
 };
 // Near zero the quotient's form is off by an absolute 6 2^-24 of the cap, however small the score: 1.8e-5 of a score
 // below a cap of 50. Weights that are rounded to 11 bits (an fp16 output) hide that up to a cap of 64. Past it, and
-// wherever weights keep 22 bits (an fp32 output), small arguments take the series, at twice the vector operations.
+// wherever weights keep 22 bits (an fp32 output), small arguments take the series.
 constexpr float kFineCap = 64.f;
 inline ScoreMod score_mod(float scale, float cap, bool out16) {
     if (!(cap > 0.f)) return {scale * kLog2e, 0.f, 0.f, 0.f};

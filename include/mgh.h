@@ -395,13 +395,15 @@ int mgh_decode_step(mgh_ctx* ctx, void* d_state, void* d_work, const float* d_lo
  *      o = softmax over the seen keys, times v; a row that sees none, or only scores of -infinity, is 0.
  *      What masked keys hold, infinities and NaN included, does not matter, nor does the value of a key
  *      whose weight is zero (below 2^-126 of the row's largest). Sums and softmax in fp32; with an fp16 output the weights are rounded to
- *      fp16 before they meet v, with an fp32 output they keep 22 bits. A capped score is off by at most 6 2^-24 cap, and with
- *      an fp32 output or a cap past 64 by 10 2^-24 of itself where it lies below a quarter of the cap.
+ *      fp16 before they meet v, with an fp32 output they keep 22 bits (at 1.4 to 1.5 times the time of long calls). A
+ *      capped score is off by at most 6 2^-24 cap, and with an fp32 output or a cap past 64 by 10 2^-24 of itself where it
+ *      lies below a quarter of the cap. How keys are split among workgroups goes by the whole call's shape, so the last
+ *      bits of a sequence's rows may differ with the number of sequences in the call.
  *      D a multiple of 16 up to 128; Sk and Sq H / Hkv up to 2^24, H and B up to 65535, and Hkv B ceil(Sq
  *      (H / Hkv) / 64) below 2^22. The output overlaps no input. Rows that are not fp16, 16-byte aligned (pointers and all
- *      strides but the first) with unit feature stride are first packed into the context's scratch,
- *      and calls with few rows keep partial results in its workspace: run a shape once before it is
- *      captured. */
+ *      strides but the first) with unit feature stride are first packed into the context's scratch (at most 32 GiB
+ *      each of q, k and v), and calls with few rows keep partial results in its workspace: run a shape once before
+ *      it is captured. */
 typedef struct mgh_attn_opts {
     float cap;                   /* 0: none */
     int causal;
@@ -428,7 +430,8 @@ int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* 
  *                 t at t % 64. The tokens behind the last whole block are read from here; a block gets
  *                 its codes from here once its 32 tokens are there. So the cache does not depend on how
  *                 tokens were grouped into calls, and a sequence may be shortened (its length lowered)
- *                 to 32 tokens below the longest that it has been.
+ *                 to 32 tokens below the longest that it has been, but not below where it was put on shared pages:
+ *                 the ring has only what was appended to this sequence.
  *      d_lens [B] holds each sequence's length before the step, d_new [B] its new tokens, 0 .. S (NULL:
  *      S each): append writes them at positions lens[b] + i, attention takes them as queries at those
  *      positions (each sees the cache up to its own position), and after the last layer mgh_kv8_advance
@@ -463,7 +466,9 @@ int mgh_kv8_append(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_k, const vo
  * length past it: set that back before the table is made wider. */
 int mgh_kv8_advance(mgh_ctx* ctx, int32_t* d_lens, const int32_t* d_new, int B, int S);
 /* q, o: {D, S, H, B} views, scores as mgh_attn_masked (cap, d_slopes [H] or NULL); calls with few rows keep
- * partial results in the context's workspace: run a shape once before it is captured */
+ * partial results in the context's workspace: run a shape once before it is captured. The parts that a sequence is
+ * taken in go by B, S and max_blocks, so the last bits of its rows may differ with these (not with its own
+ * place or the other sequences' lengths). */
 int mgh_kv8_attn(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_q, int in_f16, const int64_t q_strides[4], int S,
                  const int32_t* d_lens, const int32_t* d_new, int H, float scale, float cap, const float* d_slopes,
                  float* d_o, void* d_o16, const int64_t o_strides[4]);

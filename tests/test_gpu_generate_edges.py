@@ -245,3 +245,36 @@ def test_drafted_tokens_are_taken_back(ctx):
             for got, x in ((rk, k), (rv, v)):
                 assert np.array_equal(got[b, :, :have[b]], ref.cache_values(x[b, :have[b]]).astype(F32).transpose(1, 0, 2))
         graph.destroy()
+
+
+@pytest.mark.parametrize("spare", [1, 10, 900])
+def test_a_sequence_does_not_depend_on_the_others(ctx, spare):
+    """the same bits at another place of a batch of the same shape, beside sequences of other lengths"""
+    rng = np.random.default_rng(spare)
+    H, Hkv, D, S = 4, 2, 48, 3
+    lens, new = np.array([700, 40, 1200]), np.array([3, 1, 2])
+    with Dev(ctx) as dev:
+        c, q, k, v, have = cache_case(dev, rng, list(lens), list(new), H, Hkv, D, spare=spare)
+        for kw in ({}, {"cap": 9.0, "slopes": np.full(H, 0.05, F32)}):
+            for out16 in (True, False):
+                want = c.attend(q, lens, new, out16=out16, **kw)
+                at = np.array([2, 0, 1])
+                tails = (c.kt, c.vt)
+                one = [dev.get(x, c.B * Hkv * 64 * D, F16).reshape(c.B, -1)[at] for x in tails]
+                c.kt, c.vt = dev.up(one[0]), dev.up(one[1])
+                c.set_table(c.table[at])
+                got = c.attend(q[at], lens[at], new[at], out16=out16, **kw)
+                assert np.array_equal(got, want[at])
+                short = lens[at].copy()
+                short[0], short[2] = 0, 7                                 # (their own rows are other ones)
+                got = c.attend(q[at], short, new[at], out16=out16, **kw)
+                assert np.array_equal(got[1], want[at][1])
+                c.kt, c.vt = tails
+                c.set_table(c.table)
+    q, k, v = qkv(rng, 3, 70, 300, H, Hkv, D)
+    docs = np.sort(rng.integers(0, 4, (3, 300)).astype(I32), 1)
+    want = run_masked(ctx, q, k, v, docs=docs, causal=True)
+    at = np.array([1, 2, 0])
+    assert np.array_equal(run_masked(ctx, q[at], k[at], v[at], docs=docs[at], causal=True), want[at])
+    docs[1:] = 0
+    assert np.array_equal(run_masked(ctx, q, k, v, docs=docs, causal=True)[0], want[0])
