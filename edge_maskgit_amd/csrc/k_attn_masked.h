@@ -86,7 +86,7 @@ __device__ __forceinline__ int piece_swz(int r) {
 
 // DC 16-feature chunks (D <= 16 DC), QT 16-row tiles per wave, PS: weights as hi + lo; MOD 0: scores times a
 // positive scale, 1: any scale and slopes (0: none), 2: capped, weights in fp16, 3: capped with any scale and cap, then
-// slopes; small scores by the series (4097 tokens, cap 50, fp32 output 610 us; the quotient for all 550, both for all 722).
+// slopes; small scores by a form of their own (4097 tokens, 32 heads on 8 of 128, cap 50, fp32 output 594 us, 547 without it).
 // The VALU is the busier unit below 128 features and with a cap (per score two exponentials and a reciprocal, at
 // a quarter of its rate), so MOD 0 and 2 keep the raw scores: both maps rise with them, so the maximum is
 // taken raw, and the reference goes into the map's last fma.
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            auto mapped = [&](auto map) {            // scores of the map, then slopes
+            auto mapped = [&](auto map, auto sloped) {           // scores of the map, then slopes
 #pragma unroll
                 for (int t = 0; t < QT; t++) {
                     const float d0 = pos[t] - (float)(k0 + 4 * lg);      // (whole numbers below 2^24 throughout)
@@ -297,11 +297,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const float d = fabsf(d0 - (float)(16 * n + r));
-                            sc[t][n][r] = MOD == 3 ? fmaf(-slope2[t], d, map(sc[t][n][r])) : fmaf(sc[t][n][r], scale2, -slope2[t] * d);
+                            if (MOD == 1) sc[t][n][r] = fmaf(sc[t][n][r], scale2, -slope2[t] * d);
+                            else sc[t][n][r] = decltype(sloped)::value ? fmaf(-slope2[t], d, map(sc[t][n][r])) : map(sc[t][n][r]);
                         }
                 }
             };
-            if (MOD == 3) {                          // the series alone where the whole tile's scores are small
+            if (MOD == 3) {                          // their form alone where all of the tile's scores are small
                 float big = 0.f;
 #pragma unroll
                 for (int t = 0; t < QT; t++)
@@ -310,10 +311,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_masked(MaskedAttnArgs a, int ti
                         big = fmaxf(fmaxf(big, fabsf(sc[t][n][0])), fabsf(sc[t][n][1]));
                         big = fmaxf(fmaxf(big, fabsf(sc[t][n][2])), fabsf(sc[t][n][3]));
                     }
-                if (all_small(big, a.mod)) mapped([&](float x) { return cap_small(x, a.mod); });
-                else mapped([&](float x) { return cap_score(x, a.mod); });
+                auto small = [&](float x) { return cap_small(x, a.mod); };
+                if (!all_small(big, a.mod)) mapped([&](float x) { return cap_score(x, a.mod); }, std::true_type{});
+                else if (a.slopes) mapped(small, std::true_type{});
+                else mapped(small, std::false_type{});
             } else if (MOD == 1) {
-                mapped([](float x) { return x; });
+                mapped([](float x) { return x; }, std::true_type{});
             }
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
@@ -550,11 +553,12 @@ template <int DC, int QT, bool PS>
 hipError_t launch_masked_t(const MaskedAttnArgs& a, int splits, hipStream_t s) {
     const int tiles = (int)(((int64_t)a.Sq * (a.H / a.Hkv) + 64 * QT - 1) / (64 * QT));
     const dim3 grid((unsigned)((int64_t)tiles * splits * a.Hkv * a.B));
-    const bool capped = a.mod.cap2 != 0.f;
-    if (capped && (PS || a.slopes || !(a.mod.cap_in > 0.f) || a.mod.cap_x != 0.f))
-        hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 3>), grid, dim3(256), 0, s, a, tiles, splits);
-    else if (capped) {
-        if constexpr (!PS) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
+    constexpr bool kCapped = QT == 1 || DC > 4;      // (masked_plan takes one tile for capped scores of up to 64 features)
+    if (a.mod.cap2 != 0.f) {
+        const bool fine = PS || a.slopes || !(a.mod.cap_in > 0.f) || a.mod.cap_x != 0.f;
+        if constexpr (!kCapped) return hipErrorInvalidValue;
+        else if (fine) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 3>), grid, dim3(256), 0, s, a, tiles, splits);
+        else if constexpr (!PS) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 2>), grid, dim3(256), 0, s, a, tiles, splits);
     } else if (a.slopes || !(a.mod.scale2 > 0.f)) hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 1>), grid, dim3(256), 0, s, a, tiles, splits);
     else hipLaunchKernelGGL((k_attn_masked<DC, QT, PS, 0>), grid, dim3(256), 0, s, a, tiles, splits);
     return hipGetLastError();

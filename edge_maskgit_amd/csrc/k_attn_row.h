@@ -15,20 +15,23 @@ namespace mgh {
 
 // The score in log2 units from q . k. tanh(x) = 1 - 2 / (exp(2x) + 1): exp2 of an overflowing argument
 // is inf (its reciprocal 0: +cap), of an underflowing one 0 (-cap). Argument, exp2, sum, reciprocal and fma, a step
-// or half of one each, leave an absolute 6 2^-24 cap. Where that shows (score_mod) |x| < 1/4 takes
-// tanh x = x - x^3/3 + 2 x^5/15 - 17 x^7/315 + 62 x^9/2835 (what is left out: 8e-9 of it), off by 10 2^-24 of the score.
+// or half of one each, leave an absolute 6 2^-24 cap. Where that shows (score_mod) |x| < 3/4 takes x + x^3 Q(x^2), Q of
+// degree 4 with the least largest error relative to tanh x (4e-8 with its roundings), in all off by 10 2^-24 of the
+// score; beyond, the quotient is no farther off.
+constexpr float kSmallArg = 0.75f;
 __device__ __forceinline__ float cap_small(float s, const ScoreMod& m) {
     const float x = s * m.cap_x, z = x * x;
-    return m.cap2 * x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    const float q = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -0.0047694925f, 0.019664917f), -0.05339026f), 0.13326521f), -0.3333307f);
+    return m.cap2 * x * fmaf(z, q, 1.f);
 }
 __device__ __forceinline__ float cap_score(float s, const ScoreMod& m) {
     const float e = __builtin_amdgcn_exp2f(s * m.cap_in);
     const float y = fmaf(__builtin_amdgcn_rcpf(e + 1.f), -2.f * m.cap2, m.cap2);
-    return m.cap_x != 0.f && fabsf(s * m.cap_x) < 0.25f ? cap_small(s, m) : y;
+    return m.cap_x != 0.f && fabsf(s * m.cap_x) < kSmallArg ? cap_small(s, m) : y;
 }
 // whether all of a wave's scores, the largest of a lane's |q . k| being `big`, are small ones (a NaN comes out as NaN)
 __device__ __forceinline__ bool all_small(float big, const ScoreMod& m) {
-    return m.cap_x != 0.f && __all(big * fabsf(m.cap_x) < 0.25f);
+    return m.cap_x != 0.f && __all(big * fabsf(m.cap_x) < kSmallArg);
 }
 
 // The reference of a row that has seen nothing: below every finite score in sight, and finite

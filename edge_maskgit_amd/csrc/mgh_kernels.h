@@ -284,11 +284,11 @@ struct ScoreMod {
     float scale2;          // scale log2(e)
     float cap_in;          // 2 scale log2(e) / cap
     float cap2;            // cap log2(e); 0: not capped
-    float cap_x;           // scale / cap where small arguments of the tanh need their own form, else 0
+    float cap_x;           // scale / cap where arguments of the tanh below 3/4 need their own form, else 0
 };
 // Near zero the quotient's form is off by an absolute 6 2^-24 of the cap, however small the score: 1.8e-5 of a score
 // below a cap of 50. Weights that are rounded to 11 bits (an fp16 output) hide that up to a cap of 64. Past it, and
-// wherever weights keep 22 bits (an fp32 output), small arguments take the series.
+// wherever weights keep 22 bits (an fp32 output), arguments below 3/4 take a form of their own.
 constexpr float kFineCap = 64.f;
 inline ScoreMod score_mod(float scale, float cap, bool out16) {
     if (!(cap > 0.f)) return {scale * kLog2e, 0.f, 0.f, 0.f};

@@ -73,14 +73,15 @@ def row_tolerance(q, k, v, scale, cap=0.0, slope=None, p=0, seen=None, out16=Fal
 
     Score j: products of fp16 values are exact in fp32; the matrix unit may lose a whole step (2^-23) per
     addition of the sum of the terms that are not zero, of their magnitudes. Scaling it, with the constants'
-    own roundings, is four roundings (2^-24); the cap six of the cap (tanh = 1 - 2 r, r = 1 / (e + 1), at
-    x = s / cap >= 1/4: r itself one, e's step and its argument's two roundings 2 r (1 - r) of theirs, at most 0.94 and
-    0.9, the sum e + 1 0.75, the last fma and the constant one each, together 5.6), or below cap / 4, by its series,
-    ten of the score; with an fp16 output up to a cap of 64 the former throughout; the slope and the subtraction of the reference (within 15 log2 units of the maximum) one each of
-    what they give. A weight's exponential is off by a step, and hi + lo in fp16 by 2^-22 of it (fp16: 2^-11), with 2^-32
-    of the row's largest weight where lo leaves fp16's normal numbers. An error e_j of the weights p_j (sum 1)
-    moves the output by sum p_j e_j (v_j - o). The sums: a step per addition that a term goes through, of the terms'
-    magnitudes (64 keys, hi and lo, at a time, then chunk by chunk, waves and parts)."""
+    own roundings, is four roundings (2^-24). The cap is six of the cap (tanh = 1 - 2 r, r = 1 / (e + 1), at
+    x = s / cap >= 1/4: r itself one, e's step and its argument's two roundings 2 r (1 - r) of theirs, at most 0.94
+    and 0.9, the sum e + 1 0.75, the last fma and the constant one each, together 5.6, below that no more), or where
+    |x| < 3/4 ten of the score; with an fp16 output up to a cap of 64 the former throughout. The slope and the
+    subtraction of the reference (within 15 log2 units of the maximum) are one each of what they give. A weight's
+    exponential is off by a step, and hi + lo in fp16 by 2^-22 of it (fp16: 2^-11), with 2^-32 of the row's largest
+    weight where lo leaves fp16's normal numbers. An error e_j of the weights p_j (sum 1) moves the output by
+    sum p_j e_j (v_j - o). The sums: a step per addition that a term goes through, of the terms' magnitudes (64 keys,
+    hi and lo, at a time, then chunk by chunk, waves and parts)."""
     seen = np.ones(len(k), bool) if seen is None else seen
     at = np.nonzero(seen)[0]
     k, v, a = k[at], v[at], abs(float(scale))
@@ -90,7 +91,7 @@ def row_tolerance(q, k, v, scale, cap=0.0, slope=None, p=0, seen=None, out16=Fal
     s = terms.sum(1) * scale
     e = 2 * u * np.maximum(nnz - 1, 0) * mag + 4 * u * raw
     if cap:
-        small = (np.abs(s) < cap / 4.01) & (not out16 or cap > 64)
+        small = (np.abs(s) < 0.74 * cap) & (not out16 or cap > 64)
         s = cap * np.tanh(s / cap)
         e = e + np.where(small, 10 * u * np.abs(s), 6 * u * cap)
     if slope is not None:
