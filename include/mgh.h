@@ -394,11 +394,12 @@ int mgh_decode_step(mgh_ctx* ctx, void* d_state, void* d_work, const float* d_lo
  *        apart, 0: one row for all; negative: padding; a query before position 0 has none).
  *      o = softmax over the seen keys, times v; a row that sees none, or only scores of -infinity, is 0.
  *      What masked keys hold, infinities and NaN included, does not matter, nor does the value of a key
- *      whose weight is zero (below 2^-126 of the row's largest). Sums and softmax in fp32; with an fp16 output the weights are rounded to
- *      fp16 before they meet v, with an fp32 output they keep 22 bits (at 1.4 to 1.5 times the time of long calls). A
- *      capped score is off by at most 6 2^-24 cap, and with an fp32 output or a cap past 64 by 10 2^-24 of itself where it
- *      lies below three quarters of the cap. How keys are split among workgroups goes by the whole call's shape, so the last
- *      bits of a sequence's rows may differ with the number of sequences in the call.
+ *      whose weight is zero (below 2^-126 of the row's largest). Sums and softmax in fp32; with an fp16 output
+ *      the weights are rounded to fp16 before they meet v, with an fp32 output they keep 22 bits (at 1.4 to 1.5
+ *      times the time of long calls). A capped score is off by at most 6 2^-24 cap, and with an fp32 output or
+ *      a cap past 64 by 10 2^-24 of itself where it lies below three quarters of the cap. How keys are split
+ *      among workgroups goes by the whole call's shape, so the last bits of a sequence's rows may differ with
+ *      the number of sequences in the call.
  *      D a multiple of 16 up to 128; Sk and Sq H / Hkv up to 2^24, H and B up to 65535, and Hkv B ceil(Sq
  *      (H / Hkv) / 64) below 2^22. The output overlaps no input. Rows that are not fp16, 16-byte aligned (pointers and all
  *      strides but the first) with unit feature stride are first packed into the context's scratch (at most 32 GiB
