@@ -23,6 +23,7 @@ WTYPE_Q4_K = 12
 ACT_NONE, ACT_GELU, ACT_SILU = 0, 1, 2
 EMIT_NONE, EMIT_INT8, EMIT_DEQ_F16 = 0, 1, 2
 ALGO_AUTO, ALGO_INT8, ALGO_DEQ_F16 = 0, 1, 2
+ROPE_HALVES, ROPE_PAIRS, ROPE_AXIS_HALVES = 0, 1, 2
 
 # every entry point include/mgh.h declares (checked by tests/test_abi.py)
 MGH_SYMBOLS = [
@@ -46,6 +47,7 @@ MGH_SYMBOLS = [
     "mgh_gemm_dq_y16", "mgh_gemm_dq_ln", "mgh_dequant_weights_f32",
     "mgh_attn_masked", "mgh_kv8_code_bytes", "mgh_kv8_scale_bytes", "mgh_kv8_tail_bytes", "mgh_kv8_append",
     "mgh_kv8_advance", "mgh_kv8_attn", "mgh_kv8_read", "mgh_logits_process",
+    "mgh_rope", "mgh_kv8_append_rope", "mgh_kv8_attn_shared", "mgh_sample",
 ]
 
 _lib = None
@@ -156,6 +158,10 @@ def lib():
         L.mgh_kv8_attn.argtypes = [P, P, P, I, P, I, P, P, I, F, F, P, P, P, P]
         L.mgh_kv8_read.argtypes = [P, P, P, I, P, P, P, P, P]
         L.mgh_logits_process.argtypes = [P, P, I, I64, I, I, P, P, I64]
+        L.mgh_rope.argtypes = [P, P, P, I, P, I, I, I, I, P, P, P, P, P]
+        L.mgh_kv8_append_rope.argtypes = [P, P, P, P, P, I, P, I, P, P, P, P, I, P, P]
+        L.mgh_kv8_attn_shared.argtypes = [P, P, P, I, P, I, P, P, I, P, I, I, F, F, P, P, P, P]
+        L.mgh_sample.argtypes = [P, P, I, I64, I, I, P, P, P, P]
         L.mgh_graph_begin.argtypes = [P]
         L.mgh_graph_end.argtypes = [P, ctypes.POINTER(P)]
         L.mgh_graph_launch.argtypes = [P, P]
@@ -237,6 +243,29 @@ class Kv8(ctypes.Structure):
     def __init__(self, k, v, scales, k_tail, v_tail, table, max_blocks, pages, Hkv, D, B, table_stride=None):
         super().__init__(*map(_addr, (k, v, scales, k_tail, v_tail, table)),
                          max_blocks if table_stride is None else table_stride, pages, max_blocks, Hkv, D, B)
+
+
+class Rope(ctypes.Structure):
+    """mgh_rotation: how pairs of features turn with their token's positions (include/mgh.h has the orders). pairs: of each
+    axis; freqs: angle per unit of position of each pair; pos: whole positions (int32) on the device, pos_strides apart
+    (token, sequence, axis), or None: consecutive ones."""
+
+    _fields_ = [("axes", ctypes.c_int), ("pairs", ctypes.c_int * 4), ("order", ctypes.c_int), ("h_freqs", ctypes.c_void_p),
+                ("d_pos", ctypes.c_void_p), ("pos_strides", ctypes.c_int64 * 3)]
+
+    def __init__(self, pairs, freqs, order=ROPE_HALVES, pos=None, pos_strides=(0, 0, 0)):
+        if not 1 <= len(pairs) <= 4:
+            raise MghError("a rotation has 1 to 4 axes")
+        if len(freqs) < sum(pairs):
+            raise MghError("a frequency for every pair is needed")
+        self._freqs = (ctypes.c_double * max(len(freqs), 1))(*freqs)
+        super().__init__(len(pairs), (ctypes.c_int * 4)(*pairs), order, ctypes.addressof(self._freqs), _addr(pos),
+                         (ctypes.c_int64 * 3)(*pos_strides))
+
+
+class _SampleOpts(ctypes.Structure):
+    _fields_ = [("d_temp", ctypes.c_void_p), ("d_top_k", ctypes.c_void_p), ("d_top_p", ctypes.c_void_p),
+                ("d_min_p", ctypes.c_void_p)]
 
 
 def kv8_code_bytes(pages: int, Hkv: int, D: int) -> int:
@@ -586,6 +615,39 @@ class Context:
                          _addr(rep), _addr(freq), _addr(pres), _addr(bias), bias_stride, _addr(allowed), allowed_stride)
         self._check(lib().mgh_logits_process(self.h, self._ptr(x), int(f16), V if x_stride is None else x_stride, rows, V,
                                              ctypes.byref(op), self._ptr(y), V if y_stride is None else y_stride))
+
+    def rope(self, rot, x, x_strides, D, S, H, B, y=None, y16=None, y_strides=None, first=None, new=None, in16=True):
+        """Pairs of features of {D, S, H, B} heads turned by their tokens' positions (a Rope); exactly one of y (fp32) and y16
+        (fp16) is given, y_strides None: as x's."""
+        P = self._ptr
+        self._check(lib().mgh_rope(self.h, ctypes.byref(rot), P(x), int(in16), (ctypes.c_int64 * 4)(*x_strides), D, S, H, B,
+                                   P(first), P(new), P(y), P(y16),
+                                   (ctypes.c_int64 * 4)(*(x_strides if y_strides is None else y_strides))))
+
+    def kv8_append_rope(self, cache, rot, k, v, strides, S, lens, new=None, in16=True, q=None, q_strides=None, H=0, q_out=None,
+                        qo_strides=None):
+        """kv8_append with the keys turned by a Rope on the way, and the H heads of queries q ({D, S, H, B}, as k's type) to
+        fp16 rows in q_out; positions None: lens[b] + i."""
+        P = self._ptr
+        four = lambda st: None if st is None else (ctypes.c_int64 * 4)(*st)  # noqa: E731
+        self._check(lib().mgh_kv8_append_rope(self.h, ctypes.byref(cache), ctypes.byref(rot), P(k), P(v), int(in16), four(strides), S,
+                                              P(lens), P(new), P(q), four(q_strides), H, P(q_out), four(qo_strides)))
+
+    def kv8_attn_shared(self, cache, q, q_strides, S, lens, new, group, shared, max_shared, H, scale, o=None, o16=None,
+                        o_strides=None, in16=True, cap=0.0, slopes=None):
+        """kv8_attn where each `group` sequences in a row share their first shared[g] blocks (at most max_shared), which are
+        read once for all of them."""
+        P = self._ptr
+        ost = None if o_strides is None else (ctypes.c_int64 * 4)(*o_strides)
+        self._check(lib().mgh_kv8_attn_shared(self.h, ctypes.byref(cache), P(q), int(in16), (ctypes.c_int64 * 4)(*q_strides), S,
+                                              P(lens), P(new), group, P(shared), max_shared, H, scale, cap, P(slopes), P(o), P(o16), ost))
+
+    def sample(self, x, rows, V, u, ids, f16=False, x_stride=None, temp=None, top_k=None, top_p=None, min_p=None, prob=None):
+        """A token drawn from each of rows of V logits (temperature, top-k, top-p, min-p of each row) with the random numbers
+        u [rows] in [0, 1): ids (int32), prob its probability among the kept ones. x_stride 0: one row for all draws."""
+        op = _SampleOpts(_addr(temp), _addr(top_k), _addr(top_p), _addr(min_p))
+        self._check(lib().mgh_sample(self.h, self._ptr(x), int(f16), V if x_stride is None else x_stride, rows, V,
+                                     ctypes.byref(op), self._ptr(u), self._ptr(ids), self._ptr(prob)))
 
     # ---- graphs ----
     def graph_begin(self):

@@ -8,7 +8,11 @@
 // codes once its 32 tokens are there, from their fp16 values, which a ring of 64 tokens per sequence and
 // head keeps until then; so the cache does not depend on how tokens were grouped into calls, no code
 // is ever rescaled, and a sequence may be shortened by up to 32 tokens.
+#include <algorithm>
+#include <type_traits>
+
 #include "k_kv8.h"
+#include "k_rope.h"
 
 namespace mgh {
 
@@ -52,8 +56,10 @@ __device__ __forceinline__ void load_row(const void* p, int64_t e, int64_t st, _
 // first one's earlier tokens are still in the ring, where the third block's slots are theirs: then the first
 // workgroup stores all, after its reads. Four prompts of 2050 tokens, 8 heads of 128, 50 MB: 15.2 us, 5 us more
 // where the first workgroup stores all.
-template <bool IN16, bool VEC>
-__global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
+// ROT: keys are rotated on the way (k_rope.h), before they are rounded to fp16: the 16 features are 8 pairs, in
+// granules of ROT pairs, whose features lie in two runs; 0: as they come, 16 in a row.
+template <bool IN16, bool VEC, int ROT>
+__device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotation* r) {
     __shared__ uint32_t mx[2][4];
     const Kv8& c = a.c;
     const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, D = c.D;
@@ -98,14 +104,73 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
                 if (t + i >= from && t + i < total) one(i);
         }
     };
+    // 16 features of K that a thread takes, those of unit u of a token: runs of N
+    constexpr int N = ROT ? ROT : 16, NU = 16 / N;
+    auto runs = [&](int u, auto f) {                                     // f(index of 16, feature) per run
+        if constexpr (ROT == 0) {
+            f(std::integral_constant<int, 0>{}, 16 * u);
+        } else {
+#pragma unroll
+            for (int g = 0; g < NU / 2; g++) {
+                const Where w = pairs_at(*r, 8 * u + ROT * g, ROT);
+                f(2 * ROT * g, w.fa);
+                f(2 * ROT * g + ROT, w.fb);
+            }
+        }
+    };
+    auto load_new_k = [&](int t, int u, _Float16* x) {
+        if constexpr (ROT == 0) {
+            load_row<16, IN16, VEC>(a.k, at(t, 16 * u), a.st[0], x);
+        } else {
+            const TokenPos p = token_pos(*r, b, t - len, t);
+            float v[16];
+            runs(u, [&](int i, int d) { load_features<ROT, IN16, VEC>(a.k, at(t, d), a.st[0], v + i); });
+#pragma unroll
+            for (int g = 0; g < NU / 2; g++) {
+                const int pair = 8 * u + ROT * g;
+                if (pair < r->P) {
+                    SinCos sc[ROT];
+                    angles<ROT>(*r, p, pair, sc);
+                    rotate<ROT>(*r, sc, v + 2 * ROT * g);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = (_Float16)v[i];
+        }
+    };
+    auto load_ring_k = [&](int t, int u, _Float16* x) {
+        if constexpr (ROT == 0) {
+            load_row<16, true, true>(ring_k, (t % kKvRing) * D + 16 * u, 1, x);
+        } else {
+            float v[16];
+            runs(u, [&](int i, int d) { load_features<ROT, true, true>(ring_k, (t % kKvRing) * D + d, 1, v + i); });
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = (_Float16)v[i];
+        }
+    };
+    auto put_ring_k = [&](int t, int u, const _Float16* x) {
+        _Float16* to = ring_k + (t % kKvRing) * D;
+        if constexpr (ROT == 0) {
+            *(f16x8*)(to + 16 * u) = halves(x);
+            *(f16x8*)(to + 16 * u + 8) = halves(x + 8);
+        } else {
+            typedef _Float16 hn __attribute__((ext_vector_type(N)));
+            runs(u, [&](int i, int d) {
+                hn v;
+#pragma unroll
+                for (int j = 0; j < N; j++) v[j] = x[i + j];
+                *(hn*)(to + d) = v;
+            });
+        }
+    };
 
     const bool has = tid < 2 * D;                                        // 32 D / 16 units of K, as many of V
-    const int kt = t0 + tid / (D / 16), kd = 16 * (tid % (D / 16));
+    const int kt = t0 + tid / (D / 16), ku = tid % (D / 16);
     const int vt = t0 + 8 * (tid & 3), vd = 2 * (tid >> 2);
     _Float16 xk[16], xv[16];
     if (has && (whole || (each && kt >= r0 && kt < total))) {
-        if (kt < len) load_row<16, true, true>(ring_k, (kt % kKvRing) * D + kd, 1, xk);
-        else load_row<16, IN16, VEC>(a.k, at(kt, kd), a.st[0], xk);
+        if (kt < len) load_ring_k(kt, ku, xk);
+        else load_new_k(kt, ku, xk);
     }
     if (has && (whole || each)) {
         if (whole && vt < len) {                                         // 8 tokens of a feature side by side
@@ -115,10 +180,7 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
         load_v8(vt, vd, len, xv);
     }
     if (has && each) {
-        if (kt >= r0 && kt < total) {
-            *(f16x8*)(ring_k + (kt % kKvRing) * D + kd) = halves(xk);
-            *(f16x8*)(ring_k + (kt % kKvRing) * D + kd + 8) = halves(xk + 8);
-        }
+        if (kt >= r0 && kt < total) put_ring_k(kt, ku, xk);
         ring_v8(vt, vd, xv);
     }
     if (whole) {
@@ -154,18 +216,40 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
             if (id > 0.f)
 #pragma unroll
                 for (int i = 0; i < 16; i++) q[i >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(code_of(x[i], d, id), i & 3, q[i >> 2]);
-            const int64_t to = (page * c.Hkv + hk) * kKvBlock * D + (int64_t)16 * tid;
-            *(u32x4*)((w ? c.v : c.k) + to) = q;
+            const int64_t block = (page * c.Hkv + hk) * kKvBlock * D;
+            if (ROT == 0 || w) {
+                *(u32x4*)((w ? c.v : c.k) + block + (int64_t)16 * tid) = q;
+            } else {
+                uint8_t* to = c.k + block + (kt - t0) * D;
+                runs(ku, [&](int i, int f) {
+                    if constexpr (N == 8) {
+                        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                        *(u32x2*)(to + f) = u32x2{q[i / 4], q[i / 4 + 1]};
+                    } else if constexpr (N == 4) {
+                        *(uint32_t*)(to + f) = q[i / 4];
+                    } else {
+                        to[f] = (uint8_t)(q[i / 4] >> (8 * (i % 4)));
+                    }
+                });
+            }
             if (tid == 0) c.scales[(page * c.Hkv + hk) * 2 + w] = d;
         }
     }
     if (each || blockIdx.x) return;
     __syncthreads();                     // what the ring held has been read
-    for (int i = tid; i < (total - r0) * (D / 8); i += 256) {
-        const int t = r0 + i / (D / 8), d = 8 * (i % (D / 8));
-        _Float16 x[8];
-        load_row<8, IN16, VEC>(a.k, at(t, d), a.st[0], x);
-        *(f16x8*)(ring_k + (t % kKvRing) * D + d) = halves(x);
+    if constexpr (ROT == 0) {
+        for (int i = tid; i < (total - r0) * (D / 8); i += 256) {
+            const int t = r0 + i / (D / 8), d = 8 * (i % (D / 8));
+            _Float16 x[8];
+            load_row<8, IN16, VEC>(a.k, at(t, d), a.st[0], x);
+            *(f16x8*)(ring_k + (t % kKvRing) * D + d) = halves(x);
+        }
+    } else {
+        for (int i = tid; i < (total - r0) * (D / 16); i += 256) {
+            _Float16 x[16];
+            load_new_k(r0 + i / (D / 16), i % (D / 16), x);
+            put_ring_k(r0 + i / (D / 16), i % (D / 16), x);
+        }
     }
     const int g0 = r0 >> 3, groups = ((total + 7) >> 3) - g0;
     for (int i = tid; i < groups * (D / 2); i += 256) {
@@ -174,6 +258,32 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
         load_v8(t, d, r0, x);
         ring_v8(t, d, x);
     }
+}
+
+template <bool IN16, bool VEC>
+__global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
+    append_block<IN16, VEC, 0>(a, nullptr);
+}
+
+// The same with the keys rotated, and workgroups past the first `blocks` of a head and sequence rotating its query heads:
+// V pairs of one head of one token per thread.
+template <bool IN16, bool VEC, int ROT, int V>
+__global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int blocks) {
+    if ((int)blockIdx.x < blocks) {
+        append_block<IN16, VEC, ROT>(a.a, &a.r);
+        return;
+    }
+    const Kv8& c = a.a.c;
+    const int hk = blockIdx.y, b = blockIdx.z, G = a.H / c.Hkv, units = c.D / (2 * V), per = units * G;
+    int len, total;
+    if (!spans(c, a.a.lens, a.a.fresh, a.a.S, b, len, total)) return;
+    const int64_t at = (int64_t)(blockIdx.x - blocks) * 256, i0 = at / per;
+    const int x = (int)(at - i0 * per) + threadIdx.x, di = x / per, item = x - di * per;
+    const int64_t i = i0 + di;
+    if (i >= total - len) return;
+    const int g = item / units, pair = (item - g * units) * V, h = hk * G + g;
+    rope_heads<V, IN16, true, (V > 1)>(a.r, token_pos(a.r, b, i, len + i), pair, a.q, b * a.qst[3] + i * a.qst[1] + h * a.qst[2], 0,
+                                       a.qst[0], a.qo, b * a.qost[3] + i * a.qost[1] + h * a.qost[2], 0, a.qost[0], 1);
 }
 
 // Values of tokens [first, first + n) that a sequence has: codes times their scale, or the ring's fp16. One
@@ -274,6 +384,39 @@ hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t s) {
     else if (a.in16) hipLaunchKernelGGL((k_kv8_append<true, false>), grid, dim3(256), 0, s, a);
     else if (a.vec) hipLaunchKernelGGL((k_kv8_append<false, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_kv8_append<false, false>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+namespace {
+
+template <bool IN16, int ROT>
+void launch_append_rope(const Kv8RopeArgs& a, bool vec_q, dim3 grid, int blocks, hipStream_t s) {
+    auto go = [&](auto vec) {
+        constexpr bool VEC = decltype(vec)::value;
+        if (vec_q) hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, ROT>), grid, dim3(256), 0, s, a, blocks);
+        else hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, 1>), grid, dim3(256), 0, s, a, blocks);
+    };
+    if (a.a.vec) go(std::true_type{});
+    else go(std::false_type{});
+}
+
+}  // namespace
+
+hipError_t launch_kv8_append_rope(const Kv8RopeArgs& a, hipStream_t s) {
+    const int blocks = (int)(((int64_t)a.a.S + 2 * kKvBlock - 2) / kKvBlock), D = a.a.c.D, rot = rope_granule(a.r, D);
+    const bool vec_q = a.vec_q >= rot;
+    const int v = vec_q ? rot : 1;
+    const int64_t per = (int64_t)(a.H / a.a.c.Hkv) * (D / (2 * v));
+    const int64_t wgs = a.q ? ((int64_t)a.a.S * per + 255) / 256 : 0;
+    const dim3 grid((unsigned)(blocks + wgs), (unsigned)a.a.c.Hkv, (unsigned)a.a.c.B);
+    auto go = [&](auto in16) {
+        constexpr bool IN16 = decltype(in16)::value;
+        if (rot == 8) launch_append_rope<IN16, 8>(a, vec_q, grid, blocks, s);
+        else if (rot == 4) launch_append_rope<IN16, 4>(a, vec_q, grid, blocks, s);
+        else launch_append_rope<IN16, 1>(a, vec_q, grid, blocks, s);
+    };
+    if (a.a.in16) go(std::true_type{});
+    else go(std::false_type{});
     return hipGetLastError();
 }
 

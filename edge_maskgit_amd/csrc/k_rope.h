@@ -1,0 +1,162 @@
+// k_rope.h — the rotation of pairs of features by their token's positions (include/mgh.h has the orders).
+//
+// (a, b) -> (a cos t - b sin t, a sin t + b cos t), t = f p. Angles are kept in turns of 2^-64: the frequency as a whole
+// number F = 2^64 f / 2 pi (mod 2^64), so that p F mod 2^64 is the angle with its whole turns gone and no rounding,
+// however far the position; its highest 32 bits are used (off by less than 2^-32 turns and what F's rounding gives,
+// |p| 2^-64 each). The remainder within an eighth of a turn of the nearest quarter goes through odd and even polynomials
+// (least largest error, 2^-28 of the sine and 2^-33), fp32 throughout.
+#pragma once
+#include "mgh_common.h"
+#include "mgh_kernels.h"
+
+namespace mgh {
+
+struct SinCos {
+    float s, c;
+};
+__device__ __forceinline__ SinCos sincos_turns(uint32_t t) {
+    const uint32_t q = (t + 0x20000000u) >> 30;
+    const float x = (float)(int32_t)(t - (q << 30)) * 1.4629180792671596e-9f;        // 2 pi 2^-32
+    const float z = x * x;
+    const float s = fmaf(x * z, fmaf(z, fmaf(z, -0.00019517235f, 0.008332178f), -0.16666655f), x);
+    const float c = fmaf(z * z, fmaf(z, fmaf(z, 2.443838e-05f, -0.0013887367f), 0.041666646f), fmaf(z, -0.5f, 1.f));
+    const uint32_t a = __builtin_bit_cast(uint32_t, q & 1 ? c : s), b = __builtin_bit_cast(uint32_t, q & 1 ? s : c);
+    return {__builtin_bit_cast(float, a ^ ((q & 2) << 30)), __builtin_bit_cast(float, b ^ (((q + 1) & 2) << 30))};
+}
+
+// the highest 32 bits of p F mod 2^64
+__device__ __forceinline__ uint32_t turns_at(int32_t p, uint64_t F) { return (uint32_t)(((uint64_t)(int64_t)p * F) >> 32); }
+
+// a token's positions along the axes; `i` its index in the call, `run` its position where none are given
+struct TokenPos {
+    int32_t p[4];
+    __device__ __forceinline__ int32_t of(const Rotation& r, int pair) const {
+        int32_t x = p[0];
+#pragma unroll
+        for (int a = 1; a < 4; a++) x = pair >= r.start[a] ? p[a] : x;
+        return x;
+    }
+};
+__device__ __forceinline__ TokenPos token_pos(const Rotation& r, int64_t b, int64_t i, int64_t run) {
+    TokenPos t;
+#pragma unroll
+    for (int a = 0; a < 4; a++) {
+        if (!r.pos) t.p[a] = (int32_t)run;
+        else if (a < r.axes) t.p[a] = r.pos[i * r.pst[0] + b * r.pst[1] + a * r.pst[2]];
+        else t.p[a] = 0;
+    }
+    return t;
+}
+
+// Where the features of V pairs in a row lie: V from fa on and V from fb on. Pairs past the rotated ones are the rest of the
+// features, two and two in order.
+struct Where {
+    int fa, fb;
+};
+__device__ __forceinline__ Where pairs_at(const Rotation& r, int pair, int V) {
+    if (pair >= r.P || r.order == kRopePairs) return {2 * pair, 2 * pair + V};
+    if (r.order == kRopeHalves) return {pair, r.P + pair};
+    int s = 0, n = r.start[1];
+#pragma unroll
+    for (int a = 1; a < 4; a++)
+        if (pair >= r.start[a]) s = r.start[a], n = r.start[a + 1] - r.start[a];
+    return {s + pair, s + pair + n};
+}
+
+// cos and sin of V pairs
+template <int V>
+__device__ __forceinline__ void angles(const Rotation& r, const TokenPos& t, int pair, SinCos* sc) {
+#pragma unroll
+    for (int i = 0; i < V; i++) sc[i] = sincos_turns(turns_at(t.of(r, pair + i), r.turn[pair + i]));
+}
+
+// x: V features from fa on, V from fb on
+template <int V>
+__device__ __forceinline__ void rotate(const Rotation& r, const SinCos* sc, float* x) {
+    // (kept in registers as fp32: an fma that rounds to fp16 by itself would skip a rounding, in some kernels and not in others)
+    auto turn = [](float& a, float& b, const SinCos& w) {
+        float u = fmaf(a, w.c, -(b * w.s)), v = fmaf(a, w.s, b * w.c);
+        asm("" : "+v"(u), "+v"(v));
+        a = u, b = v;
+    };
+    if (r.order == kRopePairs) {
+#pragma unroll
+        for (int i = 0; i < V; i++) turn(x[2 * i], x[2 * i + 1], sc[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) turn(x[i], x[V + i], sc[i]);
+    }
+}
+
+// V features from e on: one access of up to 16 bytes where VEC, else one by one, `st` apart
+template <int V, bool H16, bool VEC>
+__device__ __forceinline__ void load_features(const void* p, int64_t e, int64_t st, float* x) {
+    if constexpr (VEC && V > 1) {
+        constexpr int N = H16 || V < 4 ? V : 4;
+        if constexpr (H16) {
+            typedef _Float16 hn __attribute__((ext_vector_type(N)));
+            const hn v = *(const hn*)((const _Float16*)p + e);
+#pragma unroll
+            for (int j = 0; j < N; j++) x[j] = (float)v[j];
+        } else {
+            typedef float fn __attribute__((ext_vector_type(N)));
+#pragma unroll
+            for (int i = 0; i < V; i += N) {
+                const fn v = *(const fn*)((const float*)p + e + i);
+#pragma unroll
+                for (int j = 0; j < N; j++) x[i + j] = v[j];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = H16 ? (float)((const _Float16*)p)[e + i * st] : ((const float*)p)[e + i * st];
+    }
+}
+template <int V, bool H16, bool VEC>
+__device__ __forceinline__ void store_features(void* p, int64_t e, int64_t st, const float* x) {
+    if constexpr (VEC && V > 1) {
+        constexpr int N = H16 || V < 4 ? V : 4;
+        if constexpr (H16) {
+            typedef _Float16 hn __attribute__((ext_vector_type(N)));
+            hn v;
+#pragma unroll
+            for (int j = 0; j < N; j++) v[j] = (_Float16)x[j];
+            *(hn*)((_Float16*)p + e) = v;
+        } else {
+            typedef float fn __attribute__((ext_vector_type(N)));
+#pragma unroll
+            for (int i = 0; i < V; i += N) {
+                fn v;
+#pragma unroll
+                for (int j = 0; j < N; j++) v[j] = x[i + j];
+                *(fn*)((float*)p + e + i) = v;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            if (H16) ((_Float16*)p)[e + i * st] = (_Float16)x[i];
+            else ((float*)p)[e + i * st] = x[i];
+        }
+    }
+}
+
+// V pairs of `n` heads `step` apart, of one token: the angles once, then head by head. x and y: the token's first of these heads
+template <int V, bool IN16, bool OUT16, bool VEC>
+__device__ __forceinline__ void rope_heads(const Rotation& r, const TokenPos& t, int pair, const void* x, int64_t ex, int64_t hx,
+                                           int64_t dx, void* y, int64_t ey, int64_t hy, int64_t dy, int n) {
+    const Where w = pairs_at(r, pair, V);
+    const bool turned = pair < r.P;
+    SinCos sc[V];
+    if (turned) angles<V>(r, t, pair, sc);
+    for (int h = 0; h < n; h++) {
+        float v[2 * V];
+        load_features<V, IN16, VEC>(x, ex + h * hx + w.fa * dx, dx, v);
+        load_features<V, IN16, VEC>(x, ex + h * hx + w.fb * dx, dx, v + V);
+        if (turned) rotate<V>(r, sc, v);
+        store_features<V, OUT16, VEC>(y, ey + h * hy + w.fa * dy, dy, v);
+        store_features<V, OUT16, VEC>(y, ey + h * hy + w.fb * dy, dy, v + V);
+    }
+}
+
+}  // namespace mgh

@@ -1,0 +1,73 @@
+// k_rope.hip — rotary positions on the heads of queries and keys (gfx950).
+//
+// Bound by its bytes: every feature is read and written once. A thread takes V pairs (two accesses of up to 16 bytes in,
+// two out) of some heads of one token, so their angles are computed once for those heads.
+#include <algorithm>
+
+#include "k_rope.h"
+
+namespace mgh {
+
+namespace {
+
+// items of a sequence: token, head of a step, V pairs; a thread takes heads hl, hl + HG, ...
+template <int V, bool IN16, bool OUT16>
+__global__ __launch_bounds__(256) void k_rope(RopeArgs a, int HG) {
+    const Rotation& r = a.r;
+    const int units = a.D / (2 * V), per = units * HG, b = blockIdx.y;
+    const int64_t at = (int64_t)blockIdx.x * 256, i0 = at / per;
+    const int x = (int)(at - i0 * per) + threadIdx.x, di = x / per, item = x - di * per;
+    const int64_t i = i0 + di;
+    const int n = a.fresh ? a.fresh[b] : a.S;
+    if (i >= n || n > a.S) return;
+    const int hl = item / units, pair = (item - hl * units) * V;
+    const int64_t run = (a.first ? a.first[b] : 0) + i;
+    rope_heads<V, IN16, OUT16, (V > 1)>(r, token_pos(r, b, i, run), pair, a.x, b * a.xst[3] + i * a.xst[1] + hl * a.xst[2], HG * a.xst[2],
+                                    a.xst[0], a.y, b * a.yst[3] + i * a.yst[1] + hl * a.yst[2], HG * a.yst[2], a.yst[0],
+                                    (a.H - hl + HG - 1) / HG);
+}
+
+template <int V>
+void launch_rope_v(const RopeArgs& a, const RopePlan& p, hipStream_t s) {
+    const dim3 grid((unsigned)p.wgs, (unsigned)a.B);
+    if (a.in16 && a.out16) hipLaunchKernelGGL((k_rope<V, true, true>), grid, dim3(256), 0, s, a, p.hg);
+    else if (a.in16) hipLaunchKernelGGL((k_rope<V, true, false>), grid, dim3(256), 0, s, a, p.hg);
+    else if (a.out16) hipLaunchKernelGGL((k_rope<V, false, true>), grid, dim3(256), 0, s, a, p.hg);
+    else hipLaunchKernelGGL((k_rope<V, false, false>), grid, dim3(256), 0, s, a, p.hg);
+}
+
+}  // namespace
+
+// pairs in a row whose features lie in two runs: 8, 4 or 1
+int rope_granule(const Rotation& r, int D) {
+    auto fits = [&](int n) {
+        if (r.P % n || D % (2 * n)) return false;
+        for (int i = 0; i < r.axes && r.order == kRopeAxisHalves; i++)
+            if ((r.start[i + 1] - r.start[i]) % n) return false;
+        return true;
+    };
+    return fits(8) ? 8 : fits(4) ? 4 : 1;
+}
+
+RopePlan rope_plan(const RopeArgs& a) {
+    RopePlan p{};
+    const int g = rope_granule(a.r, a.D);
+    p.v = std::min(std::min(g, a.vec), a.in16 && a.out16 ? 8 : 4);
+    const int64_t units = a.D / (2 * p.v), all = (int64_t)a.B * a.S * units;
+    // heads of a thread: more where threads enough for 8 waves per SIMD are left
+    int n = 1;
+    while (n < 8 && n < a.H && all * a.H / (2 * n) >= 256 * 2048) n *= 2;
+    p.hg = (a.H + n - 1) / n;
+    p.wgs = (a.S * units * p.hg + 255) / 256;
+    return p;
+}
+
+hipError_t launch_rope(const RopeArgs& a, const RopePlan& p, hipStream_t s) {
+    // (8 pairs with fp16 on both sides only)
+    if (p.v == 8) hipLaunchKernelGGL((k_rope<8, true, true>), dim3((unsigned)p.wgs, (unsigned)a.B), dim3(256), 0, s, a, p.hg);
+    else if (p.v == 4) launch_rope_v<4>(a, p, s);
+    else launch_rope_v<1>(a, p, s);
+    return hipGetLastError();
+}
+
+}  // namespace mgh

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -1276,12 +1277,81 @@ int check_kv8(mgh_ctx* c, const char* fn, const mgh_kv8* kv, mgh::Kv8* out) {
     return MGH_OK;
 }
 
+// elements, 8, 4 or 1, at multiples of which the rows start with their features in order, in accesses of up to 16 bytes
+int row_granule(const void* p, const int64_t st[4], bool f16) {
+    for (int n = 8; n > 1; n /= 2)
+        if (rows_aligned(p, st, n, f16 ? 2 * n : 16)) return n;
+    return 1;
+}
+
+int check_rotation(mgh_ctx* c, const char* fn, const mgh_rotation* rot, int D, mgh::Rotation* out) {
+    const std::string f(fn);
+    if (!rot) return fail(c, MGH_ERR_ARG, f + ": null rotation");
+    if (rot->axes < 1 || rot->axes > 4) return fail(c, MGH_ERR_ARG, f + ": a rotation has 1 to 4 axes");
+    if (rot->order != MGH_ROPE_HALVES && rot->order != MGH_ROPE_PAIRS && rot->order != MGH_ROPE_AXIS_HALVES)
+        return fail(c, MGH_ERR_ARG, f + ": unknown order of pairs");
+    if (D <= 0 || D % 2 || D > 2 * mgh::kMostPairs) return fail(c, MGH_ERR_UNSUPPORTED, f + ": D must be even and up to 128");
+    mgh::Rotation r{};
+    r.axes = rot->axes; r.order = rot->order;
+    for (int a = 0; a < 4; a++) {
+        if (a < rot->axes) {
+            if (rot->pairs[a] < 0 || rot->pairs[a] > D / 2) return fail(c, MGH_ERR_ARG, f + ": pairs must be between 0 and D / 2");
+            r.P += rot->pairs[a];
+        }
+        r.start[a + 1] = r.P;
+    }
+    if (r.P > D / 2) return fail(c, MGH_ERR_ARG, f + ": more pairs than D / 2");
+    if (r.P && !rot->h_freqs) return fail(c, MGH_ERR_ARG, f + ": null frequencies");
+    if (!aligned_to(rot->h_freqs, sizeof(double)) || !aligned_to(rot->d_pos, 4))
+        return fail(c, MGH_ERR_ARG, f + ": frequencies must be 8-byte and positions 4-byte aligned");
+    for (int i = 0; i < r.P; i++) {
+        const double w = rot->h_freqs[i];
+        if (!(std::fabs(w) <= 16.)) return fail(c, MGH_ERR_ARG, f + ": frequencies must be finite and at most 16");
+        // whole numbers of 2^-64 turns, whole turns left out (64-bit significands: off by less than one)
+        long double t = (long double)w * 0.159154943091895335768883763372514362L;
+        t = ldexpl(t - floorl(t), 64);
+        t = nearbyintl(t);
+        r.turn[i] = t >= 18446744073709551616.0L ? 0 : (uint64_t)t;
+    }
+    r.pos = rot->d_pos;
+    for (int i = 0; i < 3; i++) r.pst[i] = rot->pos_strides[i];
+    *out = r;
+    return MGH_OK;
+}
+
 int check_step(mgh_ctx* c, const char* fn, int S, const int32_t* lens, const int32_t* fresh) {
     const std::string f(fn);
     if (S < 0) return fail(c, MGH_ERR_ARG, f + ": negative number of tokens");
     if (S > (1 << 28)) return fail(c, MGH_ERR_UNSUPPORTED, f + ": at most 2^28 tokens");
     if (!lens) return fail(c, MGH_ERR_ARG, f + ": null lengths");
     if (!aligned_to(lens, 4) || !aligned_to(fresh, 4)) return fail(c, MGH_ERR_ARG, f + ": lengths must be 4-byte aligned");
+    return MGH_OK;
+}
+
+// the arguments of both attentions over the cache; *empty: nothing to do
+int check_kv8_attn(mgh_ctx* c, const char* fn, const mgh_kv8* kv, const void* q, int in_f16, const int64_t qst[4], int S,
+                   const int32_t* lens, const int32_t* fresh, int H, float scale, float cap, const float* slopes, float* o, void* o16,
+                   const int64_t ost[4], mgh::Kv8AttnArgs* out, bool* empty) {
+    const std::string f(fn);
+    mgh::Kv8AttnArgs& a = *out;
+    if (int r = check_kv8(c, fn, kv, &a.c)) return r;
+    if (int r = check_scores(c, fn, kv->D, H, kv->Hkv, scale, cap, o, o16)) return r;
+    *empty = kv->B == 0 || S == 0;
+    if (*empty) return MGH_OK;
+    if (int r = check_step(c, fn, S, lens, fresh)) return r;
+    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, f + ": in_f16 must be 0 or 1");
+    if (!q || !qst) return fail(c, MGH_ERR_ARG, f + ": null pointer");
+    if (!aligned_to(q, in_f16 ? 2 : 4) || !aligned_to(o, 4) || !aligned_to(o16, 2) || !aligned_to(slopes, 4))
+        return fail(c, MGH_ERR_ARG, f + ": pointers must be aligned to their elements");
+    if (H > 65535 || (int64_t)S * (H / kv->Hkv) > (1 << 24))
+        return fail(c, MGH_ERR_UNSUPPORTED, f + ": at most 65535 heads and 2^24 rows of a key head");
+    a.q = q; a.o = o; a.o16 = (_Float16*)o16; a.S = S; a.H = H; a.in16 = in_f16 != 0;
+    a.lens = lens; a.fresh = fresh; a.slopes = slopes;
+    a.mod = mgh::score_mod(scale, cap, o16 != nullptr);
+    const int64_t packed[4] = {1, kv->D, (int64_t)kv->D * S, (int64_t)kv->D * S * H};
+    for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.ost[i] = ost ? ost[i] : packed[i];
+    a.vec_q = in_f16 && rows_aligned(q, qst, 8, 16);
+    a.vec_o = o16 ? rows_aligned(o16, a.ost, 4, 8) : rows_aligned(o, a.ost, 4, 16);
     return MGH_OK;
 }
 
@@ -1391,6 +1461,67 @@ int mgh_kv8_append(mgh_ctx* c, const mgh_kv8* kv, const void* k, const void* v, 
     return MGH_OK;
 }
 
+int mgh_rope(mgh_ctx* c, const mgh_rotation* rot, const void* x, int in_f16, const int64_t xst[4], int D, int S, int H, int B,
+             const int32_t* first, const int32_t* fresh, float* y, void* y16, const int64_t yst[4]) {
+    if (!c) return MGH_ERR_ARG;
+    mgh::RopeArgs a{};
+    if (int r = check_rotation(c, "rope", rot, D, &a.r)) return r;
+    if (S < 0 || H < 0 || B < 0) return fail(c, MGH_ERR_ARG, "rope: negative shape");
+    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "rope: in_f16 must be 0 or 1");
+    if ((y != nullptr) == (y16 != nullptr)) return fail(c, MGH_ERR_ARG, "rope: exactly one of d_y and d_y16 is needed");
+    if (S == 0 || H == 0 || B == 0) return MGH_OK;
+    if (S > (1 << 28) || H > 65535 || B > 65535 || (int64_t)S * H * D > ((int64_t)1 << 33))
+        return fail(c, MGH_ERR_UNSUPPORTED, "rope: at most 2^28 tokens, 65535 heads and sequences, 2^33 values of a sequence");
+    if (!x || !xst || !yst) return fail(c, MGH_ERR_ARG, "rope: null pointer");
+    if (!aligned_to(x, in_f16 ? 2 : 4) || !aligned_to(y, 4) || !aligned_to(y16, 2) || !aligned_to(first, 4) || !aligned_to(fresh, 4))
+        return fail(c, MGH_ERR_ARG, "rope: pointers must be aligned to their elements");
+    a.x = x; a.in16 = in_f16 != 0; a.out16 = y16 != nullptr;
+    a.y = y16 ? y16 : (void*)y;
+    bool same = true;
+    for (int i = 0; i < 4; i++) a.xst[i] = xst[i], a.yst[i] = yst[i], same = same && xst[i] == yst[i];
+    if (a.y == x && (!same || a.in16 != a.out16)) return fail(c, MGH_ERR_ARG, "rope: in place needs the same type and strides");
+    a.D = D; a.S = S; a.H = H; a.B = B;
+    a.first = first; a.fresh = fresh;
+    a.vec = std::min(row_granule(x, xst, a.in16), row_granule(a.y, yst, a.out16));
+    const mgh::RopePlan plan = mgh::rope_plan(a);
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_rope(a, plan, c->stream), "k_rope");
+    return MGH_OK;
+}
+
+int mgh_kv8_append_rope(mgh_ctx* c, const mgh_kv8* kv, const mgh_rotation* rot, const void* k, const void* v, int in_f16,
+                        const int64_t st[4], int S, const int32_t* lens, const int32_t* fresh, const void* q, const int64_t qst[4],
+                        int H, void* q_out, const int64_t qost[4]) {
+    if (!c) return MGH_ERR_ARG;
+    mgh::Kv8RopeArgs a{};
+    if (int r = check_kv8(c, "kv8_append_rope", kv, &a.a.c)) return r;
+    if (int r = check_rotation(c, "kv8_append_rope", rot, kv->D, &a.r)) return r;
+    if (kv->B == 0 || S == 0) return MGH_OK;
+    if (int r = check_step(c, "kv8_append_rope", S, lens, fresh)) return r;
+    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "kv8_append_rope: in_f16 must be 0 or 1");
+    if (!k || !v || !st) return fail(c, MGH_ERR_ARG, "kv8_append_rope: null pointer");
+    const size_t eb = in_f16 ? 2 : 4;
+    if (!aligned_to(k, eb) || !aligned_to(v, eb) || !aligned_to(q, eb) || !aligned_to(q_out, 2))
+        return fail(c, MGH_ERR_ARG, "kv8_append_rope: pointers must be aligned to their elements");
+    a.a.k = k; a.a.v = v; a.a.S = S; a.a.lens = lens; a.a.fresh = fresh; a.a.in16 = in_f16 != 0;
+    for (int i = 0; i < 4; i++) a.a.st[i] = st[i];
+    a.a.vec = rows_aligned(k, st, in_f16 ? 8 : 4, 16) && rows_aligned(v, st, in_f16 ? 8 : 4, 16);
+    if (q) {
+        if (H <= 0 || H % kv->Hkv) return fail(c, MGH_ERR_ARG, "kv8_append_rope: need H > 0 and H % Hkv == 0");
+        if (!q_out || !qst || !qost) return fail(c, MGH_ERR_ARG, "kv8_append_rope: null pointer");
+        if (H > 65535 || (int64_t)S * (H / kv->Hkv) * kv->D > ((int64_t)1 << 32))
+            return fail(c, MGH_ERR_UNSUPPORTED, "kv8_append_rope: at most 65535 heads and 2^32 values of a key head's queries");
+        bool same = in_f16 != 0;
+        for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.qost[i] = qost[i], same = same && qst[i] == qost[i];
+        if (q == q_out && !same) return fail(c, MGH_ERR_ARG, "kv8_append_rope: in place needs the same type and strides");
+        a.q = q; a.qo = (_Float16*)q_out; a.H = H;
+        a.vec_q = std::min(row_granule(q, qst, a.a.in16), row_granule(q_out, qost, true));
+    }
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_kv8_append_rope(a, c->stream), "k_kv8_append_rope");
+    return MGH_OK;
+}
+
 int mgh_kv8_advance(mgh_ctx* c, int32_t* lens, const int32_t* fresh, int B, int S) {
     if (!c) return MGH_ERR_ARG;
     if (B < 0) return fail(c, MGH_ERR_ARG, "kv8_advance: negative number of sequences");
@@ -1406,23 +1537,9 @@ int mgh_kv8_attn(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const
                  void* o16, const int64_t ost[4]) {
     if (!c) return MGH_ERR_ARG;
     mgh::Kv8AttnArgs a{};
-    if (int r = check_kv8(c, "kv8_attn", kv, &a.c)) return r;
-    if (int r = check_scores(c, "kv8_attn", kv->D, H, kv->Hkv, scale, cap, o, o16)) return r;
-    if (kv->B == 0 || S == 0) return MGH_OK;
-    if (int r = check_step(c, "kv8_attn", S, lens, fresh)) return r;
-    if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "kv8_attn: in_f16 must be 0 or 1");
-    if (!q || !qst) return fail(c, MGH_ERR_ARG, "kv8_attn: null pointer");
-    if (!aligned_to(q, in_f16 ? 2 : 4) || !aligned_to(o, 4) || !aligned_to(o16, 2) || !aligned_to(slopes, 4))
-        return fail(c, MGH_ERR_ARG, "kv8_attn: pointers must be aligned to their elements");
-    if (H > 65535 || (int64_t)S * (H / kv->Hkv) > (1 << 24))
-        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn: at most 65535 heads and 2^24 rows of a key head");
-    a.q = q; a.o = o; a.o16 = (_Float16*)o16; a.S = S; a.H = H; a.in16 = in_f16 != 0;
-    a.lens = lens; a.fresh = fresh; a.slopes = slopes;
-    a.mod = mgh::score_mod(scale, cap, o16 != nullptr);
-    const int64_t packed[4] = {1, kv->D, (int64_t)kv->D * S, (int64_t)kv->D * S * H};
-    for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.ost[i] = ost ? ost[i] : packed[i];
-    a.vec_q = in_f16 && rows_aligned(q, qst, 8, 16);
-    a.vec_o = o16 ? rows_aligned(o16, a.ost, 4, 8) : rows_aligned(o, a.ost, 4, 16);
+    bool empty = false;
+    if (int r = check_kv8_attn(c, "kv8_attn", kv, q, in_f16, qst, S, lens, fresh, H, scale, cap, slopes, o, o16, ost, &a, &empty)) return r;
+    if (empty) return MGH_OK;
     const mgh::Kv8Plan plan = mgh::kv8_plan(a);
     if ((int64_t)plan.tiles * plan.splits * kv->Hkv * kv->B >= (1 << 24))
         return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn: shape too large");
@@ -1432,6 +1549,35 @@ int mgh_kv8_attn(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const
         a.ws = (float*)c->qp_ws;
     }
     MGH_HIP(c, mgh::launch_kv8_attn(a, plan, c->stream), "k_kv8_attn");
+    return MGH_OK;
+}
+
+int mgh_kv8_attn_shared(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16, const int64_t qst[4], int S,
+                        const int32_t* lens, const int32_t* fresh, int group, const int32_t* shared, int max_shared, int H,
+                        float scale, float cap, const float* slopes, float* o, void* o16, const int64_t ost[4]) {
+    if (!c) return MGH_ERR_ARG;
+    mgh::Kv8AttnArgs a{};
+    bool empty = false;
+    if (int r = check_kv8_attn(c, "kv8_attn_shared", kv, q, in_f16, qst, S, lens, fresh, H, scale, cap, slopes, o, o16, ost, &a, &empty))
+        return r;
+    if (group < 1) return fail(c, MGH_ERR_ARG, "kv8_attn_shared: a group has at least one sequence");
+    if (max_shared < 0 || max_shared > kv->max_blocks)
+        return fail(c, MGH_ERR_ARG, "kv8_attn_shared: max_shared must be between 0 and max_blocks");
+    if (empty) return MGH_OK;
+    if (!shared) return fail(c, MGH_ERR_ARG, "kv8_attn_shared: null pointer");
+    if (!aligned_to(shared, 4)) return fail(c, MGH_ERR_ARG, "kv8_attn_shared: pointers must be aligned to their elements");
+    a.shared = shared; a.group = std::min(group, kv->B); a.max_shared = max_shared;
+    const int64_t G = H / kv->Hkv, R = (int64_t)kv->B * S * G;
+    if (R > (1 << 24) || R * kv->Hkv >= ((int64_t)1 << 28))
+        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn_shared: at most 2^24 rows of a key head and 2^28 in all");
+    const mgh::Kv8SharedPlan plan = mgh::kv8_shared_plan(a);
+    if ((int64_t)plan.own.tiles * plan.own.splits * kv->Hkv * kv->B >= (1 << 24) ||
+        (int64_t)plan.shared.tiles * plan.shared.splits * kv->Hkv * ((kv->B + a.group - 1) / a.group) >= (1 << 24))
+        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn_shared: shape too large");
+    if (int r = set_dev(c)) return r;
+    if (int r = ensure_qp_ws(c, plan.ws_bytes)) return r;
+    a.ws = (float*)c->qp_ws;
+    MGH_HIP(c, mgh::launch_kv8_attn_shared(a, plan, c->stream), "k_kv8_attn_part");
     return MGH_OK;
 }
 
@@ -1488,6 +1634,31 @@ int mgh_logits_process(mgh_ctx* c, const void* x, int f16, int64_t xs, int rows,
     a.bias = op.d_bias; a.bias_stride = op.bias_stride; a.allowed = op.d_allowed; a.allowed_stride = op.allowed_stride;
     if (int r = set_dev(c)) return r;
     MGH_HIP(c, mgh::launch_logits_process(a, c->stream), "k_logits");
+    return MGH_OK;
+}
+
+int mgh_sample(mgh_ctx* c, const void* x, int f16, int64_t xs, int rows, int V, const mgh_sample_opts* opts, const float* u,
+               int32_t* ids, float* prob) {
+    if (!c) return MGH_ERR_ARG;
+    const mgh_sample_opts none{};
+    const mgh_sample_opts& op = opts ? *opts : none;
+    if (rows < 0 || V < 0) return fail(c, MGH_ERR_ARG, "sample: negative shape");
+    if (f16 != 0 && f16 != 1) return fail(c, MGH_ERR_ARG, "sample: f16 must be 0 or 1");
+    if (rows == 0) return MGH_OK;
+    if (V == 0) return fail(c, MGH_ERR_ARG, "sample: rows without tokens");
+    if (V > (1 << 24) || rows > (1 << 20)) return fail(c, MGH_ERR_UNSUPPORTED, "sample: at most 2^24 tokens and 2^20 rows");
+    if (!x || !u || !ids) return fail(c, MGH_ERR_ARG, "sample: null pointer");
+    if (rows > 1 && xs && xs < V) return fail(c, MGH_ERR_ARG, "sample: x_stride must be 0 or at least V");
+    const void* words[] = {op.d_temp, op.d_top_k, op.d_top_p, op.d_min_p, u, ids, prob};
+    bool ok = aligned_to(x, f16 ? 2 : 4);
+    for (const void* p : words) ok = ok && aligned_to(p, 4);
+    if (!ok) return fail(c, MGH_ERR_ARG, "sample: pointers must be aligned to their elements");
+    mgh::SampleArgs a{};
+    a.x = x; a.x_stride = xs; a.rows = rows; a.V = V; a.f16 = f16 != 0;
+    a.temp = op.d_temp; a.top_k = op.d_top_k; a.top_p = op.d_top_p; a.min_p = op.d_min_p;
+    a.u = u; a.ids = ids; a.prob = prob; a.unit = mgh::sample_unit(V);
+    if (int r = set_dev(c)) return r;
+    MGH_HIP(c, mgh::launch_sample(a, c->stream), "k_sample");
     return MGH_OK;
 }
 

@@ -396,6 +396,9 @@ struct Kv8AttnArgs {
     bool vec_q;            // fp16 rows, 16-byte aligned, features in order
     bool vec_o;            // 4 features of an output row: one aligned store
     float* ws;             // Kv8Plan::ws_bytes
+    // sequences that share their first blocks, `group` in a row
+    const int32_t* shared; // [ceil(B / group)] blocks
+    int group, max_shared;
 };
 struct Kv8Plan {
     int qt, tiles, splits; // 16-row tiles per workgroup, workgroups along a head's rows, parts of a sequence
@@ -404,6 +407,52 @@ struct Kv8Plan {
 };
 Kv8Plan kv8_plan(const Kv8AttnArgs& a);
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s);
+struct Kv8SharedPlan {
+    Kv8Plan own, shared;   // parts of a sequence's own blocks, parts of a group's shared ones
+    size_t ws_bytes;
+};
+Kv8SharedPlan kv8_shared_plan(const Kv8AttnArgs& a);
+hipError_t launch_kv8_attn_shared(const Kv8AttnArgs& a, const Kv8SharedPlan& p, hipStream_t s);
+
+// Rotary positions (k_rope.h): pairs start[a] .. start[a + 1] - 1 turn with axis a
+enum { kRopeHalves = 0, kRopePairs = 1, kRopeAxisHalves = 2 };
+constexpr int kMostPairs = 64;
+struct Rotation {
+    int axes, P, order;
+    int start[5];              // unused axes start at P
+    const int32_t* pos;        // or null: consecutive ones
+    int64_t pst[3];            // token, sequence, axis
+    uint64_t turn[kMostPairs]; // 2^64 turns per unit of position
+};
+int rope_granule(const Rotation& r, int D);
+struct RopeArgs {
+    Rotation r;
+    const void* x;
+    void* y;
+    int64_t xst[4], yst[4];
+    int D, S, H, B;
+    const int32_t* first;      // [B] position of a sequence's token 0, or null: 0
+    const int32_t* fresh;      // [B] tokens, or null: S
+    bool in16, out16;
+    int vec;                   // elements, 8, 4 or 1, at multiples of which rows of x and y start and are aligned
+};
+struct RopePlan {
+    int v, hg;                 // pairs of a thread, heads of a step
+    int64_t wgs;               // workgroups of a sequence
+};
+RopePlan rope_plan(const RopeArgs& a);
+hipError_t launch_rope(const RopeArgs& a, const RopePlan& p, hipStream_t s);
+// the cache's writer with the keys rotated on the way, and queries beside them
+struct Kv8RopeArgs {
+    Kv8AppendArgs a;
+    Rotation r;
+    const void* q;             // as the keys' type, or null
+    _Float16* qo;
+    int64_t qst[4], qost[4];
+    int H;
+    int vec_q;                 // as RopeArgs::vec
+};
+hipError_t launch_kv8_append_rope(const Kv8RopeArgs& a, hipStream_t s);
 
 // Penalties, bias and grammar mask on logits (k_logits.hip)
 struct LogitsArgs {
@@ -426,6 +475,24 @@ struct LogitsArgs {
 };
 constexpr int kLogitsChunk = 2048;      // tokens per workgroup
 hipError_t launch_logits_process(const LogitsArgs& a, hipStream_t s);
+
+// Drawing a token from logits (k_sample.hip)
+struct SampleArgs {
+    const void* x;
+    int64_t x_stride;
+    int rows, V;
+    bool f16;
+    const float* temp;         // [rows], or null: 1
+    const int32_t* top_k;      // ... all
+    const float* top_p;        // ... 1
+    const float* min_p;        // ... 0
+    const float* u;
+    int32_t* ids;
+    float* prob;               // or null
+    double unit;               // masses are counted in 1 / unit of the largest weight
+};
+double sample_unit(int V);
+hipError_t launch_sample(const SampleArgs& a, hipStream_t s);
 
 size_t noalloc_scratch_bytes();
 hipError_t noalloc_scratch(int device, void** out);

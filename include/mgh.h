@@ -418,6 +418,34 @@ int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* 
                     int B, float scale, const mgh_attn_opts* opts /* NULL: none */, float* d_o, void* d_o16,
                     const int64_t o_strides[4]);
 
+/* ---- rotary positions: pairs of a head's features turn with their token's positions. No counterpart in the
+ *      reference, whose positions are a learned table (pos_embd.weight). Pair i of P holds the values (a, b);
+ *      with t = h_freqs[i] p, p the token's position on the axis that the pair belongs to, they become
+ *        (a cos t - b sin t, a sin t + b cos t).
+ *      The pairs' features of D, by `order`: MGH_ROPE_HALVES i and P + i; MGH_ROPE_PAIRS 2 i and 2 i + 1;
+ *      MGH_ROPE_AXIS_HALVES each axis's 2 n features in a row, its pair j being j and n + j of them. Features from 2 P on
+ *      stay as they are. Axis a has the next pairs[a] pairs (index; row and column; time, row and column; ...).
+ *      d_pos: whole positions (any sign) of token i of sequence b on axis a at a pos_strides[2] + b pos_strides[1] +
+ *      i pos_strides[0]; NULL: consecutive ones on every axis, from where the call says. h_freqs is read when the call is
+ *      made, angles per unit of position in radians, finite, up to 16 in magnitude. An angle is exact to 2^-32 turns however
+ *      far the position (up to 2^31), its sine and cosine to 2^-23, products and sums are fp32, rounded once to an fp16 output.
+ *      D even up to 128, P up to D / 2. ---- */
+enum { MGH_ROPE_HALVES = 0, MGH_ROPE_PAIRS = 1, MGH_ROPE_AXIS_HALVES = 2 };
+typedef struct mgh_rotation {
+    int axes;                    /* 1 .. 4 */
+    int pairs[4];
+    int order;
+    const double* h_freqs;       /* [P], host */
+    const int32_t* d_pos;
+    int64_t pos_strides[3];      /* token, sequence, axis */
+} mgh_rotation;
+/* x and y: {D, S, H, B} views with element strides (d, token, head, sequence); y fp32 (d_y) or fp16 (d_y16), exactly one
+ * of them; y may be x where type and strides are the same, else they do not overlap. Sequence b's token 0 stands at
+ * d_first[b] (NULL: 0) where the rotation has no positions. d_new [B]: tokens of each sequence, 0 .. S (NULL: S each);
+ * rows past them, and all rows of a sequence whose number does not fit, are neither read nor written. S D H up to 2^33. */
+int mgh_rope(mgh_ctx* ctx, const mgh_rotation* rot, const void* d_x, int in_f16, const int64_t x_strides[4], int D, int S,
+             int H, int B, const int32_t* d_first, const int32_t* d_new, float* d_y, void* d_y16, const int64_t y_strides[4]);
+
 /* ---- a cache of keys and values in 8 bits, and attention over it, for generating token by token. No
  *      counterpart in the reference, which generates by whole bidirectional forwards. Values are held
  *      as Q8 codes (the reference's rule, mg-opencl.cpp:424-434: d = max|x| / 127 in fp32, codes x / d
@@ -462,6 +490,14 @@ size_t mgh_kv8_tail_bytes(int B, int Hkv, int D);            /* of d_k_tail, and
 /* k, v: {D, S, Hkv, B} views (element strides d, token, head, sequence), fp16 or fp32 (rounded to fp16) */
 int mgh_kv8_append(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_k, const void* d_v, int in_f16,
                    const int64_t strides[4], int S, const int32_t* d_lens, const int32_t* d_new);
+/* mgh_kv8_append with the keys rotated on the way: in fp32, from k as it comes, rounded to fp16 once, into the tails and
+ * codes; the same cache as mgh_rope to fp16 followed by mgh_kv8_append. Where d_q is not NULL the queries ({D, S, H, B}, as
+ * k's type) are rotated to fp16 rows at d_q_out beside it (q itself where types and strides are the same, else apart from
+ * it), as mgh_rope. A rotation without positions takes those in the cache, lens[b] + i. Rows past a sequence's new tokens
+ * and sequences whose numbers do not fit are left alone in d_q_out too. */
+int mgh_kv8_append_rope(mgh_ctx* ctx, const mgh_kv8* cache, const mgh_rotation* rot, const void* d_k, const void* d_v, int in_f16,
+                        const int64_t strides[4], int S, const int32_t* d_lens, const int32_t* d_new, const void* d_q,
+                        const int64_t q_strides[4], int H, void* d_q_out, const int64_t q_out_strides[4]);
 /* lens[b] += new[b] (S where d_new is NULL). A negative length, new tokens outside 0 .. S and a sum past 2^31 - 1
  * leave lens[b] as it is, so a sequence that append left alone stays refused; one that ran past its table gets a
  * length past it: set that back before the table is made wider. */
@@ -473,6 +509,15 @@ int mgh_kv8_advance(mgh_ctx* ctx, int32_t* d_lens, const int32_t* d_new, int B, 
 int mgh_kv8_attn(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_q, int in_f16, const int64_t q_strides[4], int S,
                  const int32_t* d_lens, const int32_t* d_new, int H, float scale, float cap, const float* d_slopes,
                  float* d_o, void* d_o16, const int64_t o_strides[4]);
+/* mgh_kv8_attn where sequences share their first blocks (a prompt that many go on from): `group` sequences in a row are
+ * a group (the last one may have fewer), and d_shared[g] blocks of group g, 0 .. max_shared, are read from the first of its
+ * sequences' rows of the table once for all of them (the other rows' entries for these blocks are not read). Each of
+ * its sequences must be at least that long (lens[b] >= 32 shared): one that is shorter gives NaN rows, as do all of a
+ * group whose number does not fit. The result is mgh_kv8_attn's but for the last bits. Partial results are
+ * kept in the context's workspace: run a shape once before it is captured. */
+int mgh_kv8_attn_shared(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_q, int in_f16, const int64_t q_strides[4], int S,
+                        const int32_t* d_lens, const int32_t* d_new, int group, const int32_t* d_shared, int max_shared, int H,
+                        float scale, float cap, const float* d_slopes, float* d_o, void* d_o16, const int64_t o_strides[4]);
 /* the values that the cache holds at positions first[b] + i (d_first NULL: i), i < n, of a sequence of
  * lens[b] tokens -> [B][Hkv][n][D], fp32 in d_k and d_v or fp16 in d_k16 and d_v16; rows at or past lens[b]
  * are left as they were */
@@ -503,6 +548,27 @@ typedef struct mgh_logits_opts {
 } mgh_logits_opts;
 int mgh_logits_process(mgh_ctx* ctx, const void* d_x, int f16, int64_t x_stride, int rows, int V,
                        const mgh_logits_opts* opts, void* d_y, int64_t y_stride);
+
+/* ---- a token drawn from each row of logits, with random numbers that the caller brings. No counterpart in the
+ *      reference, whose generate() draws with its own engine (mg-generate.cpp:89-97; mgh_decode_step). x: rows of V logits
+ *      x_stride apart (0: one row for all draws), fp32 or fp16. With T the row's temperature and m its largest logit
+ *      a token weighs w = exp((l - m) / T). In the order of descending logits, equal ones by their ids, the tokens kept are
+ *      the shortest of: the first top_k (0 or less, V or more: all); the fewest whose weights sum to top_p of those first
+ *      top_k's sum or more (1 or more: all; at least one); those with w >= min_p (0 or less: all; 1 or more: the
+ *      largest). d_ids[r] is the first kept token, in the order of the ids, whose running sum of weights exceeds
+ *      d_u[r] (0 <= u < 1) times the kept ones' sum; d_prob[r] (nullable) its weight's share of that sum. T that is not
+ *      above 0: the largest logit, lowest id. A row without a logit above -infinity, or with a NaN: id -1, prob 0 or NaN.
+ *      Where infinity is among a row's logits only they weigh. Weights are fp64, counted in 2^-S of the largest
+ *      (S = 51, less where V is past 2048: 62 - log2 V), and summed exactly, so ids depend neither on the order of the
+ *      sums nor on the other rows. Each part is left out where its pointer is NULL (temperature: 1). V up to 2^24. ---- */
+typedef struct mgh_sample_opts {
+    const float* d_temp;         /* [rows], as the others */
+    const int32_t* d_top_k;
+    const float* d_top_p;
+    const float* d_min_p;
+} mgh_sample_opts;
+int mgh_sample(mgh_ctx* ctx, const void* d_x, int f16, int64_t x_stride, int rows, int V, const mgh_sample_opts* opts,
+               const float* d_u, int32_t* d_ids, float* d_prob);
 
 /* ---- debug: the int32 per-block dot products exactly as the production GEMM's MFMA
  *      computes them, out[m][n][t] (t = K/32 blocks). The reference has no counterpart;

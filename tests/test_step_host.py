@@ -1,0 +1,175 @@
+"""The host side of rotary positions, rotated appending, attention over shared blocks and sampling without a GPU: what
+each call refuses, that a refused or empty call launches nothing, and which kernels the others take, on the recording HIP
+runtime of tests/test_dispatch.py."""
+import numpy as np
+import pytest
+
+import edge_maskgit_amd as ema
+from tests import step_oracle as ref
+from tests.test_dispatch import fake_hip, run  # noqa: F401 (the fixture builds the runtime)
+from tests.test_generate_host import BODY
+
+ROPE = BODY + """
+F = [1.0] * 64
+def rot(pairs=(8,), freqs=F, order=0, pos=None, **kw):
+    return ema.Rope(pairs, freqs, order, pos, **kw)
+"""
+
+
+def test_rope_refusals():
+    run(ROPE + """
+st = (1, 64, 16, 64 * 9)
+def call(r=None, x=W, x_st=st, D=16, S=9, H=4, Bn=2, y=Y, **kw):
+    c.rope(rot() if r is None else r, x, x_st, D, S, H, Bn, y=y, **kw)
+call()
+assert kernels() == ["k_rope"]
+call(y=None, y16=Y, in16=False)
+call(x=W, y=W, in16=False)                          # in place
+kernels()
+big = rot()
+big.axes = 5
+none = rot()
+none.axes = 0
+for r, what in ((big, "1 to 4 axes"), (none, "1 to 4 axes"), (rot((9,)), "pairs"), (rot((-1,)), "pairs"), (rot((4, 5)), "more pairs"), (rot(order=3), "order"),
+                (rot(order=-1), "order"), (rot(freqs=[float("nan")] * 8), "frequencies"), (rot(freqs=[float("inf")] * 8), "frequencies"),
+                (rot(freqs=[1.0] * 7 + [16.5]), "frequencies"), (rot(pos=R + 2), "aligned")):
+    refused(call, r, what=what)
+for kw, what in (({"D": 15}, "even"), ({"D": 130}, "even"), ({"D": 0}, "even"), ({"S": -1}, "negative"), ({"H": -1}, "negative"), ({"Bn": -1}, "negative"),
+                 ({"y": None}, "exactly one"), ({"y16": G}, "exactly one"), ({"x": None}, "null"), ({"x": W + 1}, "aligned"), ({"x": W + 2, "in16": False}, "aligned"),
+                 ({"y": Y + 2}, "aligned"), ({"y": None, "y16": Y + 1}, "aligned"), ({"first": R + 1}, "aligned"), ({"new": R + 2}, "aligned"),
+                 ({"y": W}, "in place"), ({"y": W, "in16": False, "y_strides": (1, 64, 16, 64 * 10)}, "in place"), ({"Bn": 65536}, "at most"), ({"H": 65536}, "at most"),
+                 ({"S": 2 ** 28 + 1}, "at most"), ({"S": 2 ** 28, "H": 3}, "at most")):
+    refused(call, what=what, **kw)
+L = ema.lib()
+four = (ctypes.c_int64 * 4)(*st)
+r = rot()
+assert L.mgh_rope(c.h, None, W, 1, four, 16, 9, 4, 2, None, None, Y, None, four) == -1
+assert L.mgh_rope(c.h, ctypes.byref(r), W, 2, four, 16, 9, 4, 2, None, None, Y, None, four) == -1
+assert L.mgh_rope(c.h, ctypes.byref(r), W, 1, None, 16, 9, 4, 2, None, None, Y, None, four) == -1
+assert L.mgh_rope(None, ctypes.byref(r), W, 1, four, 16, 9, 4, 2, None, None, Y, None, four) == -1
+r.h_freqs = None
+refused(call, r, what="null frequencies")
+for kw in ({"S": 0}, {"H": 0}, {"Bn": 0}):
+    nothing(call, **kw)
+call(rot((0,), []))                                 # nothing turns: a copy
+assert kernels() == ["k_rope"]
+try:
+    ema.Rope((8,), [1.0] * 7)
+    raise SystemExit("accepted")
+except ema.MghError:
+    pass
+""")
+
+
+def test_rotated_append_refusals():
+    run(ROPE + """
+def kv(k=W, v=X, scales=B, kt=R, vt=Y, table=G, nb=4, pages=9, Hkv=2, D=32, Bn=3, **kw):
+    return ema.Kv8(k, v, scales, kt, vt, table, nb, pages, Hkv, D, Bn, **kw)
+Q, O, N = (0x100000 * i for i in (17, 18, 19))
+st = (1, 64, 32, 64 * 5)
+qst = (1, 128, 32, 128 * 5)
+def call(h=None, r=None, S=5, lens=N, k=Q, v=Q, **kw):
+    c.kv8_append_rope(kv() if h is None else h, rot() if r is None else r, k, v, st, S, lens, **kw)
+q = dict(q=O, q_strides=qst, H=4, q_out=O + 0x80000, qo_strides=qst)
+call()
+call(**q)
+call(**dict(q, q_out=O))
+assert kernels() == ["k_kv8_append_rope"] * 3
+nothing(call, S=0)
+nothing(call, kv(Bn=0))
+for kw, what in (({"Hkv": 0}, "Hkv, D > 0"), ({"D": 20}, "D must"), ({"table_stride": 3}, "table_stride"), ({"kt": None}, "null"), ({"k": W + 8}, "aligned")):
+    refused(call, kv(**kw), what=what)
+refused(call, r=rot((17,)), what="pairs")
+refused(call, r=rot(order=7), what="order")
+for kw, what in (({"S": -1}, "negative"), ({"S": 2 ** 28 + 1}, "2^28"), ({"lens": None}, "null"), ({"lens": N + 2}, "aligned"), ({"k": None}, "null"), ({"v": None}, "null"),
+                 ({"k": Q + 1}, "aligned"), (dict(q, q=O + 1), "aligned"), (dict(q, H=3), "H % Hkv"), (dict(q, H=0), "H % Hkv"), (dict(q, q_out=None), "null"),
+                 (dict(q, q_strides=None), "null"), (dict(q, qo_strides=None), "null"), (dict(q, q_out=O + 1), "aligned"), (dict(q, q_out=O, in16=False), "in place"),
+                 (dict(q, q_out=O, qo_strides=(1, 256, 32, 1280)), "in place"), (dict(q, H=70000), "65535")):
+    refused(call, what=what, **kw)
+assert ema.lib().mgh_kv8_append_rope(c.h, ctypes.byref(kv()), None, Q, Q, 1, (ctypes.c_int64 * 4)(*st), 1, N, None, None, None, 0, None, None) == -1
+assert ema.lib().mgh_kv8_append_rope(None, ctypes.byref(kv()), ctypes.byref(rot()), Q, Q, 1, None, 1, N, None, None, None, 0, None, None) == -1
+""")
+
+
+def test_shared_attention_refusals():
+    run(BODY + """
+def kv(k=W, v=X, scales=B, kt=R, vt=Y, table=G, nb=4, pages=9, Hkv=2, D=32, Bn=3, **kw):
+    return ema.Kv8(k, v, scales, kt, vt, table, nb, pages, Hkv, D, Bn, **kw)
+Q, O, N, M = (0x100000 * i for i in (17, 18, 19, 20))
+st = (1, 64, 32, 64 * 5)
+def call(h=None, S=5, lens=N, q=Q, H=2, scale=0.1, o16=O, group=2, shared=M, most=3, **kw):
+    c.kv8_attn_shared(kv() if h is None else h, q, st, S, lens, None, group, shared, most, H, scale, o16=o16, **kw)
+call()
+assert kernels()
+nothing(call, S=0)
+nothing(call, kv(Bn=0))
+for kw, what in (({"Hkv": 0}, "Hkv, D > 0"), ({"D": 160}, "D must"), ({"table": None}, "null"), ({"vt": Y + 2}, "aligned")):
+    refused(call, kv(**kw), what=what)
+for kw, what in (({"H": 3}, "H % Hkv"), ({"scale": float("nan")}, "scale"), ({"cap": -2.0}, "cap"), ({"o": W}, "exactly one"), ({"o16": None}, "exactly one"),
+                 ({"q": None}, "null"), ({"q": Q + 1}, "aligned"), ({"slopes": N + 1}, "aligned"), ({"S": 2 ** 24 + 1}, "2^24"), ({"group": 0}, "group"), ({"group": -3}, "group"),
+                 ({"most": -1}, "max_shared"), ({"most": 5}, "max_shared"), ({"shared": None}, "null"), ({"shared": M + 2}, "aligned"), ({"lens": None}, "null"),
+                 ({"S": 2 ** 23}, "2^24")):
+    refused(call, what=what, **kw)
+call(group=1000)                                    # one group
+assert kernels()
+assert ema.lib().mgh_kv8_attn_shared(None, ctypes.byref(kv()), Q, 1, None, 1, N, None, 1, M, 1, 2, 0.1, 0.0, None, None, O, None) == -1
+""")
+
+
+def test_sample_refusals():
+    run(BODY + """
+def call(x=W, rows=3, V=1000, u=X, ids=Y, **kw):
+    c.sample(x, rows, V, u, ids, **kw)
+call()
+assert kernels()
+call(x_stride=0)
+call(rows=1, x_stride=7)
+kernels()
+for kw, what in (({"x": None}, "null"), ({"u": None}, "null"), ({"ids": None}, "null"), ({"rows": -1}, "negative"), ({"V": -1}, "negative"), ({"V": 0}, "without"),
+                 ({"V": 2 ** 24 + 1}, "at most"), ({"rows": 2 ** 20 + 1}, "at most"), ({"x_stride": 999}, "x_stride"), ({"x_stride": -1000}, "x_stride"), ({"x": W + 2}, "aligned"),
+                 ({"x": W + 1, "f16": True}, "aligned"), ({"u": X + 1}, "aligned"), ({"temp": R + 2}, "aligned"), ({"top_k": R + 2}, "aligned"),
+                 ({"top_p": R + 1}, "aligned"), ({"min_p": R + 3}, "aligned"), ({"prob": R + 2}, "aligned"), ({"ids": Y + 2}, "aligned")):
+    refused(call, what=what, **kw)
+nothing(call, rows=0)
+L = ema.lib()
+assert L.mgh_sample(c.h, W, 2, 9, 1, 9, None, X, Y, None) == -1
+assert L.mgh_sample(None, W, 0, 9, 1, 9, None, X, Y, None) == -1
+""")
+
+
+@pytest.mark.parametrize("order", [0, 1, 2])
+def test_oracle_turns_every_feature_once(order):
+    pairs = [3, 0, 2]
+    seen = sorted(f for ab in ref.features(pairs, order) for f in ab)
+    assert seen == list(range(10))
+    x = np.random.default_rng(0).standard_normal((1, 4, 1, 12))
+    pos = np.stack([np.arange(4)[None] * (a + 1) for a in range(3)])
+    y = ref.rope(x, pos, pairs, [0.3, 0.2, 0.1, 1.0, 0.5], order)
+    back = ref.rope(y, -pos, pairs, [0.3, 0.2, 0.1, 1.0, 0.5], order)
+    assert np.allclose(back, x, atol=1e-12) and np.array_equal(y[..., 10:], x[..., 10:]) and np.array_equal(y[:, 0], x[:, 0])
+
+
+def test_oracle_rotation_depends_on_the_distance():
+    """products of a rotated query and key depend on the difference of their positions"""
+    rng = np.random.default_rng(1)
+    q, k = rng.standard_normal((2, 1, 1, 1, 8))
+    f = [1.0, 0.1, 0.01, 0.001]
+    dots = [float((ref.rope(q, [[[p + 7]]], [4], f, 0) * ref.rope(k, [[[p]]], [4], f, 0)).sum()) for p in (0, 5, 1000)]
+    assert np.allclose(dots, dots[0], atol=1e-11)
+
+
+def test_oracle_keeps_what_the_definition_says():
+    x = np.log(np.array([0.1, 0.4, 0.2, 0.2, 0.1]))
+    tokens = lambda **kw: np.nonzero(ref.kept(x, **kw))[0].tolist()  # noqa: E731
+    assert tokens() == [0, 1, 2, 3, 4]
+    assert tokens(top_k=2) == [1, 2] and tokens(top_k=4) == [0, 1, 2, 3]          # equal logits by their ids
+    assert tokens(top_p=0.5) == [1, 2] and tokens(top_p=0.0) == [1] and tokens(top_p=0.79) == [1, 2, 3]
+    assert tokens(top_k=3, top_p=0.7) == [1, 2] and tokens(min_p=0.4) == [1, 2, 3] and tokens(min_p=2.0) == [1]
+    assert ref.sample(x, 0.45)[0] == 1 and ref.sample(x, 0.05)[0] == 0 and ref.sample(x, 0.95)[0] == 4
+    assert ref.sample(x, 0.9, temp=0.0)[0] == 1 and ref.sample(x, 1.0)[0] == 4
+
+
+def test_entry_points_take_no_context():
+    L = ema.lib()
+    assert L.mgh_sample(None, None, 0, 1, 1, 1, None, None, None, None) == -1
+    assert L.mgh_rope(None, None, None, 0, None, 2, 1, 1, 1, None, None, None, None, None) == -1
