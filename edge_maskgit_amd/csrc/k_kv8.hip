@@ -62,6 +62,9 @@ template <bool IN16, bool VEC, int ROT>
 __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotation* r) {
     __shared__ uint32_t mx[2][4];
     const Kv8& c = a.c;
+    if constexpr (ROT != 0)
+        asm volatile("" ::"s"(c.k), "s"(c.v), "s"(c.scales), "s"(c.k_tail), "s"(c.v_tail), "s"(c.table), "s"(c.table_stride), "s"(c.pages),
+                     "s"(a.k), "s"(a.v), "s"(a.st[0]), "s"(a.st[1]), "s"(a.st[2]), "s"(a.st[3]));
     const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, D = c.D;
     int len, total;
     if (!spans(c, a.lens, a.fresh, a.S, b, len, total)) return;
@@ -123,6 +126,9 @@ __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotat
             load_row<16, IN16, VEC>(a.k, at(t, 16 * u), a.st[0], x);
         } else {
             const TokenPos p = token_pos(*r, b, t - len, t);
+            Turns<ROT> f[NU / 2];
+#pragma unroll
+            for (int g = 0; g < NU / 2; g++) f[g].load(*r, 8 * u + ROT * g);
             float v[16];
             runs(u, [&](int i, int d) { load_features<ROT, IN16, VEC>(a.k, at(t, d), a.st[0], v + i); });
 #pragma unroll
@@ -130,7 +136,7 @@ __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotat
                 const int pair = 8 * u + ROT * g;
                 if (pair < r->P) {
                     SinCos sc[ROT];
-                    angles<ROT>(*r, p, pair, sc);
+                    angles<ROT>(*r, p, f[g], pair, sc);
                     rotate<ROT>(*r, sc, v + 2 * ROT * g);
                 }
             }
@@ -269,21 +275,27 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
 // V pairs of one head of one token per thread.
 template <bool IN16, bool VEC, int ROT, int V>
 __global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int blocks) {
+    ask_rotation(a.r);
+    asm volatile("" ::"s"(a.a.c.max_blocks), "s"(a.a.c.D), "s"(a.a.c.Hkv), "s"(a.a.lens), "s"(a.a.fresh), "s"(a.a.S));
     if ((int)blockIdx.x < blocks) {
         append_block<IN16, VEC, ROT>(a.a, &a.r);
         return;
     }
     const Kv8& c = a.a.c;
+    asm volatile("" ::"s"(a.q), "s"(a.qo), "s"(a.qst[0]), "s"(a.qst[1]), "s"(a.qst[2]), "s"(a.qst[3]), "s"(a.qost[0]), "s"(a.qost[1]),
+                 "s"(a.qost[2]), "s"(a.qost[3]), "s"(a.H), "s"(c.Hkv), "s"(c.D));
     const int hk = blockIdx.y, b = blockIdx.z, G = a.H / c.Hkv, units = c.D / (2 * V), per = units * G;
-    int len, total;
-    if (!spans(c, a.a.lens, a.a.fresh, a.a.S, b, len, total)) return;
-    const int64_t at = (int64_t)(blockIdx.x - blocks) * 256, i0 = at / per;
+    const uint32_t at = (blockIdx.x - blocks) * 256u, i0 = at / per;
     const int x = (int)(at - i0 * per) + threadIdx.x, di = x / per, item = x - di * per;
-    const int64_t i = i0 + di;
-    if (i >= total - len) return;
-    const int g = item / units, pair = (item - g * units) * V, h = hk * G + g;
-    rope_heads<V, IN16, true, (V > 1)>(a.r, token_pos(a.r, b, i, len + i), pair, a.q, b * a.qst[3] + i * a.qst[1] + h * a.qst[2], 0,
-                                       a.qst[0], a.qo, b * a.qost[3] + i * a.qost[1] + h * a.qost[2], 0, a.qost[0], 1);
+    const int i = (int)i0 + di, g = item / units, pair = (item - g * units) * V, h = hk * G + g;
+    Turns<V> f;
+    f.load(a.r, pair);
+    int len, total;
+    const bool fits = spans(c, a.a.lens, a.a.fresh, a.a.S, b, len, total);
+    const TokenPos t = token_pos(a.r, b, min(i, a.a.S - 1), len + i);
+    if (!fits || i >= total - len) return;
+    rope_heads<V, IN16, true, (V > 1)>(a.r, t, f, pair, a.q, b * a.qst[3] + i * a.qst[1] + h * a.qst[2], 0, a.qst[0], a.qo,
+                                       b * a.qost[3] + i * a.qost[1] + h * a.qost[2], 0, a.qost[0], 1);
 }
 
 // Values of tokens [first, first + n) that a sequence has: codes times their scale, or the ring's fp16. One

@@ -27,25 +27,41 @@ __device__ __forceinline__ SinCos sincos_turns(uint32_t t) {
 // the highest 32 bits of p F mod 2^64
 __device__ __forceinline__ uint32_t turns_at(int32_t p, uint64_t F) { return (uint32_t)(((uint64_t)(int64_t)p * F) >> 32); }
 
-// a token's positions along the axes; `i` its index in the call, `run` its position where none are given
+// a token's positions along the axes (`i` its index in the call, `run` its position where none are given): loads that
+// depend on nothing but the arguments, all four of them, so that none waits for another
 struct TokenPos {
-    int32_t p[4];
+    int32_t p0, p1, p2, p3;
+    // (by masks: a choice between members would keep them in memory)
     __device__ __forceinline__ int32_t of(const Rotation& r, int pair) const {
-        int32_t x = p[0];
-#pragma unroll
-        for (int a = 1; a < 4; a++) x = pair >= r.start[a] ? p[a] : x;
-        return x;
+        auto pick = [](int32_t a, int32_t b, bool c) {
+            const int32_t m = -(int32_t)c;
+            return (b & m) | (a & ~m);
+        };
+        return pick(pick(pick(p0, p1, pair >= r.start[1]), p2, pair >= r.start[2]), p3, pair >= r.start[3]);
     }
 };
-__device__ __forceinline__ TokenPos token_pos(const Rotation& r, int64_t b, int64_t i, int64_t run) {
-    TokenPos t;
+__device__ __forceinline__ TokenPos token_pos(const Rotation& r, int64_t b, int64_t i, int32_t run) {
+    if (!r.pos) return {run, run, run, run};
+    const int32_t* p = r.pos + i * r.pst[0] + b * r.pst[1];
+    const int64_t st = r.pst[2];
+    return {p[0], p[r.axes > 1 ? st : 0], p[r.axes > 2 ? 2 * st : 0], p[r.axes > 3 ? 3 * st : 0]};
+}
+
+// V pairs' turns per unit of position
+template <int V>
+struct Turns {
+    uint64_t f[V];
+    __device__ __forceinline__ void load(const Rotation& r, int pair) {      // (the table is as long as a row may be)
 #pragma unroll
-    for (int a = 0; a < 4; a++) {
-        if (!r.pos) t.p[a] = (int32_t)run;
-        else if (a < r.axes) t.p[a] = r.pos[i * r.pst[0] + b * r.pst[1] + a * r.pst[2]];
-        else t.p[a] = 0;
+        for (int i = 0; i < V; i++) f[i] = r.turn[pair + i];
     }
-    return t;
+};
+
+// The arguments that every thread needs, asked for at once where this stands: left to itself the compiler loads each
+// where it is used, behind the branches before it, a round trip to memory at a time.
+__device__ __forceinline__ void ask_rotation(const Rotation& r) {
+    asm volatile("" ::"s"(r.axes), "s"(r.P), "s"(r.order), "s"(r.start[1]), "s"(r.start[2]), "s"(r.start[3]), "s"(r.start[4]), "s"(r.pos),
+                 "s"(r.pst[0]), "s"(r.pst[1]), "s"(r.pst[2]));
 }
 
 // Where the features of V pairs in a row lie: V from fa on and V from fb on. Pairs past the rotated ones are the rest of the
@@ -65,9 +81,9 @@ __device__ __forceinline__ Where pairs_at(const Rotation& r, int pair, int V) {
 
 // cos and sin of V pairs
 template <int V>
-__device__ __forceinline__ void angles(const Rotation& r, const TokenPos& t, int pair, SinCos* sc) {
+__device__ __forceinline__ void angles(const Rotation& r, const TokenPos& t, const Turns<V>& f, int pair, SinCos* sc) {
 #pragma unroll
-    for (int i = 0; i < V; i++) sc[i] = sincos_turns(turns_at(t.of(r, pair + i), r.turn[pair + i]));
+    for (int i = 0; i < V; i++) sc[i] = sincos_turns(turns_at(t.of(r, pair + i), f.f[i]));
 }
 
 // x: V features from fa on, V from fb on
@@ -143,16 +159,16 @@ __device__ __forceinline__ void store_features(void* p, int64_t e, int64_t st, c
 
 // V pairs of `n` heads `step` apart, of one token: the angles once, then head by head. x and y: the token's first of these heads
 template <int V, bool IN16, bool OUT16, bool VEC>
-__device__ __forceinline__ void rope_heads(const Rotation& r, const TokenPos& t, int pair, const void* x, int64_t ex, int64_t hx,
+__device__ __forceinline__ void rope_heads(const Rotation& r, const TokenPos& t, const Turns<V>& f, int pair, const void* x, int64_t ex, int64_t hx,
                                            int64_t dx, void* y, int64_t ey, int64_t hy, int64_t dy, int n) {
     const Where w = pairs_at(r, pair, V);
     const bool turned = pair < r.P;
     SinCos sc[V];
-    if (turned) angles<V>(r, t, pair, sc);
     for (int h = 0; h < n; h++) {
         float v[2 * V];
         load_features<V, IN16, VEC>(x, ex + h * hx + w.fa * dx, dx, v);
         load_features<V, IN16, VEC>(x, ex + h * hx + w.fb * dx, dx, v + V);
+        if (h == 0) angles<V>(r, t, f, pair, sc);         // while the first head's features are on their way
         if (turned) rotate<V>(r, sc, v);
         store_features<V, OUT16, VEC>(y, ey + h * hy + w.fa * dy, dy, v);
         store_features<V, OUT16, VEC>(y, ey + h * hy + w.fb * dy, dy, v + V);

@@ -14,17 +14,22 @@ namespace {
 template <int V, bool IN16, bool OUT16>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs a, int HG) {
     const Rotation& r = a.r;
+    ask_rotation(r);
+    asm volatile("" ::"s"(a.x), "s"(a.y), "s"(a.xst[0]), "s"(a.xst[1]), "s"(a.xst[2]), "s"(a.xst[3]), "s"(a.yst[0]), "s"(a.yst[1]), "s"(a.yst[2]),
+                 "s"(a.yst[3]), "s"(a.D), "s"(a.S), "s"(a.H), "s"(a.first), "s"(a.fresh));
     const int units = a.D / (2 * V), per = units * HG, b = blockIdx.y;
-    const int64_t at = (int64_t)blockIdx.x * 256, i0 = at / per;
+    const uint32_t at = blockIdx.x * 256u, i0 = at / per;
     const int x = (int)(at - i0 * per) + threadIdx.x, di = x / per, item = x - di * per;
-    const int64_t i = i0 + di;
-    const int n = a.fresh ? a.fresh[b] : a.S;
+    const int i = (int)i0 + di, hl = item / units, pair = (item - hl * units) * V;
+    Turns<V> f;
+    f.load(r, pair);
+    const TokenPos t = token_pos(r, b, min(i, a.S - 1), (a.first ? a.first[b] : 0) + i);
+    int n = a.S;
+    asm volatile("" : "+s"(n));                          // (else loaded by a pointer chosen between the two)
+    if (a.fresh) n = a.fresh[b];
     if (i >= n || n > a.S) return;
-    const int hl = item / units, pair = (item - hl * units) * V;
-    const int64_t run = (a.first ? a.first[b] : 0) + i;
-    rope_heads<V, IN16, OUT16, (V > 1)>(r, token_pos(r, b, i, run), pair, a.x, b * a.xst[3] + i * a.xst[1] + hl * a.xst[2], HG * a.xst[2],
-                                    a.xst[0], a.y, b * a.yst[3] + i * a.yst[1] + hl * a.yst[2], HG * a.yst[2], a.yst[0],
-                                    (a.H - hl + HG - 1) / HG);
+    rope_heads<V, IN16, OUT16, (V > 1)>(r, t, f, pair, a.x, b * a.xst[3] + i * a.xst[1] + hl * a.xst[2], HG * a.xst[2], a.xst[0], a.y,
+                                        b * a.yst[3] + i * a.yst[1] + hl * a.yst[2], HG * a.yst[2], a.yst[0], (a.H - hl + HG - 1) / HG);
 }
 
 template <int V>

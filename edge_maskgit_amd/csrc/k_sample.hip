@@ -4,9 +4,16 @@
 // the shortest prefix of that order which top-k (its length), top-p (its share of the first k's mass) and min-p (its
 // last w) allow; drawn is the first kept token, in the order of the ids, whose running sum exceeds u times the kept mass.
 //
+// A token's place in that order is a whole number of 64 bits (its key's complement, then its id), and what is kept is all up
+// to one place. Where that lies, for top-k and then for top-p: tokens are counted and their masses summed by bins of
+// log2 w, the bin that the border falls into is found by a scan, and its tokens (few) are ranked against one another;
+// more than a list holds are first shared out again by their places, as often as it takes.
+//
 // Which token a sum's border falls on must not depend on how sums are split, so masses are whole numbers of 2^-S of the
 // largest weight, exp2 in 64 bits rounded once: they add up exactly in any order, atomics included. S leaves room for the
 // row (63 bits for its sum) and is at most 51, where the rounding is an addition of 2^52.
+#include <algorithm>
+
 #include "mgh_common.h"
 #include "mgh_kernels.h"
 
@@ -57,191 +64,633 @@ struct Weights {
     }
 };
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d), hi = __shfl_up((uint32_t)(v >> 32), d);
-    return (uint64_t)hi << 32 | lo;
-}
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int l) {
-    const uint32_t lo = __shfl((uint32_t)v, l), hi = __shfl((uint32_t)(v >> 32), l);
-    return (uint64_t)hi << 32 | lo;
-}
 // sums of the lanes up to and with this one
-__device__ __forceinline__ uint64_t scan64(uint64_t v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = shfl_up64(v, d);
-        if (lane >= d) v += o;
-    }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t scan64(uint64_t v) {
+    v += moved<0x111, 0xf>(v);           // one, two, four, eight lanes up within rows of 16
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);           // a row's last lane to the next row, then the first half's to the second
+    v += moved<0x143, 0xc>(v);
     return v;
 }
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+}
+__device__ __forceinline__ uint64_t sum64(uint64_t v) { return lane64(scan64(v), 63); }
 
-// One workgroup per row, passes over the row in memory.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_sample(SampleArgs a) {
-    __shared__ uint32_t cnt[256];
-    __shared__ uint64_t mass[256], seg[kWaves];
-    __shared__ uint32_t ties[kWaves];
-    __shared__ float redf[kWaves];
-    __shared__ int redi[kWaves];
-    __shared__ uint64_t picked[4];
+constexpr int kBins = 512, kMostWaves = 16;
+typedef unsigned long long ull;
+
+// LIST: tokens of a bin that it holds
+template <int LIST, int THREADS>
+struct Lds {
+    static constexpr int kList = LIST, kThreads = THREADS;
+    uint64_t mass[kBins], place[LIST + 64], w[LIST + 64];      // (the last 64: those that are ranked)
+    uint64_t part[kMostWaves], lo[kMostWaves], hi[kMostWaves], found[4];
+    uint32_t cnt[kBins];
+    float redf[kMostWaves][2];
+    int redi[kMostWaves];
+    uint32_t n;
+};
+
+// what a row asks for
+struct Ask {
+    float temp, top_p, min_p, u;
+    int k;
+    bool greedy, by_k, by_p;
+};
+__device__ __forceinline__ Ask ask_of(const SampleArgs& a, int64_t row) {
+    Ask q;
+    q.temp = a.temp ? a.temp[row] : 1.f;
+    q.k = a.top_k ? a.top_k[row] : 0;
+    q.top_p = a.top_p ? a.top_p[row] : 1.f;
+    q.min_p = a.min_p ? a.min_p[row] : 0.f;
+    q.u = a.u[row];
+    q.greedy = !(q.temp > 0.f);
+    q.by_k = q.k > 0 && q.k < a.V;
+    q.by_p = q.top_p < 1.f;
+    return q;
+}
+
+// weights and bins of a row whose logits lie between lo (the least that is finite) and m
+struct Scale {
+    Weights wt;
+    double cs;             // bins per unit of logit
+    __device__ __forceinline__ Scale(float m, float lo, float temp, double unit) {
+        wt = Weights{(double)m, 1.4426950408889634 / (double)temp, unit};
+        const double span = ((double)m - (double)lo) * wt.c, r = span < 64. ? span : 64.;
+        cs = span > 0. ? wt.c * ((kBins - 1) / r) : 0.;
+    }
+    __device__ __forceinline__ int bin(float l) const {
+        const double x = (wt.m - (double)l) * cs;
+        return (double)l == wt.m ? 0 : x < kBins - 1 ? (int)x : kBins - 1;
+    }
+    __device__ __forceinline__ uint64_t mass(float l) const { return wt.mass(wt.of(l)); }
+};
+__device__ __forceinline__ uint64_t place_of(float l, int i) { return (uint64_t)(~key_of(l)) << 32 | (uint32_t)i; }
+
+// Where a running count or mass, over the bins in order, reaches `k` or `target`: found = count and mass before the bin, its
+// number, its count. By wave 0; the others wait.
+template <class L>
+__device__ __forceinline__ void find_bin(L& s, bool by_count, uint64_t k, double target, uint64_t n, uint64_t m) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid < 64) {
+        constexpr int E = kBins / 64;
+        uint32_t c[E];
+        uint64_t w[E], cn = 0, wn = 0;
+#pragma unroll
+        for (int j = 0; j < E; j++) cn += c[j] = s.cnt[E * tid + j], wn += w[j] = s.mass[E * tid + j];
+        n += scan64(cn) - cn;
+        m += scan64(wn) - wn;
+        auto there = [&](uint64_t nn, uint64_t mm) { return by_count ? nn >= k : (double)mm >= target; };
+        const uint64_t who = __ballot(cn && there(n + cn, m + wn)), held = __ballot(cn != 0);
+        // (a target that rounding puts past the whole mass: the last bin that holds something)
+        if (tid == (who ? __builtin_ctzll(who) : 63 - __builtin_clzll(held))) {
+            int at = -1;
+            uint32_t have = 0;
+            uint64_t weight = 0;
+            bool done = false;
+#pragma unroll
+            for (int j = 0; j < E; j++) {
+                if (done || !c[j]) continue;
+                n += have, m += weight;
+                at = E * tid + j, have = c[j], weight = w[j];
+                done = there(n + have, m + weight);
+            }
+            s.found[0] = n, s.found[1] = m, s.found[2] = (uint64_t)at, s.found[3] = have;
+        }
+    }
+    __syncthreads();
+}
+
+struct Cut {
+    uint64_t place;        // of the last token kept
+    uint64_t mass;         // of the tokens up to it
+    int bin;               // whose tokens the list holds, -1: none
+    bool intact;           // the bins are as they were
+    uint32_t held;         // tokens of the bin
+};
+
+// The last place that a count of k or a mass of `target` keeps, at least the first: the row's bins are in s.cnt and s.mass;
+// each(bin, f) calls f(logit, id) for the tokens of a bin (and maybe others). A list is filled where it holds the bin.
+template <class L, class Each>
+__device__ __forceinline__ Cut cut_at(L& s, const Scale& sc, bool by_count, uint64_t k, double target, Each each) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nt = L::kThreads;
+    find_bin(s, by_count, k, target, 0, 0);
+    uint64_t n = s.found[0], m = s.found[1];
+    const int bin = (int)s.found[2];
+    uint32_t held = (uint32_t)s.found[3];
+    const uint32_t all = held;
+    const bool listed = L::kList && held <= (uint32_t)L::kList;
+    uint64_t lo = 0, hi = ~0ull;                         // places that are left
+    auto gather = [&](auto from, int at) {               // tokens left, in any order
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        from([&](uint64_t p, auto mass) {
+            if (p < lo || p > hi) return;
+            const uint32_t i = at + atomicAdd(&s.n, 1u);
+            s.place[i] = p, s.w[i] = mass();
+        });
+        __syncthreads();
+    };
+    auto row = [&](auto f) {
+        each(bin, [&](float l, int i) {
+            if (sc.bin(l) == bin) f(place_of(l, i), [&] { return sc.mass(l); });
+        });
+    };
+    auto list = [&](auto f) {
+        for (uint32_t i = tid; i < all; i += nt) f(s.place[i], [&] { return s.w[i]; });
+    };
+    if (listed) gather(row, 0);
+    auto narrow = [&](auto from) {                       // shared out again, by 9 bits of the span of the places left
+        uint64_t a = ~0ull, b = 0;
+        from([&](uint64_t p, auto) {
+            if (p >= lo && p <= hi) a = p < a ? p : a, b = p > b ? p : b;
+        });
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint64_t x = (uint64_t)__shfl_xor((ull)a, d), y = (uint64_t)__shfl_xor((ull)b, d);
+            a = x < a ? x : a, b = y > b ? y : b;
+        }
+        __syncthreads();
+        if (lane == 0) s.lo[wave] = a, s.hi[wave] = b;
+        for (int i = tid; i < kBins; i += nt) s.cnt[i] = 0, s.mass[i] = 0;
+        __syncthreads();
+        for (int w = 0; w < nt / 64; w++) a = s.lo[w] < a ? s.lo[w] : a, b = s.hi[w] > b ? s.hi[w] : b;
+        const int bits = b > a ? 64 - __builtin_clzll(b - a) : 0, shift = bits > 9 ? bits - 9 : 0;
+        from([&](uint64_t p, auto mass) {
+            if (p < a || p > b) return;
+            atomicAdd(&s.cnt[(p - a) >> shift], 1u);
+            atomicAdd((ull*)&s.mass[(p - a) >> shift], (ull)mass());
+        });
+        find_bin(s, by_count, k, target, n, m);
+        n = s.found[0], m = s.found[1], held = (uint32_t)s.found[3];
+        lo = a + (s.found[2] << shift);
+        hi = lo + ((1ull << shift) - 1);
+    };
+    bool intact = true;
+    while (held > 64) {
+        intact = false;
+        if (listed) narrow(list);
+        else narrow(row);
+    }
+    if (listed) gather(list, L::kList);
+    else gather(row, L::kList);
+    if (wave == 0) {                                     // ranked against one another
+        const uint64_t p = lane < (int)held ? s.place[L::kList + lane] : ~0ull, w = lane < (int)held ? s.w[L::kList + lane] : 0;
+        uint32_t rank = 0;
+        uint64_t before = 0;
+        for (uint32_t j = 0; j < held; j++) {
+            const bool b = lane64(p, j) < p;
+            rank += b;
+            before += b ? lane64(w, j) : 0;
+        }
+        const bool keep = lane < (int)held && (by_count ? n + rank < k : n + rank == 0 || (double)(m + before) < target);
+        const int last = __popcll(__ballot(keep));       // kept ones are the first of them
+        if (lane < (int)held && (int)rank + 1 == last) s.found[0] = p, s.found[1] = m + before + w;
+    }
+    __syncthreads();
+    const Cut c{s.found[0], s.found[1], listed ? bin : -1, intact, all};
+    __syncthreads();
+    return c;
+}
+
+// The least key whose weight is at least p (at most 1): 64 candidates at a time, by every wave for itself
+__device__ __forceinline__ uint32_t least_key(const Weights& wt, double p) {
+    const int lane = threadIdx.x & 63;
+    uint32_t lo = 0, hi = key_of((float)wt.m);
+    while (lo < hi) {                    // the key is in lo .. hi, and hi weighs enough
+        const uint32_t step = (hi - lo) / 64 + 1, off = step * lane;
+        const uint32_t x = off < hi - lo ? lo + off : hi;
+        const float l = logit_of(x);
+        const uint64_t ok = __ballot(l == l && wt.of(l) >= p);        // (keys below -infinity's are NaN)
+        const int first = ok ? __builtin_ctzll(ok) : 64;
+        if (first < 64) hi = (uint32_t)__builtin_amdgcn_readlane((int)x, first);
+        if (first > 0) lo = (uint32_t)__builtin_amdgcn_readlane((int)x, first - 1) + 1;
+    }
+    return hi;
+}
+
+// largest, least finite logit and whether there is a NaN, of a workgroup
+template <class L>
+__device__ __forceinline__ void reduce_range(L& s, float& m, float& lo, bool& nan) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d)), lo = fminf(lo, __shfl_xor(lo, d));
+    const bool any = __any(nan);
+    if (lane == 0) s.redf[wave][0] = m, s.redf[wave][1] = lo, s.redi[wave] = any;
+    __syncthreads();
+    nan = false;
+    for (int w = 0; w < L::kThreads / 64; w++) m = fmaxf(m, s.redf[w][0]), lo = fminf(lo, s.redf[w][1]), nan = nan || s.redi[w];
+}
+
+struct Answer {
+    int32_t* id;
+    float* prob;
+    __device__ __forceinline__ void put(int i, float p) const {
+        *id = i;
+        if (prob) *prob = p;
+    }
+};
+
+// masses of a workgroup's tokens (NV of a thread), wave by wave in s.part, and their sum
+template <int NV, class L>
+__device__ __forceinline__ uint64_t wave_sums(L& s, const uint64_t* mass) {
+    uint64_t v = 0;
+#pragma unroll
+    for (int j = 0; j < NV; j++) v += mass[j];
+    v = sum64(v);
+    if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint64_t all = 0;
+    for (int w = 0; w < L::kThreads / 64; w++) all += s.part[w];
+    return all;
+}
+// what a running sum must exceed: u of the whole, short of all of it
+__device__ __forceinline__ uint64_t draw_at(float u, uint64_t all) {
+    const double most = (double)all * (u > 0.f ? fmin((double)u, 1.) : 0.);
+    const uint64_t at = (uint64_t)most;
+    return at < all ? at : all - 1;
+}
+// The draw among a workgroup's tokens, of which (wave NV + j) 64 + lane weighs mass[j] (sums in s.part): `all` the row's mass, `at`
+// what the running sum must exceed, `ahead` the sum before the first token, id0 its id
+template <int NV, class L>
+__device__ __forceinline__ void draw(L& s, const uint64_t* mass, uint64_t ahead, uint64_t all, uint64_t at, int id0, const Answer& out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int w = 0; w < wave; w++) ahead += s.part[w];
+    if (at < ahead || at >= ahead + s.part[wave]) return;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const uint64_t run = ahead + scan64(mass[j]);
+        const uint64_t who = __ballot(run > at);
+        if (who) {
+            if (lane == __builtin_ctzll(who)) out.put(id0 + (wave * NV + j) * 64 + lane, (float)((double)mass[j] / (double)all));
+            return;
+        }
+        ahead = lane64(run, 63);
+    }
+}
+
+// Short rows: a workgroup holds a row in LDS, NV tokens of a thread: (wave NV + j) 64 + lane. Top-k counts only, so that with
+// it the exponentials are those of the first k tokens.
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT) void k_sample(SampleArgs a) {
+    __shared__ Lds<0, NT> s;
+    __shared__ float val[NT * NV];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.V;
     const int64_t row = blockIdx.x;
     const T* x = (const T*)a.x + row * a.x_stride;
-    float m = -INFINITY;
+    const Answer out{a.ids + row, a.prob ? a.prob + row : nullptr};
+    float m = -INFINITY, lo = INFINITY;
     bool nan = false;
-    for (int i = tid; i < V; i += kThreads) {
-        const float l = (float)x[i];
-        nan = nan || l != l;
-        m = fmaxf(m, l);
-    }
+    const int first = wave * NV * 64 + lane;
+    {
+        float l[NV];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    const bool any = __any(nan);
-    if (lane == 0) redf[wave] = m, redi[wave] = any;
-    __syncthreads();
-    nan = false;
-    for (int w = 0; w < kWaves; w++) m = fmaxf(m, redf[w]), nan = nan || redi[w];
-    __syncthreads();
-    auto answer = [&](int id, float p) {
-        a.ids[row] = id;
-        if (a.prob) a.prob[row] = p;
-    };
+        for (int j = 0; j < NV; j++) l[j] = first + 64 * j < V ? (float)x[first + 64 * j] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            val[first + 64 * j] = l[j];
+            nan = nan || l[j] != l[j];
+            m = fmaxf(m, l[j]);
+            lo = l[j] > -INFINITY ? fminf(lo, l[j]) : lo;
+        }
+    }
+    const Ask q = ask_of(a, row);
+    reduce_range(s, m, lo, nan);
     if (nan || m == -INFINITY) {
-        if (tid == 0) answer(-1, nan ? __builtin_nanf("") : 0.f);
+        if (tid == 0) out.put(-1, nan ? __builtin_nanf("") : 0.f);
         return;
     }
-    const float temp = a.temp ? a.temp[row] : 1.f;
-    if (!(temp > 0.f)) {
-        int best = V;
-        for (int i = tid; i < V && best == V; i += kThreads)
-            if ((float)x[i] == m) best = i;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) best = min(best, __shfl_xor(best, d));
-        if (lane == 0) redi[wave] = best;
+    if (q.greedy) {                      // the first of the largest
+        int best = INT32_MAX;
+        for (int j = NV - 1; j >= 0; j--) {
+            const uint64_t who = __ballot(val[first + 64 * j] == m);
+            best = who ? (wave * NV + j) * 64 + __builtin_ctzll(who) : best;
+        }
         __syncthreads();
-        for (int w = 0; w < kWaves; w++) best = min(best, redi[w]);
-        if (tid == 0) answer(best, 1.f);
+        if (lane == 0) s.redi[wave] = best;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; w++) best = min(best, s.redi[w]);
+        if (tid == 0) out.put(best, 1.f);
         return;
     }
-    const Weights wt{(double)m, 1.4426950408889634 / (double)temp, a.unit};
-    // kept: keys above t, and the first nt of the tokens at t
-    uint32_t t = 0, nt = V;
-    uint64_t total = 0;
+    const Scale sc(m, lo, q.temp, a.unit);
+    uint64_t last = ~0ull;               // the last place that is kept
+    auto each = [&](int, auto f) {       // this thread's tokens that are left
+#pragma unroll 1
+        for (int j = 0; j < NV; j++) {
+            const int i = first + 64 * j;
+            if (i >= V) break;
+            const float l = val[i];
+            if (place_of(l, i) <= last) f(l, i);
+        }
+    };
+    auto fill = [&](bool masses) {
+        for (int i = tid; i < kBins; i += NT) s.cnt[i] = 0, s.mass[i] = 0;
+        __syncthreads();
+        each(0, [&](float l, int) {
+            const int b = sc.bin(l);
+            atomicAdd(&s.cnt[b], 1u);
+            if (masses) atomicAdd((ull*)&s.mass[b], (ull)sc.mass(l));
+        });
+    };
+    if (q.by_k) {
+        fill(false);
+        last = cut_at(s, sc, true, (uint64_t)q.k, 0., each).place;
+    }
+    if (q.by_p) {
+        fill(true);
+        __syncthreads();
+        uint64_t v = 0;
+        for (int i = tid; i < kBins; i += NT) v += s.mass[i];
+        const uint64_t total = wave_sums<1>(s, &v);
+        last = cut_at(s, sc, false, 0, (double)q.top_p * (double)total, each).place;
+    }
+    uint64_t mass[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = first + 64 * j;
+        const float l = val[i];
+        mass[j] = 0;
+        if (i < V && place_of(l, i) <= last) {
+            const double w = sc.wt.of(l);
+            if (!(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.)) mass[j] = sc.wt.mass(w);
+        }
+        __builtin_amdgcn_sched_barrier(0);               // (one exponential's registers at a time)
+    }
+    const uint64_t all = wave_sums<NV>(s, mass);
+    draw<NV>(s, mass, 0, all, draw_at(q.u, all), 0, out);
+}
 
-    // the key and the number of its tokens where a running count reaches `k`, or a running mass `target`; `total` the mass up to there
-    auto cut = [&](bool by_count, uint64_t k, double target) {
-        uint32_t prefix = 0;
-        uint64_t above_n = 0, above_m = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kThreads) cnt[i] = 0, mass[i] = 0;
+// Long rows: chunks of kChunk tokens. The first launch notes each chunk's range; the second, which knows the row's, its bins
+// (or, where neither k nor p cuts, its kept mass); the third, a workgroup per row, adds the bins up, cuts, finds the chunk
+// in which the draw lies, and draws there.
+constexpr int kChunk = 8192, kMostChunks = (1 << 24) / kChunk;
+struct Long {
+    int chunks, row0;      // chunks of a row; the first row of this launch
+    f32x4* range;          // [rows][chunks] largest, least finite logit, NaN
+    uint64_t* kept;        // [rows][chunks]
+    uint64_t* mass;        // [rows][chunks][kBins]
+    uint32_t* cnt;
+};
+
+// NV logits of a thread of the chunk from id0 on; past the row -infinity
+template <typename T, int NT>
+__device__ __forceinline__ void load_chunk(const T* x, int V, int id0, float* l) {
+    constexpr int NV = kChunk / NT;
+    const int at = id0 + (threadIdx.x >> 6) * NV * 64 + (threadIdx.x & 63);
+    if (id0 + kChunk <= V) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) l[j] = (float)x[at + 64 * j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; j++) l[j] = at + 64 * j < V ? (float)x[at + 64 * j] : -INFINITY;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void k_sample_range(SampleArgs a, Long g) {
+    constexpr int NV = kChunk / 512;
+    __shared__ Lds<0, 512> s;
+    const int64_t row = g.row0 + blockIdx.y;
+    float l[NV], m = -INFINITY, lo = INFINITY;
+    load_chunk<T, 512>((const T*)a.x + row * a.x_stride, a.V, blockIdx.x * kChunk, l);
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        nan = nan || l[j] != l[j];
+        m = fmaxf(m, l[j]);
+        lo = l[j] > -INFINITY ? fminf(lo, l[j]) : lo;
+    }
+    reduce_range(s, m, lo, nan);
+    if (threadIdx.x == 0) g.range[(int64_t)blockIdx.y * g.chunks + blockIdx.x] = f32x4{m, lo, nan ? 1.f : 0.f, 0.f};
+}
+
+template <class L>
+__device__ __forceinline__ void row_range(L& s, const Long& g, float& m, float& lo, bool& nan) {
+    m = -INFINITY, lo = INFINITY, nan = false;
+    for (int c = threadIdx.x; c < g.chunks; c += L::kThreads) {
+        const f32x4 r = g.range[(int64_t)blockIdx.y * g.chunks + c];
+        m = fmaxf(m, r[0]), lo = fminf(lo, r[1]), nan = nan || r[2] != 0.f;
+    }
+    reduce_range(s, m, lo, nan);
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void k_sample_bins(SampleArgs a, Long g) {
+    constexpr int NV = kChunk / 512;
+    __shared__ Lds<0, 512> s;
+    const int tid = threadIdx.x, id0 = blockIdx.x * kChunk;
+    const int64_t row = g.row0 + blockIdx.y, at = (int64_t)blockIdx.y * g.chunks + blockIdx.x;
+    float l[NV], m, lo;
+    bool nan;
+    load_chunk<T, 512>((const T*)a.x + row * a.x_stride, a.V, id0, l);
+    for (int i = tid; i < kBins; i += 512) s.cnt[i] = 0, s.mass[i] = 0;
+    const Ask q = ask_of(a, row);
+    row_range(s, g, m, lo, nan);
+    if (nan || m == -INFINITY || q.greedy) return;
+    const Scale sc(m, lo, q.temp, a.unit);
+    const int first = id0 + (tid >> 6) * NV * 64 + (tid & 63);
+    if (q.by_k || q.by_p) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (first + 64 * j >= a.V) continue;
+            const int b = sc.bin(l[j]);
+            atomicAdd(&s.cnt[b], 1u);
+            atomicAdd((ull*)&s.mass[b], (ull)sc.mass(l[j]));
+        }
+        __syncthreads();
+        for (int i = tid; i < kBins; i += 512) g.cnt[at * kBins + i] = s.cnt[i], g.mass[at * kBins + i] = s.mass[i];
+        return;
+    }
+    uint64_t mass[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const double w = sc.wt.of(l[j]);
+        mass[j] = !(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.) ? sc.wt.mass(w) : 0;
+    }
+    const uint64_t all = wave_sums<NV>(s, mass);
+    if (tid == 0) g.kept[at] = all;
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
+    constexpr int NT = 1024, NV = kChunk / NT;
+    __shared__ Lds<2048, NT> s;
+    __shared__ uint64_t kept[kMostChunks];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.V;
+    const int64_t row = g.row0 + blockIdx.y, at0 = (int64_t)blockIdx.y * g.chunks;
+    const T* x = (const T*)a.x + row * a.x_stride;
+    const Answer out{a.ids + row, a.prob ? a.prob + row : nullptr};
+    float m, lo;
+    bool nan;
+    const Ask q = ask_of(a, row);
+    row_range(s, g, m, lo, nan);
+    if (nan || m == -INFINITY) {
+        if (tid == 0) out.put(-1, nan ? __builtin_nanf("") : 0.f);
+        return;
+    }
+    float l[NV];
+    const int first = wave * NV * 64 + lane;
+    if (q.greedy) {
+        auto least = [&](int v) {
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d));
             __syncthreads();
-            for (int i = tid; i < V; i += kThreads) {
-                const float l = (float)x[i];
-                const uint32_t key = key_of(l);
-                if (shift < 24 && key >> (shift + 8) != prefix) continue;
-                atomicAdd(&cnt[key >> shift & 255], 1u);
-                atomicAdd((unsigned long long*)&mass[key >> shift & 255], (unsigned long long)wt.mass(wt.of(l)));
-            }
+            if (lane == 0) s.redi[wave] = v;
             __syncthreads();
-            if (wave == 0) {                             // four bins of a lane, highest first
-                uint64_t n4 = 0, m4 = 0;
-                for (int j = 0; j < 4; j++) n4 += cnt[255 - 4 * lane - j], m4 += mass[255 - 4 * lane - j];
-                uint64_t n = above_n + scan64(n4, lane) - n4, s = above_m + scan64(m4, lane) - m4;
-                const bool here = by_count ? n + n4 >= k : (double)(s + m4) >= target && n4;
-                const uint64_t who = __ballot(here);
-                // (a target that rounding puts past the whole mass: the last bin that holds something)
-                const uint64_t held = __ballot(n4 != 0);
-                const int l0 = who ? __builtin_ctzll(who) : 63 - __builtin_clzll(held);
-                if (lane == l0) {
-                    int bin = -1;
-                    for (int j = 0; j < 4; j++) {
-                        const int q = 255 - 4 * lane - j;
-                        if (!cnt[q]) continue;
-                        if (bin >= 0) n += cnt[bin], s += mass[bin];
-                        bin = q;
-                        if (by_count ? n + cnt[q] >= k : (double)(s + mass[q]) >= target) break;
-                    }
-                    picked[0] = n, picked[1] = s, picked[2] = (uint64_t)bin, picked[3] = (uint64_t)cnt[bin];
+            for (int w = 0; w < NT / 64; w++) v = min(v, s.redi[w]);
+            return v;
+        };
+        int best = INT32_MAX;
+        for (int c = tid; c < g.chunks; c += NT)
+            if (g.range[at0 + c][0] == m) best = min(best, c);
+        const int id0 = least(best) * kChunk;
+        load_chunk<T, NT>(x, V, id0, l);
+        best = INT32_MAX;
+#pragma unroll
+        for (int j = NV - 1; j >= 0; j--)
+            if (l[j] == m) best = id0 + first + 64 * j;
+        best = least(best);
+        if (tid == 0) out.put(best, 1.f);
+        return;
+    }
+    const Scale sc(m, lo, q.temp, a.unit);
+    uint64_t last = ~0ull;
+    if (q.min_p > 0.f) last = (uint64_t)~least_key(sc.wt, fmin((double)q.min_p, 1.)) << 32 | 0xffffffffull;
+    if (q.by_k || q.by_p) {
+        auto fill = [&] {                // the row's bins: two halves of the chunks
+            const int b = tid & (kBins - 1), half = tid / kBins;
+            uint32_t n = 0;
+            uint64_t w = 0;
+#pragma unroll 4
+            for (int c = half; c < g.chunks; c += NT / kBins) n += g.cnt[(at0 + c) * kBins + b], w += g.mass[(at0 + c) * kBins + b];
+            __syncthreads();
+            if (half) s.cnt[b] = n, s.mass[b] = w;
+            __syncthreads();
+            if (!half) s.cnt[b] += n, s.mass[b] += w;
+            __syncthreads();
+        };
+        auto each = [&](int bin, auto f) {
+            for (int c0 = 0; c0 < g.chunks; c0 += 64) {  // (chunks that have some: asked for 64 at a time)
+                uint64_t some = __ballot(c0 + lane < g.chunks && g.cnt[(at0 + min(c0 + lane, g.chunks - 1)) * kBins + bin] != 0);
+                for (; some; some &= some - 1) {
+                    const int id0 = (c0 + __builtin_ctzll(some)) * kChunk;
+                    float y[NV];
+                    load_chunk<T, NT>(x, V, id0, y);
+#pragma unroll
+                    for (int j = 0; j < NV; j++)
+                        if (id0 + first + 64 * j < V) f(y[j], id0 + first + 64 * j);
                 }
             }
-            __syncthreads();
-            above_n = picked[0], above_m = picked[1];
-            prefix = prefix << 8 | (uint32_t)picked[2];
+        };
+        fill();
+        Cut c{~0ull, 0, -1, true, 0};
+        uint64_t total = 0;
+        if (q.by_k) {
+            c = cut_at(s, sc, true, (uint64_t)q.k, 0., each);
+            last = c.place < last ? c.place : last;
+            total = c.mass;
+            if (q.by_p && !c.intact) fill();
         }
-        const uint64_t held = picked[3], each = wt.mass(wt.of(logit_of(prefix)));
-        uint64_t n = 0;
-        if (by_count) {
-            n = k - above_n;
-        } else {                                         // tokens at the key whose running sum before them is below the target
-            const double left = target - (double)above_m;
-            n = left <= 0. ? 0 : each ? (uint64_t)(left / (double)each) : held;
-            while (n > 0 && (double)(above_m + (n - 1) * each) >= target) n--;
-            while (n < held && (double)(above_m + n * each) < target) n++;
+        if (q.by_p) {
+            if (!q.by_k) {
+                const uint64_t v = tid < kBins ? s.mass[tid] : 0;
+                total = wave_sums<1>(s, &v);
+            }
+            c = cut_at(s, sc, false, 0, (double)q.top_p * (double)total, each);
+            last = c.place < last ? c.place : last;
         }
-        t = prefix;
-        nt = (uint32_t)(n < 1 ? 1 : n > held ? held : n);
-        total = above_m + nt * each;
+        // each chunk's kept mass: bins before the last place's, and what is kept of that one
+        const int bin = sc.bin(logit_of(~(uint32_t)(last >> 32)));
+        for (int k = wave; k < g.chunks; k += NT / 64) {
+            uint64_t v = 0;
+#pragma unroll
+            for (int i = 0; i < kBins / 64; i++) {
+                const int b = 64 * i + lane;
+                const uint64_t w = g.mass[(at0 + k) * kBins + b];
+                v += b < bin ? w : 0;
+            }
+            v = sum64(v);
+            if (lane == 0) kept[k] = v;
+        }
         __syncthreads();
-    };
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
-    bool have = false;
-    if (k > 0 && k < V) cut(true, (uint64_t)k, 0.), have = true;
-    if (top_p < 1.f) {
-        if (!have) {
-            uint64_t s = 0;
-            for (int i = tid; i < V; i += kThreads) s += wt.mass(wt.of((float)x[i]));
-            s = scan64(s, lane);
-            if (lane == 63) seg[wave] = s;
-            __syncthreads();
-            for (int w = 0; w < kWaves; w++) total += seg[w];
-            __syncthreads();
+        auto add = [&](uint64_t p, uint64_t w) {
+            if (p <= last) atomicAdd((ull*)&kept[(uint32_t)p / kChunk], (ull)w);
+        };
+        if (c.bin == bin) {
+            const uint32_t n = c.held;
+            for (uint32_t i = tid; i < n; i += NT) add(s.place[i], s.w[i]);
+        } else {
+            each(bin, [&](float y, int i) {
+                if (sc.bin(y) == bin) add(place_of(y, i), sc.mass(y));
+            });
         }
-        cut(false, 0, (double)top_p * (double)total);
+    } else {
+        for (int c = tid; c < g.chunks; c += NT) kept[c] = g.kept[at0 + c];
     }
-    // the draw: each wave a run of the row
-    const int len = ((V + kWaves - 1) / kWaves + 63) & ~63, lo = min(wave * len, V), hi = min(lo + len, V);
-    uint32_t n = 0;
-    for (int i = lo; i < hi; i += 64) n += __popcll(__ballot(i + lane < hi && key_of((float)x[min(i + lane, V - 1)]) == t));
-    if (lane == 0) ties[wave] = n;
     __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < wave; w++) before += ties[w];
-    // mass of the token i + lane, 0 where it is not kept
-    auto kept = [&](int i, uint32_t& rank) {
-        const float l = i + lane < hi ? (float)x[i + lane] : -INFINITY;
-        const uint32_t key = key_of(l);
-        const uint64_t same = __ballot(i + lane < hi && key == t);
-        const uint32_t r = rank + __popcll(same & ((1ull << lane) - 1));
-        rank += __popcll(same);
-        const double w = wt.of(l);
-        return i + lane < hi && (key > t || (key == t && r < nt)) && (!(min_p > 0.f) || w >= fmin((double)min_p, 1.)) ? wt.mass(w) : 0;
-    };
-    uint32_t rank = before;
-    uint64_t s = 0;
-    for (int i = lo; i < hi; i += 64) s += kept(i, rank);
-    s = scan64(s, lane);
-    if (lane == 63) seg[wave] = s;
-    __syncthreads();
-    uint64_t all = 0, ahead = 0, mine = seg[wave];
-    for (int w = 0; w < kWaves; w++) all += seg[w], ahead += w < wave ? seg[w] : 0;
-    const float u = a.u[row];
-    // (past every sum, where u is 1 or more: the last kept token)
-    const double most = (double)all * (u > 0.f ? (double)u : 0.);
-    uint64_t at = (uint64_t)fmin(most, (double)all);
-    at = at < all ? at : all - 1;                        // a token's running sum must exceed it
-    if (at < ahead || at >= ahead + mine) return;
-    rank = before;
-    for (int i = lo; i < hi; i += 64) {
-        const uint64_t w = kept(i, rank), sum = ahead + scan64(w, lane);
-        const uint64_t who = __ballot(sum > at);
-        if (who) {
-            if (lane == __builtin_ctzll(who)) answer(i + lane, (float)((double)w / (double)all));
-            return;
+    uint64_t all = 0;
+    for (int c = tid; c < g.chunks; c += NT) all += kept[c];
+    all = wave_sums<1>(s, &all);
+    const uint64_t at = draw_at(q.u, all);
+    if (wave == 0) {
+        uint64_t ahead = 0;
+        for (int c0 = 0; c0 < g.chunks; c0 += 64) {
+            const uint64_t run = ahead + scan64(c0 + lane < g.chunks ? kept[c0 + lane] : 0);
+            const uint64_t who = __ballot(run > at);
+            if (who) {
+                const int w = __builtin_ctzll(who);
+                if (lane == w) s.found[0] = (uint64_t)(c0 + lane), s.found[1] = run - kept[c0 + lane];
+                break;
+            }
+            ahead = lane64(run, 63);
         }
-        ahead = shfl64(sum, 63);
+    }
+    __syncthreads();
+    const int id0 = (int)s.found[0] * kChunk;
+    const uint64_t ahead = s.found[1];
+    load_chunk<T, NT>(x, V, id0, l);
+    uint64_t mass[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = id0 + first + 64 * j;
+        mass[j] = i < V && place_of(l[j], i) <= last ? sc.mass(l[j]) : 0;
+    }
+    wave_sums<NV>(s, mass);
+    draw<NV>(s, mass, ahead, all, at, id0, out);
+}
+
+template <typename T>
+void launch_short(const SampleArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)a.rows);
+    if (a.V <= 2048) hipLaunchKernelGGL((k_sample<T, 256, 8>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_sample<T, 1024, 8>), grid, dim3(1024), 0, s, a);
+}
+
+constexpr size_t kRowBytes = sizeof(f32x4) + sizeof(uint64_t) + kBins * (sizeof(uint64_t) + sizeof(uint32_t));   // of a chunk
+
+template <typename T>
+void launch_long(const SampleArgs& a, const SamplePlan& p, hipStream_t s) {
+    for (int r0 = 0; r0 < a.rows; r0 += p.batch) {
+        const size_t n = (size_t)std::min(p.batch, a.rows - r0) * p.chunks;
+        Long g{p.chunks, r0, (f32x4*)a.ws, nullptr, nullptr, nullptr};
+        g.kept = (uint64_t*)(g.range + n);
+        g.mass = g.kept + n;
+        g.cnt = (uint32_t*)(g.mass + n * kBins);
+        const unsigned rows = (unsigned)std::min(p.batch, a.rows - r0);
+        hipLaunchKernelGGL(k_sample_range<T>, dim3((unsigned)p.chunks, rows), dim3(512), 0, s, a, g);
+        hipLaunchKernelGGL(k_sample_bins<T>, dim3((unsigned)p.chunks, rows), dim3(512), 0, s, a, g);
+        hipLaunchKernelGGL(k_sample_pick<T>, dim3(1, rows), dim3(1024), 0, s, a, g);
     }
 }
 
@@ -254,10 +703,22 @@ double sample_unit(int V) {
     return (double)(1ull << s);
 }
 
-hipError_t launch_sample(const SampleArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)a.rows);
-    if (a.f16) hipLaunchKernelGGL(k_sample<_Float16>, grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL(k_sample<float>, grid, dim3(kThreads), 0, s, a);
+// A row in one workgroup up to 8192 tokens; longer ones in chunks, as many rows at a time as 64 MB of bins hold
+SamplePlan sample_plan(const SampleArgs& a) {
+    SamplePlan p{};
+    if (a.V <= kChunk) return p;
+    p.chunks = (a.V + kChunk - 1) / kChunk;
+    const size_t per = kRowBytes * p.chunks;
+    p.batch = (int)std::min<size_t>({(size_t)a.rows, std::max<size_t>(1, ((size_t)64 << 20) / per), 65535});
+    p.ws_bytes = per * p.batch;
+    return p;
+}
+
+hipError_t launch_sample(const SampleArgs& a, const SamplePlan& p, hipStream_t s) {
+    if (p.chunks && a.f16) launch_long<_Float16>(a, p, s);
+    else if (p.chunks) launch_long<float>(a, p, s);
+    else if (a.f16) launch_short<_Float16>(a, s);
+    else launch_short<float>(a, s);
     return hipGetLastError();
 }
 

@@ -1284,6 +1284,18 @@ int row_granule(const void* p, const int64_t st[4], bool f16) {
     return 1;
 }
 
+// an angle in radians as a whole number of 2^-64 turns, whole turns left out, |w| <= 16: its 53 bits times 2^128 / 2 pi
+// (floor), 64 of the product's bits and one to round by
+uint64_t turns(double w) {
+    int e = 0;
+    const uint64_t m = (uint64_t)std::ldexp(std::frexp(std::fabs(w), &e), 53);       // |w| = m 2^(e - 53), e <= 5
+    typedef unsigned __int128 u128;
+    const u128 p = (u128)m * 0x28be60db9391054aull + ((u128)m * 0x7f09d5f47d4d3770ull >> 64);   // m 2^64 / 2 pi
+    const int s = 53 - e;
+    const uint64_t f = s > 127 ? 0 : (uint64_t)((p + ((u128)1 << (s - 1))) >> s);
+    return w < 0 ? 0 - f : f;
+}
+
 int check_rotation(mgh_ctx* c, const char* fn, const mgh_rotation* rot, int D, mgh::Rotation* out) {
     const std::string f(fn);
     if (!rot) return fail(c, MGH_ERR_ARG, f + ": null rotation");
@@ -1307,11 +1319,7 @@ int check_rotation(mgh_ctx* c, const char* fn, const mgh_rotation* rot, int D, m
     for (int i = 0; i < r.P; i++) {
         const double w = rot->h_freqs[i];
         if (!(std::fabs(w) <= 16.)) return fail(c, MGH_ERR_ARG, f + ": frequencies must be finite and at most 16");
-        // whole numbers of 2^-64 turns, whole turns left out (64-bit significands: off by less than one)
-        long double t = (long double)w * 0.159154943091895335768883763372514362L;
-        t = ldexpl(t - floorl(t), 64);
-        t = nearbyintl(t);
-        r.turn[i] = t >= 18446744073709551616.0L ? 0 : (uint64_t)t;
+        r.turn[i] = turns(w);
     }
     r.pos = rot->d_pos;
     for (int i = 0; i < 3; i++) r.pst[i] = rot->pos_strides[i];
@@ -1470,8 +1478,8 @@ int mgh_rope(mgh_ctx* c, const mgh_rotation* rot, const void* x, int in_f16, con
     if (in_f16 != 0 && in_f16 != 1) return fail(c, MGH_ERR_ARG, "rope: in_f16 must be 0 or 1");
     if ((y != nullptr) == (y16 != nullptr)) return fail(c, MGH_ERR_ARG, "rope: exactly one of d_y and d_y16 is needed");
     if (S == 0 || H == 0 || B == 0) return MGH_OK;
-    if (S > (1 << 28) || H > 65535 || B > 65535 || (int64_t)S * H * D > ((int64_t)1 << 33))
-        return fail(c, MGH_ERR_UNSUPPORTED, "rope: at most 2^28 tokens, 65535 heads and sequences, 2^33 values of a sequence");
+    if (S > (1 << 28) || H > 65535 || B > 65535 || (int64_t)S * H * D > ((int64_t)1 << 31))
+        return fail(c, MGH_ERR_UNSUPPORTED, "rope: at most 2^28 tokens, 65535 heads and sequences, 2^31 values of a sequence");
     if (!x || !xst || !yst) return fail(c, MGH_ERR_ARG, "rope: null pointer");
     if (!aligned_to(x, in_f16 ? 2 : 4) || !aligned_to(y, 4) || !aligned_to(y16, 2) || !aligned_to(first, 4) || !aligned_to(fresh, 4))
         return fail(c, MGH_ERR_ARG, "rope: pointers must be aligned to their elements");
@@ -1509,8 +1517,8 @@ int mgh_kv8_append_rope(mgh_ctx* c, const mgh_kv8* kv, const mgh_rotation* rot, 
     if (q) {
         if (H <= 0 || H % kv->Hkv) return fail(c, MGH_ERR_ARG, "kv8_append_rope: need H > 0 and H % Hkv == 0");
         if (!q_out || !qst || !qost) return fail(c, MGH_ERR_ARG, "kv8_append_rope: null pointer");
-        if (H > 65535 || (int64_t)S * (H / kv->Hkv) * kv->D > ((int64_t)1 << 32))
-            return fail(c, MGH_ERR_UNSUPPORTED, "kv8_append_rope: at most 65535 heads and 2^32 values of a key head's queries");
+        if (H > 65535 || (int64_t)S * (H / kv->Hkv) * kv->D > ((int64_t)1 << 31))
+            return fail(c, MGH_ERR_UNSUPPORTED, "kv8_append_rope: at most 65535 heads and 2^31 values of a key head's queries");
         bool same = in_f16 != 0;
         for (int i = 0; i < 4; i++) a.qst[i] = qst[i], a.qost[i] = qost[i], same = same && qst[i] == qost[i];
         if (q == q_out && !same) return fail(c, MGH_ERR_ARG, "kv8_append_rope: in place needs the same type and strides");
@@ -1657,8 +1665,13 @@ int mgh_sample(mgh_ctx* c, const void* x, int f16, int64_t xs, int rows, int V, 
     a.x = x; a.x_stride = xs; a.rows = rows; a.V = V; a.f16 = f16 != 0;
     a.temp = op.d_temp; a.top_k = op.d_top_k; a.top_p = op.d_top_p; a.min_p = op.d_min_p;
     a.u = u; a.ids = ids; a.prob = prob; a.unit = mgh::sample_unit(V);
+    const mgh::SamplePlan plan = mgh::sample_plan(a);
     if (int r = set_dev(c)) return r;
-    MGH_HIP(c, mgh::launch_sample(a, c->stream), "k_sample");
+    if (plan.ws_bytes) {
+        if (int r = ensure_qp_ws(c, plan.ws_bytes)) return r;
+        a.ws = c->qp_ws;
+    }
+    MGH_HIP(c, mgh::launch_sample(a, plan, c->stream), "k_sample");
     return MGH_OK;
 }
 

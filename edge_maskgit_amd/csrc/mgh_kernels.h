@@ -490,9 +490,15 @@ struct SampleArgs {
     int32_t* ids;
     float* prob;               // or null
     double unit;               // masses are counted in 1 / unit of the largest weight
+    void* ws;                  // SamplePlan::ws_bytes
+};
+struct SamplePlan {
+    int chunks, batch;         // of long rows (0: none), rows of them at a time
+    size_t ws_bytes;
 };
 double sample_unit(int V);
-hipError_t launch_sample(const SampleArgs& a, hipStream_t s);
+SamplePlan sample_plan(const SampleArgs& a);
+hipError_t launch_sample(const SampleArgs& a, const SamplePlan& p, hipStream_t s);
 
 size_t noalloc_scratch_bytes();
 hipError_t noalloc_scratch(int device, void** out);

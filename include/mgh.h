@@ -442,7 +442,7 @@ typedef struct mgh_rotation {
 /* x and y: {D, S, H, B} views with element strides (d, token, head, sequence); y fp32 (d_y) or fp16 (d_y16), exactly one
  * of them; y may be x where type and strides are the same, else they do not overlap. Sequence b's token 0 stands at
  * d_first[b] (NULL: 0) where the rotation has no positions. d_new [B]: tokens of each sequence, 0 .. S (NULL: S each);
- * rows past them, and all rows of a sequence whose number does not fit, are neither read nor written. S D H up to 2^33. */
+ * rows past them, and all rows of a sequence whose number does not fit, are neither read nor written. S D H up to 2^31. */
 int mgh_rope(mgh_ctx* ctx, const mgh_rotation* rot, const void* d_x, int in_f16, const int64_t x_strides[4], int D, int S,
              int H, int B, const int32_t* d_first, const int32_t* d_new, float* d_y, void* d_y16, const int64_t y_strides[4]);
 

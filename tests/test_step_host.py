@@ -38,7 +38,7 @@ for kw, what in (({"D": 15}, "even"), ({"D": 130}, "even"), ({"D": 0}, "even"), 
                  ({"y": None}, "exactly one"), ({"y16": G}, "exactly one"), ({"x": None}, "null"), ({"x": W + 1}, "aligned"), ({"x": W + 2, "in16": False}, "aligned"),
                  ({"y": Y + 2}, "aligned"), ({"y": None, "y16": Y + 1}, "aligned"), ({"first": R + 1}, "aligned"), ({"new": R + 2}, "aligned"),
                  ({"y": W}, "in place"), ({"y": W, "in16": False, "y_strides": (1, 64, 16, 64 * 10)}, "in place"), ({"Bn": 65536}, "at most"), ({"H": 65536}, "at most"),
-                 ({"S": 2 ** 28 + 1}, "at most"), ({"S": 2 ** 28, "H": 3}, "at most")):
+                 ({"S": 2 ** 28 + 1}, "at most"), ({"S": 2 ** 25 + 1}, "at most")):
     refused(call, what=what, **kw)
 L = ema.lib()
 four = (ctypes.c_int64 * 4)(*st)
