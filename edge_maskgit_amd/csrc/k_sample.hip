@@ -30,24 +30,16 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 2^t, t <= 0, off by 2^-51 of it and 2^-53 |t|: the nearest whole number's power and the series of the rest, |f| <= 1/2
+// 2^t, t <= 0, off by 2^-51 of it and 2^-53 |t|: the nearest whole number's power and the series of the rest, |f| <= 1/2, by
+// pairs of terms (Horner's rule is a chain of 13 dependent steps: a row of 2025 tokens 16.5 us with it)
 __device__ __forceinline__ double exp2_64(double t) {
-    if (t < -1000.) return 0.;
-    const double n = rint(t), f = t - n;
-    double p = 2.5678435993488206e-11;
-    p = fma(p, f, 4.44553827187081e-10);
-    p = fma(p, f, 7.054911620801121e-09);
-    p = fma(p, f, 1.0178086009239696e-07);
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 0.00015403530393381606);
-    p = fma(p, f, 0.0013333558146428441);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.055504108664821576);
-    p = fma(p, f, 0.2402265069591007);
-    p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.);
-    return ldexp(p, (int)n);
+    const double n = rint(fmax(t, -1100.)), f = t - n, f2 = f * f, f4 = f2 * f2;
+    const double p0 = fma(0.6931471805599453, f, 1.), p1 = fma(0.055504108664821576, f, 0.2402265069591007);
+    const double p2 = fma(0.0013333558146428441, f, 0.009618129107628477), p3 = fma(1.5252733804059838e-05, f, 0.00015403530393381606);
+    const double p4 = fma(1.0178086009239696e-07, f, 1.3215486790144305e-06), p5 = fma(4.44553827187081e-10, f, 7.054911620801121e-09);
+    const double q0 = fma(p1, f2, p0), q1 = fma(p3, f2, p2), q2 = fma(fma(2.5678435993488206e-11, f2, p5), f2, p4);
+    const double p = fma(fma(q2, f4, q1), f4, q0);
+    return t < -1000. ? 0. : ldexp(p, (int)n);
 }
 
 struct Weights {
@@ -55,9 +47,9 @@ struct Weights {
     double unit;           // 2^S
     // weight of a logit relative to the largest one's
     __device__ __forceinline__ double of(float l) const {
-        if ((double)l == m) return 1.;                   // (infinities among themselves)
-        if (l == -INFINITY || m == INFINITY) return 0.;  // (whatever T is)
-        return exp2_64(((double)l - m) * c);
+        const double w = exp2_64(((double)l - m) * c);
+        // (whatever T is; infinities among themselves)
+        return (double)l == m ? 1. : l == -INFINITY || m == INFINITY ? 0. : w;
     }
     __device__ __forceinline__ uint64_t mass(double w) const {
         return __builtin_bit_cast(uint64_t, fma(w, unit, 4503599627370496.)) & 0xfffffffffffffull;
@@ -386,12 +378,11 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a) {
     const Scale sc(m, lo, q.temp, a.unit);
     uint64_t last = ~0ull;               // the last place that is kept
     auto each = [&](int, auto f) {       // this thread's tokens that are left
-#pragma unroll 1
+#pragma unroll (NT == 256 ? NV : 2)
         for (int j = 0; j < NV; j++) {
             const int i = first + 64 * j;
-            if (i >= V) break;
             const float l = val[i];
-            if (place_of(l, i) <= last) f(l, i);
+            if (i < V && place_of(l, i) <= last) f(l, i);
         }
     };
     auto fill = [&](bool masses) {
@@ -416,16 +407,25 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a) {
         last = cut_at(s, sc, false, 0, (double)q.top_p * (double)total, each).place;
     }
     uint64_t mass[NV];
+    constexpr int U = NT == 256 ? 4 : 2;                 // exponentials beside one another
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int i = first + 64 * j;
-        const float l = val[i];
-        mass[j] = 0;
-        if (i < V && place_of(l, i) <= last) {
-            const double w = sc.wt.of(l);
-            if (!(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.)) mass[j] = sc.wt.mass(w);
+    for (int j0 = 0; j0 < NV; j0 += U) {
+        float l[U];
+        bool keep[U], some = false;
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int i = first + 64 * (j0 + j);
+            l[j] = val[i];
+            keep[j] = i < V && place_of(l[j], i) <= last;
+            some = some || keep[j];
+            mass[j0 + j] = 0;
         }
-        __builtin_amdgcn_sched_barrier(0);               // (one exponential's registers at a time)
+        if (!__any(some)) continue;
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const double w = sc.wt.of(l[j]);
+            mass[j0 + j] = keep[j] && (!(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.)) ? sc.wt.mass(w) : 0;
+        }
     }
     const uint64_t all = wave_sums<NV>(s, mass);
     draw<NV>(s, mass, 0, all, draw_at(q.u, all), 0, out);
@@ -583,10 +583,15 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
         auto each = [&](int bin, auto f) {
             for (int c0 = 0; c0 < g.chunks; c0 += 64) {  // (chunks that have some: asked for 64 at a time)
                 uint64_t some = __ballot(c0 + lane < g.chunks && g.cnt[(at0 + min(c0 + lane, g.chunks - 1)) * kBins + bin] != 0);
+                float next[NV];                          // the next one's logits on their way while one is looked at
+                auto id_of = [&](uint64_t set) { return (c0 + __builtin_ctzll(set)) * kChunk; };
+                if (some) load_chunk<T, NT>(x, V, id_of(some), next);
                 for (; some; some &= some - 1) {
-                    const int id0 = (c0 + __builtin_ctzll(some)) * kChunk;
+                    const int id0 = id_of(some);
                     float y[NV];
-                    load_chunk<T, NT>(x, V, id0, y);
+#pragma unroll
+                    for (int j = 0; j < NV; j++) y[j] = next[j];
+                    if (some & (some - 1)) load_chunk<T, NT>(x, V, id_of(some & (some - 1)), next);
 #pragma unroll
                     for (int j = 0; j < NV; j++)
                         if (id0 + first + 64 * j < V) f(y[j], id0 + first + 64 * j);
