@@ -111,23 +111,42 @@ __device__ __forceinline__ Ask ask_of(const SampleArgs& a, int64_t row) {
     return q;
 }
 
-// weights and bins of a row whose logits lie between lo (the least that is finite) and m
+// weights and bins of a row whose logits lie between lo (the least that is finite) and m: bins of equal parts of that span,
+// or of the 64 octaves below m where it is wider. fp32: all that a bin needs is that a larger logit's is no later
 struct Scale {
     Weights wt;
-    double cs;             // bins per unit of logit
-    __device__ __forceinline__ Scale(float m, float lo, float temp, double unit) {
-        wt = Weights{(double)m, 1.4426950408889634 / (double)temp, unit};
-        const double span = ((double)m - (double)lo) * wt.c, r = span < 64. ? span : 64.;
-        cs = span > 0. ? wt.c * ((kBins - 1) / r) : 0.;
+    float m, cs;           // largest logit, bins per unit of logit
+    __device__ __forceinline__ Scale(float most, float lo, float temp, double unit) {
+        wt = Weights{(double)most, 1.4426950408889634 / (double)temp, unit};
+        m = most;
+        const double span = (double)most - (double)lo, octaves = 64. / wt.c;
+        cs = span > 0. ? (float)((kBins - 1) / (span < octaves ? span : octaves)) : 0.f;
     }
     __device__ __forceinline__ int bin(float l) const {
-        const double x = (wt.m - (double)l) * cs;
-        return (double)l == wt.m ? 0 : x < kBins - 1 ? (int)x : kBins - 1;
+        const float x = (m - l) * cs;
+        return l == m ? 0 : x < (float)(kBins - 1) ? (int)x : kBins - 1;
     }
     __device__ __forceinline__ uint64_t mass(float l) const { return wt.mass(wt.of(l)); }
 };
 __device__ __forceinline__ uint64_t place_of(float l, int i) { return (uint64_t)(~key_of(l)) << 32 | (uint32_t)i; }
 
+// The least key of a logit that is no NaN for which ok holds, as it does from there up to `hi`: 64 candidates at a time, by every
+// wave for itself
+template <class F>
+__device__ __forceinline__ uint32_t least_key(uint32_t hi, F ok) {
+    const int lane = threadIdx.x & 63;
+    uint32_t lo = 0;
+    while (lo < hi) {                    // the key is in lo .. hi
+        const uint32_t step = (hi - lo) / 64 + 1, off = step * lane;
+        const uint32_t x = off < hi - lo ? lo + off : hi;
+        const float l = logit_of(x);
+        const uint64_t some = __ballot(l == l && ok(l));              // (keys below -infinity's are NaN)
+        const int first = some ? __builtin_ctzll(some) : 64;
+        if (first < 64) hi = (uint32_t)__builtin_amdgcn_readlane((int)x, first);
+        if (first > 0) lo = (uint32_t)__builtin_amdgcn_readlane((int)x, first - 1) + 1;
+    }
+    return hi;
+}
 // Where a running count or mass, over the bins in order, reaches `k` or `target`: found = count and mass before the bin, its
 // number, its count. By wave 0; the others wait.
 template <class L>
@@ -253,22 +272,6 @@ __device__ __forceinline__ Cut cut_at(L& s, const Scale& sc, bool by_count, uint
     const Cut c{s.found[0], s.found[1], listed ? bin : -1, intact, all};
     __syncthreads();
     return c;
-}
-
-// The least key whose weight is at least p (at most 1): 64 candidates at a time, by every wave for itself
-__device__ __forceinline__ uint32_t least_key(const Weights& wt, double p) {
-    const int lane = threadIdx.x & 63;
-    uint32_t lo = 0, hi = key_of((float)wt.m);
-    while (lo < hi) {                    // the key is in lo .. hi, and hi weighs enough
-        const uint32_t step = (hi - lo) / 64 + 1, off = step * lane;
-        const uint32_t x = off < hi - lo ? lo + off : hi;
-        const float l = logit_of(x);
-        const uint64_t ok = __ballot(l == l && wt.of(l) >= p);        // (keys below -infinity's are NaN)
-        const int first = ok ? __builtin_ctzll(ok) : 64;
-        if (first < 64) hi = (uint32_t)__builtin_amdgcn_readlane((int)x, first);
-        if (first > 0) lo = (uint32_t)__builtin_amdgcn_readlane((int)x, first - 1) + 1;
-    }
-    return hi;
 }
 
 // largest, least finite logit and whether there is a NaN, of a workgroup
@@ -431,16 +434,18 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a) {
     draw<NV>(s, mass, 0, all, draw_at(q.u, all), 0, out);
 }
 
-// Long rows: chunks of kChunk tokens. The first launch notes each chunk's range; the second, which knows the row's, its bins
-// (or, where neither k nor p cuts, its kept mass); the third, a workgroup per row, adds the bins up, cuts, finds the chunk
-// in which the draw lies, and draws there.
+// Long rows: chunks of kChunk tokens. The first launch notes each chunk's range; the second, which knows the row's, its bins and
+// its ids in the order of the bins (or, where neither k nor p cuts, its kept mass); the third, a workgroup per row, adds
+// the bins up, cuts (a bin's tokens by their ids: reading the row again took 28 us of a cut in its bulk), finds the chunk in
+// which the draw lies, and draws there.
 constexpr int kChunk = 8192, kMostChunks = (1 << 24) / kChunk;
 struct Long {
     int chunks, row0;      // chunks of a row; the first row of this launch
     f32x4* range;          // [rows][chunks] largest, least finite logit, NaN
     uint64_t* kept;        // [rows][chunks]
     uint64_t* mass;        // [rows][chunks][kBins]
-    uint32_t* cnt;
+    uint32_t* cnt;         // 16 bits: where a bin's ids begin, 16 bits: their number
+    uint16_t* ids;         // [rows][chunks][kChunk] within the chunk
 };
 
 // NV logits of a thread of the chunk from id0 on; past the row -infinity
@@ -486,9 +491,10 @@ __device__ __forceinline__ void row_range(L& s, const Long& g, float& m, float& 
 }
 
 template <typename T>
-__global__ __launch_bounds__(512) void k_sample_bins(SampleArgs a, Long g) {
+__global__ __launch_bounds__(512, 6) void k_sample_bins(SampleArgs a, Long g) {
     constexpr int NV = kChunk / 512;
     __shared__ Lds<0, 512> s;
+    __shared__ __attribute__((aligned(16))) uint16_t ids[kChunk];
     const int tid = threadIdx.x, id0 = blockIdx.x * kChunk;
     const int64_t row = g.row0 + blockIdx.y, at = (int64_t)blockIdx.y * g.chunks + blockIdx.x;
     float l[NV], m, lo;
@@ -501,15 +507,42 @@ __global__ __launch_bounds__(512) void k_sample_bins(SampleArgs a, Long g) {
     const Scale sc(m, lo, q.temp, a.unit);
     const int first = id0 + (tid >> 6) * NV * 64 + (tid & 63);
     if (q.by_k || q.by_p) {
+        uint32_t bin[NV];                // and the number of the token among its bin's; past the row: none
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            if (first + 64 * j >= a.V) continue;
-            const int b = sc.bin(l[j]);
-            atomicAdd(&s.cnt[b], 1u);
-            atomicAdd((ull*)&s.mass[b], (ull)sc.mass(l[j]));
+            bin[j] = first + 64 * j < a.V ? sc.bin(l[j]) : kBins;
+            if (bin[j] < kBins) bin[j] |= atomicAdd(&s.cnt[bin[j]], 1u) << 16;
+        }
+        uint32_t most = kBins - 1;
+        if (q.by_k && q.k < kChunk) {    // what the first k of the row cannot hold is left out: all but the chunk's own first k
+            find_bin(s, true, (uint64_t)q.k, 0., 0, 0);
+            most = (uint32_t)s.found[2];
+        } else {
+            __syncthreads();
+        }
+        if (tid < 64) {                  // where each bin's ids begin
+            constexpr int E = kBins / 64;
+            uint32_t c[E], n = 0;
+#pragma unroll
+            for (int j = 0; j < E; j++) c[j] = s.cnt[E * tid + j], n += c[j];
+            uint32_t o = (uint32_t)scan64(n) - n;
+#pragma unroll
+            for (int j = 0; j < E; j++) s.cnt[E * tid + j] = o << 16 | c[j], o += c[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const uint32_t b = bin[j] & 0xffff;
+            if (b <= most) {
+                atomicAdd((ull*)&s.mass[b], (ull)sc.mass(l[j]));
+                ids[(s.cnt[b] >> 16) + (bin[j] >> 16)] = (uint16_t)(first - id0 + 64 * j);
+            }
+            if (j % 2) __builtin_amdgcn_sched_barrier(0);            // (two exponentials' registers at a time)
         }
         __syncthreads();
         for (int i = tid; i < kBins; i += 512) g.cnt[at * kBins + i] = s.cnt[i], g.mass[at * kBins + i] = s.mass[i];
+        const int n = ((s.cnt[most] >> 16) + (s.cnt[most] & 0xffff) + 7) / 8;
+        for (int i = tid; i < n; i += 512) *(u32x4*)(g.ids + at * kChunk + 8 * i) = *(const u32x4*)(ids + 8 * i);
         return;
     }
     uint64_t mass[NV];
@@ -566,35 +599,30 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
     }
     const Scale sc(m, lo, q.temp, a.unit);
     uint64_t last = ~0ull;
-    if (q.min_p > 0.f) last = (uint64_t)~least_key(sc.wt, fmin((double)q.min_p, 1.)) << 32 | 0xffffffffull;
+    if (q.min_p > 0.f) {
+        const double p = fmin((double)q.min_p, 1.);
+        last = (uint64_t)~least_key(key_of(m), [&](float y) { return sc.wt.of(y) >= p; }) << 32 | 0xffffffffull;
+    }
     if (q.by_k || q.by_p) {
         auto fill = [&] {                // the row's bins: two halves of the chunks
             const int b = tid & (kBins - 1), half = tid / kBins;
             uint32_t n = 0;
             uint64_t w = 0;
-#pragma unroll 4
-            for (int c = half; c < g.chunks; c += NT / kBins) n += g.cnt[(at0 + c) * kBins + b], w += g.mass[(at0 + c) * kBins + b];
+#pragma unroll 8
+            for (int c = half; c < g.chunks; c += NT / kBins) n += g.cnt[(at0 + c) * kBins + b] & 0xffff, w += g.mass[(at0 + c) * kBins + b];
             __syncthreads();
             if (half) s.cnt[b] = n, s.mass[b] = w;
             __syncthreads();
             if (!half) s.cnt[b] += n, s.mass[b] += w;
             __syncthreads();
         };
-        auto each = [&](int bin, auto f) {
-            for (int c0 = 0; c0 < g.chunks; c0 += 64) {  // (chunks that have some: asked for 64 at a time)
-                uint64_t some = __ballot(c0 + lane < g.chunks && g.cnt[(at0 + min(c0 + lane, g.chunks - 1)) * kBins + bin] != 0);
-                float next[NV];                          // the next one's logits on their way while one is looked at
-                auto id_of = [&](uint64_t set) { return (c0 + __builtin_ctzll(set)) * kChunk; };
-                if (some) load_chunk<T, NT>(x, V, id_of(some), next);
-                for (; some; some &= some - 1) {
-                    const int id0 = id_of(some);
-                    float y[NV];
-#pragma unroll
-                    for (int j = 0; j < NV; j++) y[j] = next[j];
-                    if (some & (some - 1)) load_chunk<T, NT>(x, V, id_of(some & (some - 1)), next);
-#pragma unroll
-                    for (int j = 0; j < NV; j++)
-                        if (id0 + first + 64 * j < V) f(y[j], id0 + first + 64 * j);
+        auto each = [&](int bin, auto f) {               // a wave per chunk
+            for (int c = wave; c < g.chunks; c += NT / 64) {
+                const uint32_t w = g.cnt[(at0 + c) * kBins + bin], n = w & 0xffff;
+                const uint16_t* ids = g.ids + (at0 + c) * kChunk + (w >> 16);
+                for (uint32_t i = lane; i < n; i += 64) {
+                    const int id = c * kChunk + ids[i];
+                    f((float)x[id], id);
                 }
             }
         };
@@ -637,7 +665,7 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
             for (uint32_t i = tid; i < n; i += NT) add(s.place[i], s.w[i]);
         } else {
             each(bin, [&](float y, int i) {
-                if (sc.bin(y) == bin) add(place_of(y, i), sc.mass(y));
+                if (sc.bin(y) == bin && place_of(y, i) <= last) add(place_of(y, i), sc.mass(y));
             });
         }
     } else {
@@ -682,16 +710,17 @@ void launch_short(const SampleArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((k_sample<T, 1024, 8>), grid, dim3(1024), 0, s, a);
 }
 
-constexpr size_t kRowBytes = sizeof(f32x4) + sizeof(uint64_t) + kBins * (sizeof(uint64_t) + sizeof(uint32_t));   // of a chunk
+constexpr size_t kRowBytes = sizeof(f32x4) + sizeof(uint64_t) + kBins * (sizeof(uint64_t) + sizeof(uint32_t)) + kChunk * sizeof(uint16_t);   // of a chunk
 
 template <typename T>
 void launch_long(const SampleArgs& a, const SamplePlan& p, hipStream_t s) {
     for (int r0 = 0; r0 < a.rows; r0 += p.batch) {
         const size_t n = (size_t)std::min(p.batch, a.rows - r0) * p.chunks;
-        Long g{p.chunks, r0, (f32x4*)a.ws, nullptr, nullptr, nullptr};
-        g.kept = (uint64_t*)(g.range + n);
-        g.mass = g.kept + n;
-        g.cnt = (uint32_t*)(g.mass + n * kBins);
+        Long g{p.chunks, r0, (f32x4*)a.ws, nullptr, nullptr, nullptr, nullptr};
+        g.ids = (uint16_t*)(g.range + n);
+        g.mass = (uint64_t*)(g.ids + n * kChunk);
+        g.kept = g.mass + n * kBins;
+        g.cnt = (uint32_t*)(g.kept + n);
         const unsigned rows = (unsigned)std::min(p.batch, a.rows - r0);
         hipLaunchKernelGGL(k_sample_range<T>, dim3((unsigned)p.chunks, rows), dim3(512), 0, s, a, g);
         hipLaunchKernelGGL(k_sample_bins<T>, dim3((unsigned)p.chunks, rows), dim3(512), 0, s, a, g);
@@ -708,13 +737,13 @@ double sample_unit(int V) {
     return (double)(1ull << s);
 }
 
-// A row in one workgroup up to 8192 tokens; longer ones in chunks, as many rows at a time as 64 MB of bins hold
+// A row in one workgroup up to 8192 tokens; longer ones in chunks, as many rows at a time as 128 MB of bins and ids hold
 SamplePlan sample_plan(const SampleArgs& a) {
     SamplePlan p{};
     if (a.V <= kChunk) return p;
     p.chunks = (a.V + kChunk - 1) / kChunk;
     const size_t per = kRowBytes * p.chunks;
-    p.batch = (int)std::min<size_t>({(size_t)a.rows, std::max<size_t>(1, ((size_t)64 << 20) / per), 65535});
+    p.batch = (int)std::min<size_t>({(size_t)a.rows, std::max<size_t>(1, ((size_t)128 << 20) / per), 65535});
     p.ws_bytes = per * p.batch;
     return p;
 }
