@@ -491,7 +491,7 @@ __device__ __forceinline__ void row_range(L& s, const Long& g, float& m, float& 
 }
 
 template <typename T>
-__global__ __launch_bounds__(512, 6) void k_sample_bins(SampleArgs a, Long g) {
+__global__ __launch_bounds__(512, 4) void k_sample_bins(SampleArgs a, Long g) {
     constexpr int NV = kChunk / 512;
     __shared__ Lds<0, 512> s;
     __shared__ __attribute__((aligned(16))) uint16_t ids[kChunk];
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(512, 6) void k_sample_bins(SampleArgs a, Long g) {
                 atomicAdd((ull*)&s.mass[b], (ull)sc.mass(l[j]));
                 ids[(s.cnt[b] >> 16) + (bin[j] >> 16)] = (uint16_t)(first - id0 + 64 * j);
             }
-            if (j % 2) __builtin_amdgcn_sched_barrier(0);            // (two exponentials' registers at a time)
+            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);       // (four exponentials' registers at a time)
         }
         __syncthreads();
         for (int i = tid; i < kBins; i += 512) g.cnt[at * kBins + i] = s.cnt[i], g.mass[at * kBins + i] = s.mass[i];
@@ -550,6 +550,7 @@ __global__ __launch_bounds__(512, 6) void k_sample_bins(SampleArgs a, Long g) {
     for (int j = 0; j < NV; j++) {
         const double w = sc.wt.of(l[j]);
         mass[j] = !(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.) ? sc.wt.mass(w) : 0;
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
     const uint64_t all = wave_sums<NV>(s, mass);
     if (tid == 0) g.kept[at] = all;
