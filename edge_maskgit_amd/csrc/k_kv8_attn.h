@@ -61,6 +61,171 @@ __device__ __forceinline__ f16x8 widen(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(f16x8, v);
 }
 
+// A wave's QT tiles of 16 rows on their way over the blocks: lane l16 + 16 lg holds row l16's scores of the keys 8 lg + 0 .. 7 of a
+// block, and its output's features 32 g + 8 lg + 2 r + (c & 1), c = 2 g + ..., r
+template <int DG, int QT, bool PS, bool MOD>
+struct CacheRows {
+    static constexpr int DK = (DG + 1) / 2;
+    f16x8 qf[QT][2 * DK];                // rows of Q as the B operand: features 64 g + 16 lg + 8 j + e
+    float slope2[QT];
+    int lim[QT];                         // a row's position, the last key it sees; -1: none
+    float mref[QT], S1[QT];
+    f32x4 O[QT][2 * DG];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            mref[t] = kNoScore;
+            S1[t] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2 * DG; c++) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // tile t's row of this lane: sequence b, token i, head h. Rows of whole pieces: all their loads at once (a branch for each
+    // piece made them wait for one another: 8 round trips for two tiles of 128 features)
+    __device__ __forceinline__ void load(const Kv8AttnArgs& a, int t, int b, int i, int h, int last) {
+        const int D = a.c.D, lg = (threadIdx.x >> 4) & 3;
+        lim[t] = last;
+        slope2[t] = MOD && a.slopes ? a.slopes[h] * kLog2e : 0.f;
+        const int64_t e = b * a.qst[3] + (int64_t)h * a.qst[2] + i * a.qst[1];
+        auto at = [&](int c) { return 64 * (c >> 1) + 16 * lg + 8 * (c & 1); };
+        const f16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < 2 * DK; c++) qf[t][c] = zero;
+        if (last < 0) return;
+        if (a.vec_q) {
+#pragma unroll
+            for (int c = 0; c < 2 * DK; c++) qf[t][c] = *(const f16x8*)((const _Float16*)a.q + e + (at(c) < D ? at(c) : 0));
+#pragma unroll
+            for (int c = 0; c < 2 * DK; c++) qf[t][c] = at(c) < D ? qf[t][c] : zero;
+            return;
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * DK; c++) {
+            if (at(c) >= D) continue;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int64_t x = e + (int64_t)(at(c) + j) * a.qst[0];
+                qf[t][c][j] = a.in16 ? ((const _Float16*)a.q)[x] : (_Float16)((const float*)a.q)[x];
+            }
+        }
+    }
+    // one block: kf(t, c) K's fragment of key tile t and features c, vf(c) V's of features 32 (c / 2) + 2 l16 + c % 2, between(): what
+    // is asked for while the scores become weights. MASK: some row may not see some key
+    template <bool MASK, class KF, class VF>
+    __device__ __forceinline__ void block(const ScoreMod& mod, int blk, float ks, float vs, KF kf, VF vf) {
+        block<MASK>(mod, blk, ks, vs, kf, vf, [] {});
+    }
+    template <bool MASK, class KF, class VF, class B>
+    __device__ __forceinline__ void block(const ScoreMod& mod, int blk, float ks, float vs, KF kf, VF vf, B between) {
+        const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+        f32x4 sc[QT][2];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+            for (int t = 0; t < QT; t++) sc[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2 * DK; c++) {
+                const f16x8 k = kf(n, c);
+#pragma unroll
+                for (int t = 0; t < QT; t++) sc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[t][c], sc[t][n], 0, 0, 0);
+            }
+        }
+        between();
+        const int j0 = blk * kKvBlock + 8 * ((threadIdx.x >> 4) & 3);              // this lane's keys: j0 + 4 n + r
+        const float scale = ks * (MOD && mod.cap2 != 0.f ? 1.f : mod.scale2);
+        auto mapped = [&](auto map) {                        // scores of the map, then slopes (of the keys that a row sees)
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                const float d0 = (float)(lim[t] - j0);
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float s = map(sc[t][n][r] * scale);
+                        sc[t][n][r] = MOD ? fmaf(-slope2[t], d0 - (float)(4 * n + r), s) : s;
+                    }
+            }
+        };
+        if (MOD && mod.cap2 != 0.f) {
+            float big = 0.f;
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    big = fmaxf(fmaxf(big, fabsf(sc[t][n][0])), fabsf(sc[t][n][1]));
+                    big = fmaxf(fmaxf(big, fabsf(sc[t][n][2])), fabsf(sc[t][n][3]));
+                }
+            if (all_small(big * scale, mod)) mapped([&](float x) { return cap_small(x, mod); });
+            else mapped([&](float x) { return cap_score(x, mod); });
+        } else {
+            mapped([](float x) { return x; });
+        }
+        float mx[QT];
+        bool any = false;
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            mx[t] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float s = MASK && j0 + 4 * n + r > lim[t] ? -INFINITY : sc[t][n][r];
+                    sc[t][n][r] = s;
+                    mx[t] = fmaxf(mx[t], s);
+                }
+            any = any || __any(mx[t] > mref[t] + 15.f);
+        }
+        if (any) {
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                float v = fmaxf(mx[t] - 7.f, mref[t]);
+                v = fmaxf(v, __shfl_xor(v, 16));
+                v = fmaxf(v, __shfl_xor(v, 32));
+                const float al = __builtin_amdgcn_exp2f(mref[t] - v);
+                mref[t] = v;
+                S1[t] *= al;
+#pragma unroll
+                for (int c = 0; c < 2 * DG; c++) O[t][c] *= al;
+            }
+        }
+        f16x8 ph[QT], pl[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f32x2 e = {__builtin_amdgcn_exp2f(sc[t][j >> 1][2 * (j & 1)] - mref[t]),
+                                 __builtin_amdgcn_exp2f(sc[t][j >> 1][2 * (j & 1) + 1] - mref[t])};
+                const f16x2 h = __builtin_convertvector(e, f16x2);
+                hi[j] = __builtin_bit_cast(uint32_t, h);
+                if (PS) {
+                    const f32x2 d = {e[0] - (float)h[0], e[1] - (float)h[1]};
+                    lo[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, f16x2));
+                }
+            }
+            ph[t] = __builtin_bit_cast(f16x8, hi);
+            if (PS) pl[t] = __builtin_bit_cast(f16x8, lo);
+            f32x4 s1 = {0.f, 0.f, 0.f, 0.f};
+            if (PS) s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t], s1, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[t], s1, 0, 0, 0);
+            S1[t] += s1[0];
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * DG; c++) {
+            const f16x8 v = vf(c);
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+                if (PS) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[t], o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) O[t][c][r] = fmaf(vs, o[r], O[t][c][r]);
+            }
+        }
+    }
+};
+
 // What a workgroup's rows and blocks are. kAlone: one sequence's rows over its blocks. Sequences that share their first
 // blocks: kOwn, one sequence's rows over the blocks behind the shared ones; kShared, the rows of all sequences of a
 // group over the shared ones, which the group's first sequence's row of the table names and which all its rows see whole.
@@ -81,18 +246,26 @@ __device__ __forceinline__ bool spans_of(const Kv8AttnArgs& a, int b, int& len, 
 
 // DG 32-feature groups (D <= 32 DG), QT 16-row tiles, PS: weights as hi + lo, MOD: capped or sloped. The part sp of this
 // launch's `splits` is part part0 + sp of all `parts` that the join sees.
+template <int DG, int QT>
+struct CacheLds {
+    __attribute__((aligned(16))) float so[4][16 * QT][32 * DG + 4];
+    float sm[4][16 * QT][2];
+    int odd[16 * QT], gone[4];
+};
 template <int DG, int QT, bool PS, bool MOD, int MODE>
-__device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles, int splits, int least, int parts, int part0) {
-    constexpr int DK = (DG + 1) / 2, ROWS = 16 * QT, OLD = 32 * DG + 4;
-    __shared__ __attribute__((aligned(16))) float so[4][ROWS][OLD];
-    __shared__ float sm[4][ROWS][2];
-    __shared__ int odd[ROWS], gone[4];
+__device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int wg, int tiles, int splits, int least, int parts, int part0,
+                                                CacheLds<DG, QT>& lds) {
+    constexpr int DK = (DG + 1) / 2, ROWS = 16 * QT;
+    auto& so = lds.so;
+    auto& sm = lds.sm;
+    auto& odd = lds.odd;
+    auto& gone = lds.gone;
     const Kv8& cache = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, lg = lane >> 4, D = cache.D;
     // heads innermost, so that each XCD (blockIdx % 8) gets as many of the first parts, which every sequence has
     const int sets = MODE == kShared ? (cache.B + a.group - 1) / a.group : cache.B;
-    const int heads = cache.Hkv * sets, hb = blockIdx.x % heads, in_h = blockIdx.x / heads;
+    const int heads = cache.Hkv * sets, hb = wg % heads, in_h = wg / heads;
     const int sp = in_h / tiles, tile = in_h - sp * tiles;
     const int hk = hb % cache.Hkv, G = a.H / cache.Hkv, b = hb / cache.Hkv * (MODE == kShared ? a.group : 1);
     const int RB = a.S * G;                                  // rows of a sequence
@@ -147,32 +320,12 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
         if (parts > 1 && b0 >= b1 && fits) return;
     }
 
-    // rows of Q as the B operand: features 64 g + 16 lg + 8 j + e
-    f16x8 qf[QT][2 * DK];
-    float slope2[QT];
-    int lim[QT];
+    CacheRows<DG, QT, PS, MOD> st;
+    st.clear();
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const Row row = row_of(min(r0 + 16 * t + l16, RS - 1));
-        lim[t] = r0 + 16 * t + l16 < R && row.live ? row.p : -1;
-        slope2[t] = MOD && a.slopes ? a.slopes[hk * G + row.g] * kLog2e : 0.f;
-        const int64_t e = row.b * a.qst[3] + (int64_t)(hk * G + row.g) * a.qst[2] + row.i * a.qst[1];
-#pragma unroll
-        for (int c = 0; c < 2 * DK; c++) {
-            const int d = 64 * (c >> 1) + 16 * lg + 8 * (c & 1);
-            qf[t][c] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (d < D && lim[t] >= 0) {
-                if (a.vec_q) {
-                    qf[t][c] = *(const f16x8*)((const _Float16*)a.q + e + d);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int64_t x = e + (int64_t)(d + j) * a.qst[0];
-                        qf[t][c][j] = a.in16 ? ((const _Float16*)a.q)[x] : (_Float16)((const float*)a.q)[x];
-                    }
-                }
-            }
-        }
+        st.load(a, t, row.b, row.i, hk * G + row.g, r0 + 16 * t + l16 < R && row.live ? row.p : -1);
     }
 
     // where this lane reads in a block: K's key and features of tile t (+ 4 keys), V's feature pair and keys;
@@ -183,124 +336,6 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
     for (int g = 0; g < DK; g++) ka[g] = key * D + (64 * g + 16 * lg < D ? 64 * g + 16 * lg : 0);
 #pragma unroll
     for (int g = 0; g < DG; g++) va[g] = 32 * g + 2 * l16 < D ? ((16 * g + l16) * 4 + lg) * 16 : 0;
-
-    float mref[QT], S1[QT];
-    f32x4 O[QT][2 * DG];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        mref[t] = kNoScore;
-        S1[t] = 0.f;
-#pragma unroll
-        for (int c = 0; c < 2 * DG; c++) O[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-
-    // one block: kf(t, c) K's fragment of key tile t and features c, vf(c) V's of features 32 (c / 2) + 2 l16 + c % 2
-    auto block = [&](int blk, float ks, float vs, auto kf, auto vf) {
-        f32x4 sc[QT][2];
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-#pragma unroll
-            for (int t = 0; t < QT; t++) sc[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 2 * DK; c++) {
-                const f16x8 k = kf(n, c);
-#pragma unroll
-                for (int t = 0; t < QT; t++) sc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[t][c], sc[t][n], 0, 0, 0);
-            }
-        }
-        const int j0 = blk * kKvBlock + 8 * lg;              // this lane's keys: j0 + 4 n + r
-        const float scale = ks * (MOD && a.mod.cap2 != 0.f ? 1.f : a.mod.scale2);
-        auto mapped = [&](auto map) {                        // scores of the map, then slopes (of the keys that a row sees)
-#pragma unroll
-            for (int t = 0; t < QT; t++) {
-                const float d0 = (float)(lim[t] - j0);
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float s = map(sc[t][n][r] * scale);
-                        sc[t][n][r] = MOD ? fmaf(-slope2[t], d0 - (float)(4 * n + r), s) : s;
-                    }
-            }
-        };
-        if (MOD && a.mod.cap2 != 0.f) {
-            float big = 0.f;
-#pragma unroll
-            for (int t = 0; t < QT; t++)
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    big = fmaxf(fmaxf(big, fabsf(sc[t][n][0])), fabsf(sc[t][n][1]));
-                    big = fmaxf(fmaxf(big, fabsf(sc[t][n][2])), fabsf(sc[t][n][3]));
-                }
-            if (all_small(big * scale, a.mod)) mapped([&](float x) { return cap_small(x, a.mod); });
-            else mapped([&](float x) { return cap_score(x, a.mod); });
-        } else {
-            mapped([](float x) { return x; });
-        }
-        float mx[QT];
-        bool any = false;
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            mx[t] = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float s = j0 + 4 * n + r > lim[t] ? -INFINITY : sc[t][n][r];
-                    sc[t][n][r] = s;
-                    mx[t] = fmaxf(mx[t], s);
-                }
-            any = any || __any(mx[t] > mref[t] + 15.f);
-        }
-        if (any) {
-#pragma unroll
-            for (int t = 0; t < QT; t++) {
-                float v = fmaxf(mx[t] - 7.f, mref[t]);
-                v = fmaxf(v, __shfl_xor(v, 16));
-                v = fmaxf(v, __shfl_xor(v, 32));
-                const float al = __builtin_amdgcn_exp2f(mref[t] - v);
-                mref[t] = v;
-                S1[t] *= al;
-#pragma unroll
-                for (int c = 0; c < 2 * DG; c++) O[t][c] *= al;
-            }
-        }
-        f16x8 ph[QT], pl[QT];
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            u32x4 hi, lo;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f32x2 e = {__builtin_amdgcn_exp2f(sc[t][j >> 1][2 * (j & 1)] - mref[t]),
-                                 __builtin_amdgcn_exp2f(sc[t][j >> 1][2 * (j & 1) + 1] - mref[t])};
-                const f16x2 h = __builtin_convertvector(e, f16x2);
-                hi[j] = __builtin_bit_cast(uint32_t, h);
-                if (PS) {
-                    const f32x2 d = {e[0] - (float)h[0], e[1] - (float)h[1]};
-                    lo[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, f16x2));
-                }
-            }
-            ph[t] = __builtin_bit_cast(f16x8, hi);
-            if (PS) pl[t] = __builtin_bit_cast(f16x8, lo);
-            f32x4 s1 = {0.f, 0.f, 0.f, 0.f};
-            if (PS) s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[t], s1, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[t], s1, 0, 0, 0);
-            S1[t] += s1[0];
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * DG; c++) {
-            const f16x8 v = vf(c);
-#pragma unroll
-            for (int t = 0; t < QT; t++) {
-                f32x4 o = {0.f, 0.f, 0.f, 0.f};
-                if (PS) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[t], o, 0, 0, 0);
-                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; r++) O[t][c][r] = fmaf(vs, o[r], O[t][c][r]);
-            }
-        }
-    };
 
     // this wave's whole blocks b0 + wave, + 4, ..., two sets of registers in turn. Every load is made, past the last
     // block that one's again and for a page outside the pool page 0's: behind a branch around them the compiler
@@ -334,7 +369,7 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
         x.s = *(const f32x2*)(cache.scales + 2 * at);
     };
     auto use = [&](int blk, const Set& x) {
-        block(blk, x.s[0], x.s[1],
+        st.template block<true>(a.mod, blk, x.s[0], x.s[1],
               [&](int n, int c) { const u32x4 w = x.k[2 * (c >> 1) + n]; return c & 1 ? widen(w[2], w[3]) : widen(w[0], w[1]); },
               [&](int c) { const u32x4 w = x.v[c >> 1]; return c & 1 ? widen(w[2], w[3]) : widen(w[0], w[1]); });
     };
@@ -355,7 +390,7 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
         const _Float16* K = cache.k_tail + at * kKvRing * D;
         const _Float16* V = cache.v_tail + at * D * kKvRing;
         const int slot = cut % kKvRing, left = total - cut - 8 * lg;         // values of this lane's 8 keys
-        block(whole, 1.f, 1.f,
+        st.template block<true>(a.mod, whole, 1.f, 1.f,
               [&](int n, int c) {
                   const int d = 64 * (c >> 1) + 16 * lg + 8 * (c & 1);
                   const f16x8 k = *(const f16x8*)(K + (slot + key + 4 * n) * D + (d < D ? d : 0));
@@ -379,10 +414,10 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 // features 32 g + 8 lg + 2 r + (c & 1), r = 2 h, 2 h + 1
-                const f32x4 v = {O[t][2 * g][2 * h], O[t][2 * g + 1][2 * h], O[t][2 * g][2 * h + 1], O[t][2 * g + 1][2 * h + 1]};
+                const f32x4 v = {st.O[t][2 * g][2 * h], st.O[t][2 * g + 1][2 * h], st.O[t][2 * g][2 * h + 1], st.O[t][2 * g + 1][2 * h + 1]};
                 *(f32x4*)&so[wave][16 * t + l16][32 * g + 8 * lg + 4 * h] = v;
             }
-        if (lg == 0) sm[wave][16 * t + l16][0] = mref[t], sm[wave][16 * t + l16][1] = S1[t];
+        if (lg == 0) sm[wave][16 * t + l16][0] = st.mref[t], sm[wave][16 * t + l16][1] = st.S1[t];
     }
     if (MODE != kShared && tid < ROWS) odd[tid] = 0;
     if (lane == 0) gone[wave] = lost;
@@ -437,7 +472,7 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
     for (int r = wave; r < nr; r += 4) {
         if (MODE == kShared ? odd[r] != 1 : !odd[r]) continue;
         const Row row = row_of(r0 + r);
-        RowState st{0.f, 1.f, {__builtin_nanf(""), __builtin_nanf("")}};
+        RowState again_st{0.f, 1.f, {__builtin_nanf(""), __builtin_nanf("")}};
         if (fits) {
             const int64_t e = row.b * a.qst[3] + (int64_t)(hk * G + row.g) * a.qst[2] + row.i * a.qst[1];
             for (int d = lane; d < D; d += 64) {
@@ -452,14 +487,14 @@ __device__ __forceinline__ void cache_attention(const Kv8AttnArgs& a, int tiles,
                 spans_of<MODE>(a, row.b, l, n, row_same);
                 row_cut = n / kKvBlock * kKvBlock;
             }
-            st = attn_row(CacheSrc{cache, row.b, hk, row_cut, MODE == kAlone ? b : row.b / a.group * a.group, row_same}, a.mod,
+            again_st = attn_row(CacheSrc{cache, row.b, hk, row_cut, MODE == kAlone ? b : row.b / a.group * a.group, row_same}, a.mod,
                           a.slopes ? a.slopes[hk * G + row.g] * kLog2e : 0.f, p, p + 1, (int64_t)b0 * kKvBlock,
                           min((int64_t)b1 * kKvBlock, p + 1), D, qs, qs + 128, lane);
             __builtin_amdgcn_wave_barrier();
         }
-        qs[lane] = st.o[0], qs[lane + 64] = st.o[1];
+        qs[lane] = again_st.o[0], qs[lane + 64] = again_st.o[1];
         __builtin_amdgcn_wave_barrier();
-        if (4 * lane < D) put(r0 + r, 4 * lane, *(const f32x4*)&qs[4 * lane], st.m == -INFINITY ? kNoScore : st.m, st.l);
+        if (4 * lane < D) put(r0 + r, 4 * lane, *(const f32x4*)&qs[4 * lane], again_st.m == -INFINITY ? kNoScore : again_st.m, again_st.l);
         __builtin_amdgcn_wave_barrier();
     }
 }

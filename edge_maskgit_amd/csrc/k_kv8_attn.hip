@@ -30,7 +30,8 @@ namespace {
 
 template <int DG, int QT, bool PS, bool MOD>
 __global__ __launch_bounds__(256, QT == 1 ? 3 : 2) void k_kv8_attn(Kv8AttnArgs a, int tiles, int splits, int least) {
-    cache_attention<DG, QT, PS, MOD, kAlone>(a, tiles, splits, least, splits, 0);
+    __shared__ CacheLds<DG, QT> lds;
+    cache_attention<DG, QT, PS, MOD, kAlone>(a, blockIdx.x, tiles, splits, least, splits, 0, lds);
 }
 
 }  // namespace

@@ -409,6 +409,7 @@ Kv8Plan kv8_plan(const Kv8AttnArgs& a);
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, const Kv8Plan& p, hipStream_t s);
 struct Kv8SharedPlan {
     Kv8Plan own, shared;   // parts of a sequence's own blocks, parts of a group's shared ones
+    bool rows;             // each wave rows of its own over the shared blocks, 16 qt of them
     size_t ws_bytes;
 };
 Kv8SharedPlan kv8_shared_plan(const Kv8AttnArgs& a);

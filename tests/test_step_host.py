@@ -173,3 +173,76 @@ def test_entry_points_take_no_context():
     L = ema.lib()
     assert L.mgh_sample(None, None, 0, 1, 1, 1, None, None, None, None) == -1
     assert L.mgh_rope(None, None, None, 0, None, 2, 1, 1, 1, None, None, None, None, None) == -1
+
+
+def test_which_kernels_shared_attention_takes():
+    """few rows of a group, 64 and 128 of them to a workgroup; a workgroup of the shared blocks per CU, then the own ones'"""
+    run(BODY + """
+def call(S, H, Hkv, D, Bn, nb, group, most, **kw):
+    kv = ema.Kv8(W, X, B, R, Y, G, nb, 1 << 20, Hkv, D, Bn)
+    launches()
+    c.kv8_attn_shared(kv, 0x1200000, (1, H * D, D, S * H * D), S, 0x1300000, None, group, 0x1600000, most, H, D ** -0.5, o16=0x1400000, **kw)
+    l = launches()
+    m = re.search(r"k_kv8_attn_sharedILi(\\d)ELb(\\d)ELb(\\d)ELi(\\d)E", l[0][1])
+    return tuple(map(int, m.groups())), l[0][2][0], [k for k, _, _ in l[1:]]
+
+few, many = ["k_attn_join_few"], ["k_attn_join"]
+# 256 rows of a key head: two tiles of 128, 16 parts; the own blocks of 64 sequences
+assert call(1, 32, 8, 128, 64, 266, 64, 250) == ((4, 0, 0, 2), 8 * 2 * 16 + 512, many)
+assert call(1, 32, 8, 128, 64, 266, 16, 250) == ((4, 0, 0, 1), 8 * 4 * 8 + 512, many)
+assert call(1, 32, 8, 128, 64, 266, 8, 250) == ((4, 0, 0, 0), 8 * 8 * 2 * 2 + 512, few)
+assert call(1, 32, 8, 128, 64, 266, 4, 250)[0] == (4, 0, 0, 0)
+# at least eight blocks to a part; no shared block at all
+assert call(1, 32, 8, 128, 64, 30, 64, 20) == ((4, 0, 0, 2), 8 * 2 * 3 + 512, few)
+assert call(1, 32, 8, 128, 64, 30, 64, 0) == ((4, 0, 0, 2), 8 * 2 + 512, few)
+# own rows of more than 16: tiles of 16
+assert call(5, 32, 8, 128, 4, 40, 4, 32)[1] == 8 * 4 + 8 * 4 * 2
+for D, dg in ((16, 1), (32, 1), (48, 2), (64, 2), (80, 3), (96, 3), (112, 4)):
+    assert call(1, 8, 8, D, 64, 8, 64, 4)[0] == (dg, 0, 0, 1)
+assert call(1, 8, 8, 64, 64, 8, 64, 4, cap=3.0)[0] == call(1, 8, 8, 64, 64, 8, 64, 4, slopes=0x1500000)[0] == (2, 0, 1, 1)
+""")
+
+
+def test_which_kernels_rope_takes():
+    """granules of 8, 4 and 1 pairs by order, type and alignment; heads of a thread by the number of rows"""
+    run(ROPE + """
+def call(pairs, D, order=0, in16=True, out16=True, S=9, H=4, Bn=2, x=W, st=None):
+    st = st or (1, H * D, D, S * H * D)
+    launches()
+    c.rope(rot(pairs, order=order), x, st, D, S, H, Bn, in16=in16, y_strides=(1, H * D, D, S * H * D), **{"y16" if out16 else "y": Y})
+    (k, n, g), = launches()
+    m = re.search(r"k_ropeILi(\\d)ELb(\\d)ELb(\\d)E", n)
+    return tuple(map(int, m.groups())), g[:2]
+
+assert call((8,), 16) == ((8, 1, 1), (1, 2))
+assert call((8,), 16, in16=False) == ((4, 0, 1), (1, 2)) and call((8,), 16, out16=False)[0] == (4, 1, 0) and call((8,), 16, in16=False, out16=False)[0] == (4, 0, 0)
+assert call((12, 12), 48)[0] == (8, 1, 1) and call((12, 12), 48, order=1)[0] == (8, 1, 1) and call((12, 12), 48, order=2)[0] == (4, 1, 1)
+assert call((5,), 16)[0] == (1, 1, 1) and call((4,), 16)[0] == (4, 1, 1) and call((0,), 24)[0] == (4, 1, 1) and call((3,), 6)[0] == (1, 1, 1)
+assert call((8,), 16, x=W + 2)[0] == (1, 1, 1) and call((8,), 16, x=W + 8)[0] == (4, 1, 1) and call((8,), 16, st=(1, 66, 16, 66 * 9))[0] == (1, 1, 1)
+# a thread takes 1 head of few rows, 8 of very many
+assert call((64,), 128, S=100, H=32)[1] == (100 * 32 * 8 // 256, 2)
+assert call((64,), 128, S=65536, H=32)[1] == (65536 * 4 * 8 // 256, 2)
+""")
+
+
+def test_which_kernels_sampling_takes():
+    """rows up to 2048 and 8192 tokens in one workgroup, longer ones in chunks of 8192, rows by rows of 128 MB"""
+    run(BODY + """
+def call(rows, V, **kw):
+    launches()
+    c.sample(W, rows, V, X, Y, **kw)
+    return [(k, g[:2]) for k, _, g in launches()]
+
+assert call(3, 2048) == [("k_sample", (3, 1))] and call(3, 2049) == call(3, 8192) == [("k_sample", (3, 1))]
+assert call(3, 8193) == [("k_sample_range", (2, 3)), ("k_sample_bins", (2, 3)), ("k_sample_pick", (1, 3))]
+l = call(1000, 128001, f16=True)
+assert [k for k, _ in l] == ["k_sample_range", "k_sample_bins", "k_sample_pick"] * 3
+assert sum(g[1] for k, g in l if k == "k_sample_pick") == 1000
+assert call(1, 1 << 24)[0] == ("k_sample_range", (2048, 1))
+c.graph_begin()
+try:
+    call(1, (1 << 24) - 1)
+    call(64, 128001)
+finally:
+    c.graph_end().destroy()
+""")
