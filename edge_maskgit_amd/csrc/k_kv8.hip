@@ -57,7 +57,9 @@ __device__ __forceinline__ void load_row(const void* p, int64_t e, int64_t st, _
 // workgroup stores all, after its reads. Four prompts of 2050 tokens, 8 heads of 128, 50 MB: 15.2 us, 5 us more
 // where the first workgroup stores all.
 // ROT: keys are rotated on the way (k_rope.h), before they are rounded to fp16: the 16 features are 8 pairs, in
-// granules of ROT pairs, whose features lie in two runs; 0: as they come, 16 in a row.
+// granules of ROT pairs, whose features lie in two runs; 0: as they come, 16 in a row. In 64 bits: with fp32's 2^-23 one value
+// in 2^12 rounds to the other fp16 number, and one in 2^16 to another code, an error of 1 / 127 of the block's largest, which
+// made half of what all roundings to fp16 together make (2.4e-4 against 2.1e-4 of the values read back).
 template <bool IN16, bool VEC, int ROT>
 __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotation* r) {
     __shared__ uint32_t mx[2][4];
@@ -132,16 +134,12 @@ __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotat
             float v[16];
             runs(u, [&](int i, int d) { load_features<ROT, IN16, VEC>(a.k, at(t, d), a.st[0], v + i); });
 #pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = (_Float16)v[i];
+#pragma unroll
             for (int g = 0; g < NU / 2; g++) {
                 const int pair = 8 * u + ROT * g;
-                if (pair < r->P) {
-                    SinCos sc[ROT];
-                    angles<ROT>(*r, p, f[g], pair, sc);
-                    rotate<ROT>(*r, sc, v + 2 * ROT * g);
-                }
+                if (pair < r->P) rotate64<ROT>(*r, p, f[g], pair, v + 2 * ROT * g, x + 2 * ROT * g);
             }
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = (_Float16)v[i];
         }
     };
     auto load_ring_k = [&](int t, int u, _Float16* x) {

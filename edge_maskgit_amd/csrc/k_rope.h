@@ -24,8 +24,41 @@ __device__ __forceinline__ SinCos sincos_turns(uint32_t t) {
     return {__builtin_bit_cast(float, a ^ ((q & 2) << 30)), __builtin_bit_cast(float, b ^ (((q + 1) & 2) << 30))};
 }
 
-// the highest 32 bits of p F mod 2^64
-__device__ __forceinline__ uint32_t turns_at(int32_t p, uint64_t F) { return (uint32_t)(((uint64_t)(int64_t)p * F) >> 32); }
+// The same in 64 bits, for values whose rounding decides about a code: sine and cosine of t 2^-64 turns to 2^-45, by their series
+struct SinCos64 {
+    double s, c;
+};
+__device__ __forceinline__ SinCos64 sincos_turns64(uint64_t t) {
+    const uint32_t q = (uint32_t)((t + (1ull << 61)) >> 62);
+    const int64_t r = (int64_t)(t - ((uint64_t)q << 62));
+    const double x = fma((double)(int32_t)(r >> 32), 4294967296., (double)(uint32_t)r) * 3.406121580086554e-19;       // 2 pi 2^-64
+    const double z = x * x, z2 = z * z;
+    const double s1 = fma(z, 0.008333333333333333, -0.16666666666666666), s2 = fma(z, 2.7557319223985893e-06, -0.0001984126984126984);
+    const double s3 = fma(z, 1.6059043836821613e-10, -2.505210838544172e-08);
+    const double s = fma(x * z, fma(fma(s3, z2, s2), z2, s1), x);
+    const double c1 = fma(z, 0.041666666666666664, -0.5), c2 = fma(z, 2.48015873015873e-05, -0.001388888888888889);
+    const double c3 = fma(z, 2.08767569878681e-09, -2.755731922398589e-07);
+    const double c = fma(z, fma(fma(fma(z2, -1.1470745597729725e-11, c3), z2, c2), z2, c1), 1.);
+    const bool odd = q & 1;
+    const double a = odd ? c : s, b = odd ? s : c;
+    return {q & 2 ? -a : a, (q + 1) & 2 ? -b : b};
+}
+
+// to fp16 with one rounding: to fp32 by way of the neighbour whose last bit is 1 where v is not one of them
+__device__ __forceinline__ _Float16 half_of(double v) {
+    const float f = (float)v;
+    const double e = v - (double)f;
+    uint32_t u = __builtin_bit_cast(uint32_t, f);
+    if (e != 0. && !(u & 1) && f - f == 0.f) u += (e > 0.) == (f > 0.f) ? 1u : ~0u;
+    return (_Float16)__builtin_bit_cast(float, u);
+}
+
+// p F mod 2^64: two 32-bit products, p's sign taken off the upper half
+__device__ __forceinline__ uint64_t turns64_at(int32_t p, uint64_t F) {
+    const uint32_t lo = (uint32_t)F, hi = (uint32_t)(F >> 32), less = p < 0 ? lo : 0u;
+    return (uint64_t)(uint32_t)p * lo + ((uint64_t)((uint32_t)p * hi - less) << 32);
+}
+__device__ __forceinline__ uint32_t turns_at(int32_t p, uint64_t F) { return (uint32_t)(turns64_at(p, F) >> 32); }
 
 // a token's positions along the axes (`i` its index in the call, `run` its position where none are given): loads that
 // depend on nothing but the arguments, all four of them, so that none waits for another
@@ -101,6 +134,24 @@ __device__ __forceinline__ void rotate(const Rotation& r, const SinCos* sc, floa
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++) turn(x[i], x[V + i], sc[i]);
+    }
+}
+
+// x as rotate's, in 64 bits, to fp16
+template <int V>
+__device__ __forceinline__ void rotate64(const Rotation& r, const TokenPos& t, const Turns<V>& f, int pair, const float* x, _Float16* y) {
+    auto turn = [&](int i, float a0, float b0, _Float16& u, _Float16& v) {
+        const SinCos64 w = sincos_turns64(turns64_at(t.of(r, pair + i), f.f[i]));
+        const double a = a0, b = b0;
+        u = half_of(fma(a, w.c, -(b * w.s)));
+        v = half_of(fma(a, w.s, b * w.c));
+    };
+    if (r.order == kRopePairs) {
+#pragma unroll
+        for (int i = 0; i < V; i++) turn(i, x[2 * i], x[2 * i + 1], y[2 * i], y[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) turn(i, x[i], x[V + i], y[i], y[V + i]);
     }
 }
 

@@ -187,8 +187,9 @@ def same_state(a, b):
 @pytest.mark.parametrize("order", [0, 1, 2])
 @pytest.mark.parametrize("D,Hkv,G,pairs", [(16, 1, 1, [8]), (48, 3, 1, [12, 12]), (64, 2, 4, [16]), (80, 1, 2, [5, 7, 9]), (128, 2, 3, [16, 24, 24]), (96, 2, 1, [0])])
 def test_rotated_append_is_rope_and_append(ctx, D, Hkv, G, pairs, order):
-    """the same cache, byte for byte, as rotating to fp16 and appending, and the same queries; in odd pieces, from either type,
-    positions given and not"""
+    """the same cache, byte for byte, as appending keys that were rotated in 64 bits and rounded once (the kernel's own 64 bits
+    are off by 2^-45: one value in 2^33 lies so near a border of fp16's), and mgh_rope's queries; in odd pieces, from either
+    type, positions given and not"""
     print(f"append {D} {Hkv} {pairs} {order}", flush=True)
     rng = np.random.default_rng(D + order)
     B, n, H = 2, 150, Hkv * G
@@ -201,7 +202,8 @@ def test_rotated_append_is_rope_and_append(ctx, D, Hkv, G, pairs, order):
         for given in (True, False):
             at = pos if given else np.broadcast_to(np.arange(n, dtype=I32), (len(pairs), B, n))
             with Dev(ctx) as dev:
-                turned, tq = (run_rope(ctx, x.astype(t), at, pairs, f, order, True) for x in (k, q))
+                tq = run_rope(ctx, q.astype(t), at, pairs, f, order, True)
+                turned = ref.rope(k, at, pairs, f, order).astype(F16)
                 want = Cache(dev, B, Hkv, D, 5, np.random.default_rng(1))
                 want.append(turned, v, [0, 0])
                 for steps in ([np.array([n, n])], [np.array([7, 33])] * 22, [np.array([0, 64]), np.array([90, 1])] * 10):
@@ -226,7 +228,7 @@ def test_rotated_append_is_rope_and_append(ctx, D, Hkv, G, pairs, order):
 
 
 def test_rotated_append_against_the_definition(ctx):
-    """keys within the rotation's bound of 64 bits; codes of whole blocks from exactly the fp16 values that the ring had"""
+    """keys rotated in 64 bits and rounded once; codes of whole blocks from exactly the fp16 values that the ring had"""
     rng = np.random.default_rng(3)
     D, Hkv, pairs = 64, 2, [16, 16]
     f = freqs_of(pairs)
@@ -238,13 +240,37 @@ def test_rotated_append_against_the_definition(ctx):
         rot = lambda a, b: ema.Rope(pairs, f, 0, dev.up(np.ascontiguousarray(pos[:, :, a:b])), (1, b - a, b - a))  # noqa: E731
         append_rope(c, rot(0, 31), k[:, :31], v[:, :31], q[:, :31], [0])
         early, _ = c.read([31], 31)
-        check_rope(early.transpose(0, 2, 1, 3).astype(F16), k[:, :31], pos[:, :, :31], pairs, f, 0, True)
+        turned = ref.rope(k, pos, pairs, f, 0).astype(F16)
+        assert np.array_equal(turned[0, :31], early[0].transpose(1, 0, 2))
         append_rope(c, rot(31, 50), k[:, 31:], v[:, 31:], q[:, 31:], [31])
         got, gv = c.read([50], 50)
-        turned = run_rope(ctx, k, pos, pairs, f, 0, True)
-        assert np.array_equal(turned[0, :31], early[0].transpose(1, 0, 2))
         assert np.array_equal(got[0], gen.cache_values(turned[0]).astype(F32).transpose(1, 0, 2))
         assert np.array_equal(gv[0], gen.cache_values(v[0]).astype(F32).transpose(1, 0, 2))
+
+
+def test_rotated_append_of_any_size(ctx):
+    """fp32 keys from fp16's smallest numbers to past its largest, at positions to the ends of 32 bits: rounded once"""
+    rng = np.random.default_rng(33)
+    D, Hkv, pairs = 32, 2, [16]
+    f = [1.0, -1.0, 16.0, 1e-4, 2 * np.pi, np.pi / 2, 1e-9, 0.0, 3.7, 0.1, np.pi, 1 / 3, 15.99999, -1e-3, 5.0, 0.7]
+    size = 2.0 ** rng.integers(-30, 17, (1, 30, Hkv, D))
+    k = (rng.standard_normal((1, 30, Hkv, D)) * size).astype(F32)
+    k[0, 3, 0, 2], k[0, 4, 1, 7], k[0, 5, 0, 31] = np.inf, np.nan, -np.inf
+    pos = rng.integers(-2 ** 31, 2 ** 31, (1, 1, 30)).astype(I32)
+    pos[0, 0, :4] = 0, -2 ** 31, 2 ** 31 - 1, 5
+    for order in (0, 1):
+        with Dev(ctx) as dev:
+            c = Cache(dev, 1, Hkv, D, 1, rng)
+            append_rope(c, ema.Rope(pairs, f, order, dev.up(pos), (1, 30, 30)), k, k, np.zeros((1, 30, Hkv, D), F32), [0], in16=False)
+            got = dev.get(c.kt, (1, Hkv, 64, D), F16)[0, :, :30].transpose(1, 0, 2)
+        with np.errstate(all="ignore"):
+            want = ref.rope(k, pos, pairs, f, order)[0]
+            # the frequency is a whole number of 2^-64 turns: an angle at 2^31 is off by 2^-33 turns, 7e-10 of |a| + |b|
+            room = ref.rope_bound(k, pairs, order, False)[0] / (5 * ref.U) * 1e-9
+            lo, hi = (want - room).astype(F16), (want + room).astype(F16)
+        odd = ~np.isfinite(want)
+        assert not np.isfinite(got[odd]).any()
+        assert ((got >= lo) & (got <= hi))[~odd].all()
 
 
 def test_rotated_append_refuses_bad_numbers_on_the_device(ctx):
