@@ -270,9 +270,9 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
 }
 
 // The same with the keys rotated, and workgroups past the first `blocks` of a head and sequence rotating its query heads:
-// V pairs of one head of one token per thread.
+// V pairs of the heads g, g + HG, ... of one token per thread, so that their angles are computed once.
 template <bool IN16, bool VEC, int ROT, int V>
-__global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int blocks) {
+__global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int blocks, int HG) {
     ask_rotation(a.r);
     asm volatile("" ::"s"(a.a.c.max_blocks), "s"(a.a.c.D), "s"(a.a.c.Hkv), "s"(a.a.lens), "s"(a.a.fresh), "s"(a.a.S));
     if ((int)blockIdx.x < blocks) {
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int bloc
     const Kv8& c = a.a.c;
     asm volatile("" ::"s"(a.q), "s"(a.qo), "s"(a.qst[0]), "s"(a.qst[1]), "s"(a.qst[2]), "s"(a.qst[3]), "s"(a.qost[0]), "s"(a.qost[1]),
                  "s"(a.qost[2]), "s"(a.qost[3]), "s"(a.H), "s"(c.Hkv), "s"(c.D));
-    const int hk = blockIdx.y, b = blockIdx.z, G = a.H / c.Hkv, units = c.D / (2 * V), per = units * G;
+    const int hk = blockIdx.y, b = blockIdx.z, G = a.H / c.Hkv, units = c.D / (2 * V), per = units * HG;
     const uint32_t at = (blockIdx.x - blocks) * 256u, i0 = at / per;
     const int x = (int)(at - i0 * per) + threadIdx.x, di = x / per, item = x - di * per;
     const int i = (int)i0 + di, g = item / units, pair = (item - g * units) * V, h = hk * G + g;
@@ -400,11 +400,11 @@ hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t s) {
 namespace {
 
 template <bool IN16, int ROT>
-void launch_append_rope(const Kv8RopeArgs& a, bool vec_q, dim3 grid, int blocks, hipStream_t s) {
+void launch_append_rope(const Kv8RopeArgs& a, bool vec_q, dim3 grid, int blocks, int hg, hipStream_t s) {
     auto go = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
-        if (vec_q) hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, ROT>), grid, dim3(256), 0, s, a, blocks);
-        else hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, 1>), grid, dim3(256), 0, s, a, blocks);
+        if (vec_q) hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, ROT>), grid, dim3(256), 0, s, a, blocks, hg);
+        else hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, 1>), grid, dim3(256), 0, s, a, blocks, hg);
     };
     if (a.a.vec) go(std::true_type{});
     else go(std::false_type{});
@@ -416,14 +416,20 @@ hipError_t launch_kv8_append_rope(const Kv8RopeArgs& a, hipStream_t s) {
     const int blocks = (int)(((int64_t)a.a.S + 2 * kKvBlock - 2) / kKvBlock), D = a.a.c.D, rot = rope_granule(a.r, D);
     const bool vec_q = a.vec_q >= rot;
     const int v = vec_q ? rot : 1;
-    const int64_t per = (int64_t)(a.H / a.a.c.Hkv) * (D / (2 * v));
+    // heads of a thread: more where threads enough for 8 waves per SIMD are left
+    const int G = a.q ? a.H / a.a.c.Hkv : 1;
+    const int64_t all = (int64_t)a.a.S * G * (D / (2 * v)) * a.a.c.Hkv * a.a.c.B;
+    int n = 1;
+    while (n < 8 && n < G && all / (2 * n) >= 256 * 2048) n *= 2;
+    const int hg = (G + n - 1) / n;
+    const int64_t per = (int64_t)hg * (D / (2 * v));
     const int64_t wgs = a.q ? ((int64_t)a.a.S * per + 255) / 256 : 0;
     const dim3 grid((unsigned)(blocks + wgs), (unsigned)a.a.c.Hkv, (unsigned)a.a.c.B);
     auto go = [&](auto in16) {
         constexpr bool IN16 = decltype(in16)::value;
-        if (rot == 8) launch_append_rope<IN16, 8>(a, vec_q, grid, blocks, s);
-        else if (rot == 4) launch_append_rope<IN16, 4>(a, vec_q, grid, blocks, s);
-        else launch_append_rope<IN16, 1>(a, vec_q, grid, blocks, s);
+        if (rot == 8) launch_append_rope<IN16, 8>(a, vec_q, grid, blocks, hg, s);
+        else if (rot == 4) launch_append_rope<IN16, 4>(a, vec_q, grid, blocks, hg, s);
+        else launch_append_rope<IN16, 1>(a, vec_q, grid, blocks, hg, s);
     };
     if (a.a.in16) go(std::true_type{});
     else go(std::false_type{});
