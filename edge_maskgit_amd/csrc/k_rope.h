@@ -44,12 +44,13 @@ __device__ __forceinline__ SinCos64 sincos_turns64(uint64_t t) {
     return {q & 2 ? -a : a, (q + 1) & 2 ? -b : b};
 }
 
-// to fp16 with one rounding: to fp32 by way of the neighbour whose last bit is 1 where v is not one of them
+// to fp16 with one rounding: to fp32 by way of the neighbour whose last bit is 1 where v is not one of them (what fp32 rounds
+// to 0 or infinity fp16 does too)
 __device__ __forceinline__ _Float16 half_of(double v) {
     const float f = (float)v;
     const double e = v - (double)f;
     uint32_t u = __builtin_bit_cast(uint32_t, f);
-    if (e != 0. && !(u & 1) && f - f == 0.f) u += (e > 0.) == (f > 0.f) ? 1u : ~0u;
+    if (e != 0. && !(u & 1) && f != 0.f && f - f == 0.f) u += (e > 0.) == (f > 0.f) ? 1u : ~0u;
     return (_Float16)__builtin_bit_cast(float, u);
 }
 

@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a, int HG) {
     const int i = (int)i0 + di, hl = item / units, pair = (item - hl * units) * V;
     Turns<V> f;
     f.load(r, pair);
-    const TokenPos t = token_pos(r, b, min(i, a.S - 1), (a.first ? a.first[b] : 0) + i);
+    const TokenPos t = token_pos(r, b, min(i, a.S - 1), (int32_t)((a.first ? (uint32_t)a.first[b] : 0u) + (uint32_t)i));
     int n = a.S;
     asm volatile("" : "+s"(n));                          // (else loaded by a pointer chosen between the two)
     if (a.fresh) n = a.fresh[b];

@@ -1579,8 +1579,8 @@ int mgh_kv8_attn_shared(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16
     if (R > (1 << 24) || R * kv->Hkv >= ((int64_t)1 << 28))
         return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn_shared: at most 2^24 rows of a key head and 2^28 in all");
     const mgh::Kv8SharedPlan plan = mgh::kv8_shared_plan(a);
-    if ((int64_t)plan.own.tiles * plan.own.splits * kv->Hkv * kv->B >= (1 << 24) ||
-        (int64_t)plan.shared.tiles * plan.shared.splits * kv->Hkv * ((kv->B + a.group - 1) / a.group) >= (1 << 24))
+    if ((int64_t)plan.own.tiles * plan.own.splits * kv->Hkv * kv->B +
+            (int64_t)plan.shared.tiles * plan.shared.splits * kv->Hkv * ((kv->B + a.group - 1) / a.group) >= (1 << 24))
         return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn_shared: shape too large");
     if (int r = set_dev(c)) return r;
     if (int r = ensure_qp_ws(c, plan.ws_bytes)) return r;

@@ -490,8 +490,8 @@ size_t mgh_kv8_tail_bytes(int B, int Hkv, int D);            /* of d_k_tail, and
 /* k, v: {D, S, Hkv, B} views (element strides d, token, head, sequence), fp16 or fp32 (rounded to fp16) */
 int mgh_kv8_append(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_k, const void* d_v, int in_f16,
                    const int64_t strides[4], int S, const int32_t* d_lens, const int32_t* d_new);
-/* mgh_kv8_append with the keys rotated on the way: in fp32, from k as it comes, rounded to fp16 once, into the tails and
- * codes; the same cache as mgh_rope to fp16 followed by mgh_kv8_append. Where d_q is not NULL the queries ({D, S, H, B}, as
+/* mgh_kv8_append with the keys rotated on the way: in fp64 (sine and cosine to 2^-45), from k as it comes, rounded to fp16 once, into
+ * the tails and codes, so that codes are the definition's but for one value in 2^30. Where d_q is not NULL the queries ({D, S, H, B}, as
  * k's type) are rotated to fp16 rows at d_q_out beside it (q itself where types and strides are the same, else apart from
  * it), as mgh_rope. A rotation without positions takes those in the cache, lens[b] + i. Rows past a sequence's new tokens
  * and sequences whose numbers do not fit are left alone in d_q_out too. */
@@ -560,7 +560,8 @@ int mgh_logits_process(mgh_ctx* ctx, const void* d_x, int f16, int64_t x_stride,
  *      above 0: the largest logit, lowest id. A row without a logit above -infinity, or with a NaN: id -1, prob 0 or NaN.
  *      Where infinity is among a row's logits only they weigh. Weights are fp64, counted in 2^-S of the largest
  *      (S = 51, less where V is past 2048: 62 - log2 V), and summed exactly, so ids depend neither on the order of the
- *      sums nor on the other rows. Each part is left out where its pointer is NULL (temperature: 1). V up to 2^24. ---- */
+ *      sums nor on the other rows. Each part is left out where its pointer is NULL (temperature: 1). V up to 2^24, 2^20 rows;
+ *      past 8192 tokens counts are kept in the context's workspace: run a shape once before it is captured. ---- */
 typedef struct mgh_sample_opts {
     const float* d_temp;         /* [rows], as the others */
     const int32_t* d_top_k;

@@ -254,6 +254,7 @@ def test_rotated_append_of_any_size(ctx):
     D, Hkv, pairs = 32, 2, [16]
     f = [1.0, -1.0, 16.0, 1e-4, 2 * np.pi, np.pi / 2, 1e-9, 0.0, 3.7, 0.1, np.pi, 1 / 3, 15.99999, -1e-3, 5.0, 0.7]
     size = 2.0 ** rng.integers(-30, 17, (1, 30, Hkv, D))
+    size[:, 20:] = 2.0 ** rng.integers(-149, -100, (1, 10, Hkv, D))         # (products below fp32's smallest number)
     k = (rng.standard_normal((1, 30, Hkv, D)) * size).astype(F32)
     k[0, 3, 0, 2], k[0, 4, 1, 7], k[0, 5, 0, 31] = np.inf, np.nan, -np.inf
     pos = rng.integers(-2 ** 31, 2 ** 31, (1, 1, 30)).astype(I32)

@@ -112,6 +112,9 @@ for kw, what in (({"H": 3}, "H % Hkv"), ({"scale": float("nan")}, "scale"), ({"c
     refused(call, what=what, **kw)
 call(group=1000)                                    # one group
 assert kernels()
+big = kv(Hkv=2, Bn=65535, nb=4)
+refused(call, big, S=512, what="2^24")
+refused(call, kv(Hkv=256, Bn=65535, nb=4), S=1, H=256, what="too large")
 assert ema.lib().mgh_kv8_attn_shared(None, ctypes.byref(kv()), Q, 1, None, 1, N, None, 1, M, 1, 2, 0.1, 0.0, None, None, O, None) == -1
 """)
 
