@@ -292,8 +292,8 @@ __global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int bloc
     const bool fits = spans(c, a.a.lens, a.a.fresh, a.a.S, b, len, total);
     const TokenPos t = token_pos(a.r, b, min(i, a.a.S - 1), len + i);
     if (!fits || i >= total - len) return;
-    rope_heads<V, IN16, true, (V > 1)>(a.r, t, f, pair, a.q, b * a.qst[3] + i * a.qst[1] + h * a.qst[2], 0, a.qst[0], a.qo,
-                                       b * a.qost[3] + i * a.qost[1] + h * a.qost[2], 0, a.qost[0], 1);
+    rope_heads<V, IN16, true, (V > 1)>(a.r, t, f, pair, a.q, b * a.qst[3] + i * a.qst[1] + h * a.qst[2], HG * a.qst[2], a.qst[0], a.qo,
+                                       b * a.qost[3] + i * a.qost[1] + h * a.qost[2], HG * a.qost[2], a.qost[0], (G - g + HG - 1) / HG);
 }
 
 // Values of tokens [first, first + n) that a sequence has: codes times their scale, or the ring's fp16. One

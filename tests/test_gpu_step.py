@@ -227,6 +227,36 @@ def test_rotated_append_is_rope_and_append(ctx, D, Hkv, G, pairs, order):
                     same_state(c.state(), want.state())
 
 
+# (B, S, Hkv, G, D): threads for 8 waves per SIMD with 2, 4 and 8 heads of each, groups that these do not divide, and few rows
+MANY = [(2, 2100, 8, 4, 128), (1, 2500, 8, 3, 128), (3, 900, 4, 17, 48), (2, 700, 2, 32, 128), (2, 33, 1, 9, 64), (1, 1, 2, 16, 128), (2, 2100, 16, 2, 80)]
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("B,S,Hkv,G,D", MANY)
+def test_rotated_append_turns_every_query_head(ctx, B, S, Hkv, G, D, aligned):
+    """mgh_rope's queries, all of them, where threads take several heads of a group, and nothing past them"""
+    print(f"append heads {B} {S} {Hkv} {G} {D} {aligned}", flush=True)
+    rng = np.random.default_rng(S + G)
+    H, pairs = Hkv * G, [D // 2]
+    f = freqs_of(pairs)
+    q = rng.standard_normal((B, S, H, D)).astype(F16)
+    q[q == 7] = 6
+    k, v = tokens(rng, B, S, Hkv, D)
+    at = np.broadcast_to(np.arange(S, dtype=I32), (1, B, S))
+    w = H * D + (8 if aligned else 1)
+    rows = np.full((B, S, w), 7, F16)
+    rows[..., :H * D] = q.reshape(B, S, H * D)
+    with Dev(ctx) as dev:
+        want = run_rope(ctx, q, at, pairs, f, 0, True)
+        c = Cache(dev, B, Hkv, D, (S + 31) // 32, np.random.default_rng(1))
+        out, st, kst = dev.up(np.full(rows.shape, 7, F16)), (1, w, D, S * w), (1, Hkv * D, D, S * Hkv * D)
+        c.dev.ctx.kv8_append_rope(c.h, ema.Rope(pairs, f, 0), dev.up(k, F16), dev.up(v, F16), kst, S, dev.up(np.zeros(B, I32)), None,
+                                  in16=True, q=dev.up(rows), q_strides=st, H=H, q_out=out, qo_strides=st)
+        got = dev.get(out, rows.shape, F16)
+    assert np.array_equal(got[..., :H * D].reshape(q.shape), want)
+    assert (got[..., H * D:] == 7).all()
+
+
 def test_rotated_append_against_the_definition(ctx):
     """keys rotated in 64 bits and rounded once; codes of whole blocks from exactly the fp16 values that the ring had"""
     rng = np.random.default_rng(3)
