@@ -6,8 +6,10 @@
 // row 4 D flop each and next to no bytes: bound by the VALU that stands beside the matrix products (per 32 rows and 32 keys
 // 64 fma that scale a block's share of the output, 64 issue slots of exponentials, 16 to 32 of each other step).
 //
-// Measured (32 heads on 8 of 128, one launch and the join): 64 sequences on 8000 shared and up to 500 own tokens 38 us (8.6
-// GFLOP, 40 MB; as 64 sequences of 8000 to 8500 without sharing 220), 8 groups of 8 on 2000 to 4000 with capped scores 34.
+// Measured (32 heads on 8 of 128, one launch and the join; in brackets k_kv8_attn on the same tables, which reads the shared
+// blocks from the caches): 64 sequences on 8000 shared and up to 500 own tokens 36 us (105; 8.6 GFLOP, 40 MB), 8 groups of 8 on
+// up to 4000 with capped scores 32 (62), 32 sequences on 32000 52 (191), 16 on 8000 21 (35), 8 on 8000 19 (23). With few sequences
+// there is little to share: 4 on 8000 19 (16.7), 4 drafts of 5 tokens on 1024 the same.
 // Loop of one 128-row tile: 0.93 us a block alone on its CU (370 instructions a wave); before it 6 us of dependent loads
 // (arguments, lengths, pages, codes and queries), after it 3 of partial results (17 MB in all).
 #include <algorithm>

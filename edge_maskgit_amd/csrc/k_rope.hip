@@ -1,7 +1,8 @@
 // k_rope.hip — rotary positions on the heads of queries and keys (gfx950).
 //
 // Bound by its bytes: every feature is read and written once. A thread takes V pairs (two accesses of up to 16 bytes in,
-// two out) of some heads of one token, so their angles are computed once for those heads.
+// two out) of up to 8 heads of one token, so their angles are computed once for those heads. Measured: 2 x 8191 tokens, 40 heads
+// of 128 in fp16, 67.0 us (5.0 TB/s); 3 x 1021, 40 heads of 64 in fp32, 11.4; one image (257 tokens) 6, of which the launch is most.
 #include <algorithm>
 
 #include "k_rope.h"
@@ -57,20 +58,20 @@ int rope_granule(const Rotation& r, int D) {
 RopePlan rope_plan(const RopeArgs& a) {
     RopePlan p{};
     const int g = rope_granule(a.r, a.D);
-    p.v = std::min(std::min(g, a.vec), a.in16 && a.out16 ? 8 : 4);
+    // (8 pairs where both sides are fp16: 2 x 8191 tokens, 40 heads of 128, 71.5 us instead of 67.0)
+    p.v = std::min(std::min(g, a.vec), 4);
     const int64_t units = a.D / (2 * p.v), all = (int64_t)a.B * a.S * units;
-    // heads of a thread: more where threads enough for 8 waves per SIMD are left
+    // heads of a thread: more where threads enough for 2 waves per SIMD are left (for 8 waves 3 x 1021 tokens, 40 heads of 64, take
+    // 11.9 us instead of 11.4; always 8 heads: one image's kernel 5.8 instead of 3.8)
     int n = 1;
-    while (n < 8 && n < a.H && all * a.H / (2 * n) >= 256 * 2048) n *= 2;
+    while (n < 8 && n < a.H && all * a.H / (2 * n) >= 256 * 512) n *= 2;
     p.hg = (a.H + n - 1) / n;
     p.wgs = (a.S * units * p.hg + 255) / 256;
     return p;
 }
 
 hipError_t launch_rope(const RopeArgs& a, const RopePlan& p, hipStream_t s) {
-    // (8 pairs with fp16 on both sides only)
-    if (p.v == 8) hipLaunchKernelGGL((k_rope<8, true, true>), dim3((unsigned)p.wgs, (unsigned)a.B), dim3(256), 0, s, a, p.hg);
-    else if (p.v == 4) launch_rope_v<4>(a, p, s);
+    if (p.v == 4) launch_rope_v<4>(a, p, s);
     else launch_rope_v<1>(a, p, s);
     return hipGetLastError();
 }

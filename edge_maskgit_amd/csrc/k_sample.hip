@@ -12,6 +12,9 @@
 // Which token a sum's border falls on must not depend on how sums are split, so masses are whole numbers of 2^-S of the
 // largest weight, exp2 in 64 bits rounded once: they add up exactly in any order, atomics included. S leaves room for the
 // row (63 bits for its sum) and is at most 51, where the rounding is an addition of 2^52.
+//
+// Measured: one row of 2025 with top-k and top-p 13 us, 1028 rows with min-p 9.4 (0.9 TB/s; the exponentials); 64 rows of 128001
+// 32 us without a cut, 42 with top-k and top-p, 53 with top-p alone; one row of 128001 17, 27 and 32, of a million 17, 44 and 70.
 #include <algorithm>
 
 #include "mgh_common.h"
@@ -707,6 +710,8 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
 template <typename T>
 void launch_short(const SampleArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)a.rows);
+    // (1024 threads for short rows too: one row of 1000 5.9 us instead of 5.3, of 2025 with top-k and top-p 15 instead of 13,
+    // 1028 rows with top-k 45 instead of 16)
     if (a.V <= 2048) hipLaunchKernelGGL((k_sample<T, 256, 8>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_sample<T, 1024, 8>), grid, dim3(1024), 0, s, a);
 }
@@ -738,7 +743,8 @@ double sample_unit(int V) {
     return (double)(1ull << s);
 }
 
-// A row in one workgroup up to 8192 tokens; longer ones in chunks, as many rows at a time as 128 MB of bins and ids hold
+// A row in one workgroup up to 8192 tokens (in chunks instead: one row of 8000 17 us instead of 8, with top-p 27 instead of 18; 64
+// rows 29 instead of 20; 1028 rows 71 instead of 40); longer ones in chunks, as many rows at a time as 128 MB of bins and ids hold
 SamplePlan sample_plan(const SampleArgs& a) {
     SamplePlan p{};
     if (a.V <= kChunk) return p;

@@ -207,7 +207,7 @@ assert call(1, 8, 8, 64, 64, 8, 64, 4, cap=3.0)[0] == call(1, 8, 8, 64, 64, 8, 6
 
 
 def test_which_kernels_rope_takes():
-    """granules of 8, 4 and 1 pairs by order, type and alignment; heads of a thread by the number of rows"""
+    """granules of 4 and 1 pairs by order and alignment; heads of a thread by the number of rows"""
     run(ROPE + """
 def call(pairs, D, order=0, in16=True, out16=True, S=9, H=4, Bn=2, x=W, st=None):
     st = st or (1, H * D, D, S * H * D)
@@ -217,14 +217,13 @@ def call(pairs, D, order=0, in16=True, out16=True, S=9, H=4, Bn=2, x=W, st=None)
     m = re.search(r"k_ropeILi(\\d)ELb(\\d)ELb(\\d)E", n)
     return tuple(map(int, m.groups())), g[:2]
 
-assert call((8,), 16) == ((8, 1, 1), (1, 2))
+assert call((8,), 16) == ((4, 1, 1), (1, 2))
 assert call((8,), 16, in16=False) == ((4, 0, 1), (1, 2)) and call((8,), 16, out16=False)[0] == (4, 1, 0) and call((8,), 16, in16=False, out16=False)[0] == (4, 0, 0)
-assert call((12, 12), 48)[0] == (8, 1, 1) and call((12, 12), 48, order=1)[0] == (8, 1, 1) and call((12, 12), 48, order=2)[0] == (4, 1, 1)
+assert call((12, 12), 48)[0] == (4, 1, 1) and call((12, 12), 48, order=1)[0] == (4, 1, 1) and call((12, 12), 48, order=2)[0] == (4, 1, 1)
 assert call((5,), 16)[0] == (1, 1, 1) and call((4,), 16)[0] == (4, 1, 1) and call((0,), 24)[0] == (4, 1, 1) and call((3,), 6)[0] == (1, 1, 1)
 assert call((8,), 16, x=W + 2)[0] == (1, 1, 1) and call((8,), 16, x=W + 8)[0] == (4, 1, 1) and call((8,), 16, st=(1, 66, 16, 66 * 9))[0] == (1, 1, 1)
-# a thread takes 1 head of few rows, 8 of very many
-assert call((64,), 128, S=100, H=32)[1] == (100 * 32 * 8 // 256, 2)
-assert call((64,), 128, S=65536, H=32)[1] == (65536 * 4 * 8 // 256, 2)
+assert call((64,), 128, S=100, H=32)[1] == (100 * 32 * 16 // 256, 2) and call((64,), 128, S=16, H=9)[1] == (16 * 9 * 16 // 256, 2)
+assert call((64,), 128, S=65536, H=32)[1] == (65536 * 4 * 16 // 256, 2)
 """)
 
 
