@@ -693,6 +693,25 @@ def test_sample_rows_apart_and_without_options(ctx):
                 assert np.array_equal(dev.get(out, 5, I32), run_sample(ctx, x, u)[0])
 
 
+@pytest.mark.parametrize("rows,V", [(400, 128001), (170, 300001)])
+def test_sample_rows_past_one_workspace(ctx, rows, V):
+    """more rows than the workspace holds at a time (371 and 160): each as by itself"""
+    print(f"sample batches {rows} {V}", flush=True)
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((rows, V), dtype=F32) * F32(2)
+    u = rng.random(rows).astype(F32)
+    k, p, T = rng.integers(1, 2000, rows).astype(I32), (rng.random(rows) * 0.9 + 0.1).astype(F32), (0.5 + rng.random(rows)).astype(F32)
+    with Dev(ctx) as dev:
+        dx, du, dk, dp, dt = dev.up(x), dev.up(u), dev.up(k), dev.up(p), dev.up(T)
+        ids, prob = dev.up(np.full(rows, -7, I32)), dev.up(np.full(rows, -7, F32))
+        ctx.sample(dx, rows, V, du, ids, temp=dt, top_k=dk, top_p=dp, prob=prob)
+        got, gp = dev.get(ids, rows, I32), dev.get(prob, rows, F32)
+    for r in sorted({*range(0, rows, 23), 159, 160, rows - 1} | {r for r in (370, 371) if r < rows}):
+        one = run_sample(ctx, x[r:r + 1], u[r:r + 1], top_k=k[r], top_p=p[r], temp=T[r])
+        assert got[r] == one[0][0] and gp[r] == one[1][0], r
+    check_sample(ctx, x[-1:], u[-1:], top_k=k[-1:], top_p=p[-1:], temp=T[-1:])
+
+
 def test_sample_many_rows(ctx):
     """what a row gives does not depend on the others, nor on the call"""
     rng = np.random.default_rng(5)
