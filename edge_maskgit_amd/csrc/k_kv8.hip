@@ -60,9 +60,9 @@ __device__ __forceinline__ void load_row(const void* p, int64_t e, int64_t st, _
 // granules of ROT pairs, whose features lie in two runs; 0: as they come, 16 in a row. In 64 bits: with fp32's 2^-23 one value
 // in 2^12 rounds to the other fp16 number, and one in 2^16 to another code, an error of 1 / 127 of the block's largest, which
 // made half of what all roundings to fp16 together make (2.4e-4 against 2.1e-4 of the values read back).
-template <bool IN16, bool VEC, int ROT>
+template <bool IN16, bool VEC, int ROT, int NT>
 __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotation* r) {
-    __shared__ uint32_t mx[2][4];
+    __shared__ uint32_t mx[2][NT / 64];
     const Kv8& c = a.c;
     if constexpr (ROT != 0)
         asm volatile("" ::"s"(c.k), "s"(c.v), "s"(c.scales), "s"(c.k_tail), "s"(c.v_tail), "s"(c.table), "s"(c.table_stride), "s"(c.pages),
@@ -212,7 +212,7 @@ __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotat
         for (int w = 0; w < 2; w++) {
             uint32_t u = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++) u = u > mx[w][i] ? u : mx[w][i];
+            for (int i = 0; i < NT / 64; i++) u = u > mx[w][i] ? u : mx[w][i];
             const float top = h2f(u), d = top / 127.f, id = u && u < 0x7c00u ? 127.f / top : 0.f;
             if (page < 0 || !has) continue;
             const _Float16* x = w ? xv : xk;
@@ -242,21 +242,21 @@ __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotat
     if (each || blockIdx.x) return;
     __syncthreads();                     // what the ring held has been read
     if constexpr (ROT == 0) {
-        for (int i = tid; i < (total - r0) * (D / 8); i += 256) {
+        for (int i = tid; i < (total - r0) * (D / 8); i += NT) {
             const int t = r0 + i / (D / 8), d = 8 * (i % (D / 8));
             _Float16 x[8];
             load_row<8, IN16, VEC>(a.k, at(t, d), a.st[0], x);
             *(f16x8*)(ring_k + (t % kKvRing) * D + d) = halves(x);
         }
     } else {
-        for (int i = tid; i < (total - r0) * (D / 16); i += 256) {
+        for (int i = tid; i < (total - r0) * (D / 16); i += NT) {
             _Float16 x[16];
             load_new_k(r0 + i / (D / 16), i % (D / 16), x);
             put_ring_k(r0 + i / (D / 16), i % (D / 16), x);
         }
     }
     const int g0 = r0 >> 3, groups = ((total + 7) >> 3) - g0;
-    for (int i = tid; i < groups * (D / 2); i += 256) {
+    for (int i = tid; i < groups * (D / 2); i += NT) {
         const int t = 8 * (g0 + i / (D / 2)), d = 2 * (i % (D / 2));
         _Float16 x[16];
         load_v8(t, d, r0, x);
@@ -266,24 +266,24 @@ __device__ __forceinline__ void append_block(const Kv8AppendArgs& a, const Rotat
 
 template <bool IN16, bool VEC>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8AppendArgs a) {
-    append_block<IN16, VEC, 0>(a, nullptr);
+    append_block<IN16, VEC, 0, 256>(a, nullptr);
 }
 
 // The same with the keys rotated, and workgroups past the first `blocks` of a head and sequence rotating its query heads:
 // V pairs of the heads g, g + HG, ... of one token per thread, so that their angles are computed once.
-template <bool IN16, bool VEC, int ROT, int V>
-__global__ __launch_bounds__(256) void k_kv8_append_rope(Kv8RopeArgs a, int blocks, int HG) {
+template <bool IN16, bool VEC, int ROT, int V, int NT>
+__global__ __launch_bounds__(NT) void k_kv8_append_rope(Kv8RopeArgs a, int blocks, int HG) {
     ask_rotation(a.r);
     asm volatile("" ::"s"(a.a.c.max_blocks), "s"(a.a.c.D), "s"(a.a.c.Hkv), "s"(a.a.lens), "s"(a.a.fresh), "s"(a.a.S));
     if ((int)blockIdx.x < blocks) {
-        append_block<IN16, VEC, ROT>(a.a, &a.r);
+        append_block<IN16, VEC, ROT, NT>(a.a, &a.r);
         return;
     }
     const Kv8& c = a.a.c;
     asm volatile("" ::"s"(a.q), "s"(a.qo), "s"(a.qst[0]), "s"(a.qst[1]), "s"(a.qst[2]), "s"(a.qst[3]), "s"(a.qost[0]), "s"(a.qost[1]),
                  "s"(a.qost[2]), "s"(a.qost[3]), "s"(a.H), "s"(c.Hkv), "s"(c.D));
     const int hk = blockIdx.y, b = blockIdx.z, G = a.H / c.Hkv, units = c.D / (2 * V), per = units * HG;
-    const uint32_t at = (blockIdx.x - blocks) * 256u, i0 = at / per;
+    const uint32_t at = (blockIdx.x - blocks) * (uint32_t)NT, i0 = at / per;
     const int x = (int)(at - i0 * per) + threadIdx.x, di = x / per, item = x - di * per;
     const int i = (int)i0 + di, g = item / units, pair = (item - g * units) * V, h = hk * G + g;
     Turns<V> f;
@@ -399,12 +399,12 @@ hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t s) {
 
 namespace {
 
-template <bool IN16, int ROT>
+template <bool IN16, int ROT, int NT>
 void launch_append_rope(const Kv8RopeArgs& a, bool vec_q, dim3 grid, int blocks, int hg, hipStream_t s) {
     auto go = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
-        if (vec_q) hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, ROT>), grid, dim3(256), 0, s, a, blocks, hg);
-        else hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, 1>), grid, dim3(256), 0, s, a, blocks, hg);
+        if (vec_q) hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, ROT, NT>), grid, dim3(NT), 0, s, a, blocks, hg);
+        else hipLaunchKernelGGL((k_kv8_append_rope<IN16, VEC, ROT, 1, NT>), grid, dim3(NT), 0, s, a, blocks, hg);
     };
     if (a.a.vec) go(std::true_type{});
     else go(std::false_type{});
@@ -421,16 +421,24 @@ hipError_t launch_kv8_append_rope(const Kv8RopeArgs& a, hipStream_t s) {
     // instead of 14.5
     const int G = a.q ? a.H / a.a.c.Hkv : 1, hg = (G + 7) / 8;
     const int64_t per = (int64_t)hg * (D / (2 * v));
-    const int64_t wgs = a.q ? ((int64_t)a.a.S * per + 255) / 256 : 0;
+    // 2 D threads have codes of a block: 128 where that is enough (4 x 1025 tokens, 16 heads of 48 in fp32, read back: 27.9 us, with
+    // 256 threads 31.2; calls of a few tokens the same)
+    const int nt = 2 * D <= 128 ? 128 : 256;
+    const int64_t wgs = a.q ? ((int64_t)a.a.S * per + nt - 1) / nt : 0;
     const dim3 grid((unsigned)(blocks + wgs), (unsigned)a.a.c.Hkv, (unsigned)a.a.c.B);
-    auto go = [&](auto in16) {
+    auto go = [&](auto in16, auto threads) {
         constexpr bool IN16 = decltype(in16)::value;
-        if (rot == 8) launch_append_rope<IN16, 8>(a, vec_q, grid, blocks, hg, s);
-        else if (rot == 4) launch_append_rope<IN16, 4>(a, vec_q, grid, blocks, hg, s);
-        else launch_append_rope<IN16, 1>(a, vec_q, grid, blocks, hg, s);
+        constexpr int NT = decltype(threads)::value;
+        if (rot == 8) launch_append_rope<IN16, 8, NT>(a, vec_q, grid, blocks, hg, s);
+        else if (rot == 4) launch_append_rope<IN16, 4, NT>(a, vec_q, grid, blocks, hg, s);
+        else launch_append_rope<IN16, 1, NT>(a, vec_q, grid, blocks, hg, s);
     };
-    if (a.a.in16) go(std::true_type{});
-    else go(std::false_type{});
+    auto of = [&](auto in16) {
+        if (nt == 128) go(in16, std::integral_constant<int, 128>{});
+        else go(in16, std::integral_constant<int, 256>{});
+    };
+    if (a.a.in16) of(std::true_type{});
+    else of(std::false_type{});
     return hipGetLastError();
 }
 
