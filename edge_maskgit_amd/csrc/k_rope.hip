@@ -59,7 +59,7 @@ RopePlan rope_plan(const RopeArgs& a) {
     RopePlan p{};
     const int g = rope_granule(a.r, a.D);
     // (8 pairs where both sides are fp16: 2 x 8191 tokens, 40 heads of 128, 71.5 us instead of 67.0)
-    p.v = std::min(std::min(g, a.vec), 4);
+    p.v = std::min(g, a.vec) >= 4 ? 4 : 1;
     const int64_t units = a.D / (2 * p.v), all = (int64_t)a.B * a.S * units;
     // heads of a thread: more where threads enough for 2 waves per SIMD are left (for 8 waves 3 x 1021 tokens, 40 heads of 64, take
     // 11.9 us instead of 11.4; always 8 heads: one image's kernel 5.8 instead of 3.8)
@@ -72,7 +72,8 @@ RopePlan rope_plan(const RopeArgs& a) {
 
 hipError_t launch_rope(const RopeArgs& a, const RopePlan& p, hipStream_t s) {
     if (p.v == 4) launch_rope_v<4>(a, p, s);
-    else launch_rope_v<1>(a, p, s);
+    else if (p.v == 1) launch_rope_v<1>(a, p, s);
+    else return hipErrorInvalidValue;                    // (the plan's workgroups are those of v pairs per thread)
     return hipGetLastError();
 }
 

@@ -1279,7 +1279,7 @@ int check_kv8(mgh_ctx* c, const char* fn, const mgh_kv8* kv, mgh::Kv8* out) {
 
 // elements, 8, 4 or 1, at multiples of which the rows start with their features in order, in accesses of up to 16 bytes
 int row_granule(const void* p, const int64_t st[4], bool f16) {
-    for (int n = 8; n > 1; n /= 2)
+    for (int n = 8; n >= 4; n /= 2)
         if (rows_aligned(p, st, n, f16 ? 2 * n : 16)) return n;
     return 1;
 }

@@ -137,6 +137,40 @@ def test_rope_layouts(ctx):
                 assert np.array_equal(dev.get(y, (B, H, S, D), t).transpose(0, 2, 1, 3), want)
 
 
+@pytest.mark.parametrize("B,S,H,D,pairs", [(2, 100, 16, 48, [24]), (1, 1000, 32, 64, [16, 16]), (3, 37, 5, 32, [4, 8])])
+@pytest.mark.parametrize("t", [F16, F32])
+def test_rope_rows_of_every_alignment(ctx, B, S, H, D, pairs, t):
+    """rows, heads and pointers at multiples of one, two, three, four and six elements, of x, of y and in place: what contiguous
+    rows give, every token of it, and nothing beside it"""
+    print(f"rope alignment {B} {S} {H} {D} {pairs} {t.__name__}", flush=True)
+    rng = np.random.default_rng(D)
+    f, n, e = freqs_of(pairs), H * D, np.dtype(t).itemsize
+    x = rng.standard_normal((B, S, H, D)).astype(t)
+    x[x == 9] = 8
+    pos = positions(rng, len(pairs), B, S)
+    out = "y16" if t == F16 else "y"
+    for order in (0, 1, 2):
+        want = run_rope(ctx, x, pos, pairs, f, order, t == F16)
+        with Dev(ctx) as dev:
+            rot = ema.Rope(pairs, f, order, dev.up(pos), (1, S, B * S))
+            dx, st = dev.up(x), (1, n, D, S * n)
+            for pad, gap, off in ((2, 0, 0), (6, 0, 0), (0, 2, 0), (0, 6, 0), (0, 0, 2), (0, 0, 6), (2, 2, 2), (0, 0, 4), (0, 0, 1), (1, 0, 0), (3, 3, 3), (4, 4, 0), (8, 8, 8)):
+                w = H * (D + gap) + pad                             # rows of heads D + gap apart, from element `off` on
+                rows = np.full(off + B * S * w, 9, t)
+                rows[off:].reshape(B, S, w)[..., :H * (D + gap)].reshape(B, S, H, D + gap)[..., :D] = x
+                there = np.zeros(rows.shape, bool)
+                there[off:].reshape(B, S, w)[..., :H * (D + gap)].reshape(B, S, H, D + gap)[..., :D] = True
+                wide = (1, w, D + gap, S * w)
+                d, y, z = dev.up(rows), dev.up(np.full(x.shape, 9, t)), dev.up(np.full(rows.shape, 9, t))
+                ctx.rope(rot, d.ptr + e * off, wide, D, S, H, B, in16=t == F16, y_strides=st, **{out: y})
+                ctx.rope(rot, dx, st, D, S, H, B, in16=t == F16, y_strides=wide, **{out: z.ptr + e * off})
+                ctx.rope(rot, d.ptr + e * off, wide, D, S, H, B, in16=t == F16, **{out: d.ptr + e * off})
+                assert np.array_equal(dev.get(y, x.shape, t), want), (order, pad, gap, off)
+                for b in (z, d):
+                    got = dev.get(b, rows.shape, t)
+                    assert np.array_equal(got[there], want.ravel()) and (got[~there] == 9).all(), (order, pad, gap, off)
+
+
 def test_rope_of_anything(ctx):
     """infinities and NaN stay within their pair"""
     x = np.ones((1, 4, 1, 16), F32)

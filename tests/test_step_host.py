@@ -227,6 +227,36 @@ assert call((64,), 128, S=65536, H=32)[1] == (65536 * 4 * 16 // 256, 2)
 """)
 
 
+def test_rope_covers_rows_of_every_alignment():
+    """threads for all pairs of all heads of all tokens, whatever the rows' and pointers' alignment, of x or y: one, two, four or
+    eight elements, with one head of each thread and with several"""
+    run(ROPE + """
+def call(p, D, S, H, x=W, wx=0, y=Y, wy=0, head=0, seq=0, **kw):
+    launches()
+    w = H * (D + head)
+    out = {"y16" if kw.pop("out16", True) else "y": y}
+    c.rope(rot((p,)), x, (1, w + wx, D + head, S * (w + wx) + seq), D, S, H, 2, y_strides=(1, H * D + wy, D, S * (H * D + wy)), **out, **kw)
+    (k, n, g), = launches()
+    v = int(re.search(r"k_ropeILi(\\d)E", n).group(1))
+    return v, g[:2]
+
+for p, D, S, H in ((24, 48, 100, 16), (32, 64, 1000, 32), (8, 16, 9, 4), (12, 48, 33, 5), (0, 32, 70, 3)):
+    def needs(v):                                       # heads of a thread: up to 8 while 2^17 threads are left
+        n = 1
+        while n < 8 and n < H and 2 * S * (D // 2 // v) * H // (2 * n) >= 256 * 512:
+            n *= 2
+        return v, (-(-S * (D // 2 // v) * -(-H // n) // 256), 2)
+    at = lambda **kw: call(p, D, S, H, **kw)  # noqa: E731
+    for wide, v in ((0, 4), (1, 1), (2, 1), (3, 1), (4, 4), (6, 1), (8, 4), (10, 1), (12, 4)):
+        got = [at(wx=wide), at(wy=wide), at(seq=wide), at(wx=wide, in16=False), at(wy=wide, out16=False), at(head=wide), at(wx=wide, in16=False, out16=False)]
+        assert got == [needs(v)] * 7, (wide, got, needs(v))
+    for b, v in ((2, 1), (4, 1), (6, 1), (8, 4), (10, 1), (12, 1), (16, 4)):
+        assert at(x=W + b) == at(y=Y + b) == needs(v), (b, at(x=W + b), at(y=Y + b), needs(v))
+    for b in (4, 8, 12):
+        assert at(x=W + b, in16=False) == at(y=Y + b, out16=False) == needs(1), b
+""")
+
+
 def test_which_kernels_sampling_takes():
     """rows up to 2048 and 8192 tokens in one workgroup, longer ones in chunks of 8192, rows by rows of 128 MB"""
     run(BODY + """
