@@ -33,10 +33,11 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 2^t, t <= 0, off by 2^-51 of it and 2^-53 |t|: the nearest whole number's power and the series of the rest, |f| <= 1/2, by
-// pairs of terms (Horner's rule is a chain of 13 dependent steps: a row of 2025 tokens 16.5 us with it)
-__device__ __forceinline__ double exp2_64(double t) {
-    const double n = rint(fmax(t, -1100.)), f = t - n, f2 = f * f, f4 = f2 * f2;
+// 2^t, t = d c <= 0, off by 2^-51 of it and 2^-53 |t|: the nearest whole number's power and the series of the rest, |f| <= 1/2, by
+// pairs of terms (Horner's rule is a chain of 13 dependent steps: a row of 2025 tokens 16.5 us with it). Every fused step
+// is written out: kernels that must agree on a token's mass to the last bit do not leave it to the compiler
+__device__ __forceinline__ double exp2_64(double d, double c) {
+    const double t = d * c, n = rint(fmax(t, -1100.)), f = fma(d, c, -n), f2 = f * f, f4 = f2 * f2;
     const double p0 = fma(0.6931471805599453, f, 1.), p1 = fma(0.055504108664821576, f, 0.2402265069591007);
     const double p2 = fma(0.0013333558146428441, f, 0.009618129107628477), p3 = fma(1.5252733804059838e-05, f, 0.00015403530393381606);
     const double p4 = fma(1.0178086009239696e-07, f, 1.3215486790144305e-06), p5 = fma(4.44553827187081e-10, f, 7.054911620801121e-09);
@@ -50,7 +51,7 @@ struct Weights {
     double unit;           // 2^S
     // weight of a logit relative to the largest one's
     __device__ __forceinline__ double of(float l) const {
-        const double w = exp2_64(((double)l - m) * c);
+        const double w = exp2_64((double)l - m, c);
         // (whatever T is; infinities among themselves)
         return (double)l == m ? 1. : l == -INFINITY || m == INFINITY ? 0. : w;
     }
@@ -100,6 +101,8 @@ struct Ask {
     float temp, top_p, min_p, u;
     int k;
     bool greedy, by_k, by_p;
+    // whether min-p leaves a token of this weight in
+    __device__ __forceinline__ bool likely(double w) const { return !(min_p > 0.f) || w >= fmin((double)min_p, 1.); }
 };
 __device__ __forceinline__ Ask ask_of(const SampleArgs& a, int64_t row) {
     Ask q;
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < U; j++) {
             const double w = sc.wt.of(l[j]);
-            mass[j0 + j] = keep[j] && (!(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.)) ? sc.wt.mass(w) : 0;
+            mass[j0 + j] = keep[j] && q.likely(w) ? sc.wt.mass(w) : 0;
         }
     }
     const uint64_t all = wave_sums<NV>(s, mass);
@@ -552,7 +555,7 @@ __global__ __launch_bounds__(512, 4) void k_sample_bins(SampleArgs a, Long g) {
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const double w = sc.wt.of(l[j]);
-        mass[j] = !(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.) ? sc.wt.mass(w) : 0;
+        mass[j] = q.likely(w) ? sc.wt.mass(w) : 0;
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
     const uint64_t all = wave_sums<NV>(s, mass);
@@ -603,11 +606,10 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
     }
     const Scale sc(m, lo, q.temp, a.unit);
     uint64_t last = ~0ull;
-    if (q.min_p > 0.f) {
-        const double p = fmin((double)q.min_p, 1.);
-        last = (uint64_t)~least_key(key_of(m), [&](float y) { return sc.wt.of(y) >= p; }) << 32 | 0xffffffffull;
-    }
-    if (q.by_k || q.by_p) {
+    const bool cut = q.by_k || q.by_p;
+    if (cut) {
+        if (q.min_p > 0.f)
+            last = (uint64_t)~least_key(key_of(m), [&](float y) { return q.likely(sc.wt.of(y)); }) << 32 | 0xffffffffull;
         auto fill = [&] {                // the row's bins: two halves of the chunks
             const int b = tid & (kBins - 1), half = tid / kBins;
             uint32_t n = 0;
@@ -697,11 +699,14 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
     const int id0 = (int)s.found[0] * kChunk;
     const uint64_t ahead = s.found[1];
     load_chunk<T, NT>(x, V, id0, l);
+    // Without a cut by the comparison that the chunk's mass was kept by and not by a place: weights within 2^-51 of min-p need not
+    // fall with the logits, and a draw past what the tokens of this chunk add up to would be none of them
     uint64_t mass[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = id0 + first + 64 * j;
-        mass[j] = i < V && place_of(l[j], i) <= last ? sc.mass(l[j]) : 0;
+        const double w = sc.wt.of(l[j]);
+        mass[j] = i < V && (cut ? place_of(l[j], i) <= last : q.likely(w)) ? sc.wt.mass(w) : 0;
     }
     wave_sums<NV>(s, mass);
     draw<NV>(s, mass, ahead, all, at, id0, out);

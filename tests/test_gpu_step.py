@@ -713,6 +713,36 @@ def test_sample_special_values(ctx, V):
     assert ids[:2].tolist() == [-1, -1] and prob[0] == 0 and np.isnan(prob[1]) and ids[2] == 7 and ids[8] == V // 2
 
 
+# min-p, largest logit, temperature, and two logits next to each other's weight: in 64 bits the lower one weighs min-p and the
+# higher one 2^-53 less (computed weights are within 2^-51 of theirs, and do not all fall with the logits)
+MIN_P_BORDERS = [("0x1.a3f7ccp-1", "0x1.7816bep+0", "0x1.da825ep+2", "0x1.87e6cp-34", "0x1.87e78p-34"),
+                 ("0x1.8689d2p-1", "0x1.57fd6ap+0", "0x1.3d91fp+2", "0x1.ac008p-34", "0x1.ac01p-34"),
+                 ("0x1.7797fcp-1", "0x1.05c666p+0", "0x1.a677b2p+1", "-0x1.8ba8p-35", "-0x1.8ba78p-35")]
+
+
+@pytest.mark.parametrize("V", [300, 5000, 8193, 40000])
+@pytest.mark.parametrize("border", MIN_P_BORDERS)
+def test_sample_weights_that_are_min_p(ctx, V, border):
+    """tokens whose weight is min-p to the last bit are all kept or all left out, and one of what is kept is drawn"""
+    print(f"sample min-p {V} {border[0]}", flush=True)
+    p, m, T, low, high = (F32(float.fromhex(t)) for t in border)
+    u = np.array([0, 0.1234, 0.37, 0.5617, 0.777, 0.9123, 0.98765, 0.99999], F32)
+    for kind in range(3):
+        x = np.full((1, V), (low, high, low)[kind], F32)
+        if kind == 2:
+            x[0, ::2] = high
+        x[0, 5] = m
+        ids, prob = run_sample(ctx, x, u, one_row=True, temp=T, min_p=p)
+        w = np.exp((x[0].astype(F64) - F64(m)) / F64(T))
+        sets = [np.arange(V) == 5, np.ones(V, bool), x[0] != high, x[0] != low]         # of which one is kept
+        fits = []
+        for keep in sets:
+            run = np.cumsum(w * keep)
+            at = np.searchsorted(run, u.astype(F64) * run[-1], side="right")
+            fits.append(np.array_equal(ids, at) and np.allclose(prob, w[at] / run[-1], rtol=1e-6))
+        assert any(fits), (kind, ids, prob)
+
+
 def test_sample_rows_apart_and_without_options(ctx):
     rng = np.random.default_rng(4)
     for V, pad in ((1001, 23), (30000, 1)):
