@@ -1,6 +1,10 @@
 """The host side of rotary positions, rotated appending, attention over shared blocks and sampling without a GPU: what
 each call refuses, that a refused or empty call launches nothing, and which kernels the others take, on the recording HIP
 runtime of tests/test_dispatch.py."""
+import os
+import struct
+
+import msgpack
 import numpy as np
 import pytest
 
@@ -278,3 +282,30 @@ try:
 finally:
     c.graph_end().destroy()
 """)
+
+
+def device_kernels():
+    """{name: metadata} of the built library's kernels: the note of each device code object in its bundles"""
+    with open(os.path.join(os.path.dirname(ema.__file__), "lib", "libmgh.so"), "rb") as f:
+        data = f.read()
+    magic, found, at = b"__CLANG_OFFLOAD_BUNDLE__", {}, 0
+    while (at := data.find(magic, at)) >= 0:
+        entry = at + len(magic) + 8
+        for _ in range(struct.unpack_from("<Q", data, at + len(magic))[0]):
+            off, size, n = struct.unpack_from("<QQQ", data, entry)
+            if size and b"gfx950" in data[entry + 24:entry + 24 + n]:
+                obj = data[at + off:at + off + size]
+                note = obj.find(b"AMDGPU\0\0")
+                notes = struct.unpack_from("<III", obj, note - 12)
+                for k in msgpack.unpackb(obj[note + 8:note + 8 + notes[1]])["amdhsa.kernels"]:
+                    found[k[".name"]] = k
+            entry += 24 + n
+        at += len(magic)
+    return found
+
+
+def test_cache_attention_keeps_its_registers():
+    """no kernel of the cache's attention has scratch memory (a register spilled across its loop cost 3% of capped calls)"""
+    attn = {n: k for n, k in device_kernels().items() if "k_kv8_attn" in n}
+    assert len(attn) == 32 + 48
+    assert [n for n, k in attn.items() if k[".private_segment_fixed_size"]] == []
