@@ -1576,8 +1576,8 @@ int mgh_kv8_attn_shared(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16
     if (!aligned_to(shared, 4)) return fail(c, MGH_ERR_ARG, "kv8_attn_shared: pointers must be aligned to their elements");
     a.shared = shared; a.group = std::min(group, kv->B); a.max_shared = max_shared;
     const int64_t G = H / kv->Hkv, R = (int64_t)kv->B * S * G;
-    if (R > (1 << 24) || R * kv->Hkv >= ((int64_t)1 << 28))
-        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn_shared: at most 2^24 rows of a key head and 2^28 in all");
+    if (R > (1 << 24) || R * kv->Hkv >= ((int64_t)1 << 27))             // (the join: 32 threads per row)
+        return fail(c, MGH_ERR_UNSUPPORTED, "kv8_attn_shared: at most 2^24 rows of a key head and fewer than 2^27 in all");
     const mgh::Kv8SharedPlan plan = mgh::kv8_shared_plan(a);
     if ((int64_t)plan.own.tiles * plan.own.splits * kv->Hkv * kv->B +
             (int64_t)plan.shared.tiles * plan.shared.splits * kv->Hkv * ((kv->B + a.group - 1) / a.group) >= (1 << 24))
@@ -1585,7 +1585,7 @@ int mgh_kv8_attn_shared(mgh_ctx* c, const mgh_kv8* kv, const void* q, int in_f16
     if (int r = set_dev(c)) return r;
     if (int r = ensure_qp_ws(c, plan.ws_bytes)) return r;
     a.ws = (float*)c->qp_ws;
-    MGH_HIP(c, mgh::launch_kv8_attn_shared(a, plan, c->stream), "k_kv8_attn_part");
+    MGH_HIP(c, mgh::launch_kv8_attn_shared(a, plan, c->stream), "k_kv8_attn_shared");
     return MGH_OK;
 }
 

@@ -123,6 +123,22 @@ assert ema.lib().mgh_kv8_attn_shared(None, ctypes.byref(kv()), Q, 1, None, 1, N,
 """)
 
 
+def test_shared_attention_refuses_what_its_join_cannot_launch():
+    """the join takes 32 threads per row: rows up to 2^27 - 1, refused before anything is launched; fewer run"""
+    run(BODY + """
+Q, O, N, M = (0x100000 * i for i in (17, 18, 19, 20))
+def call(Bn, S=1024, Hkv=16, D=16):
+    c.kv8_attn_shared(ema.Kv8(W, X, B, R, Y, G, 4, 9, Hkv, D, Bn), Q, (1, D, D, D), S, N, None, 64, M, 3, Hkv, 0.1, o16=O)
+launches()
+refused(call, 8192, what="2^27")
+refused(call, 16383, what="2^27")
+assert launches() == []
+call(8191)
+g = {k: n for k, _, n in launches()}
+assert [n[0] * 256 < 2 ** 32 for n in g.values()] == [True, True] and g["k_attn_join_few"][0] * 8 >= 8191 * 2 ** 14
+""")
+
+
 def test_sample_refusals():
     run(BODY + """
 def call(x=W, rows=3, V=1000, u=X, ids=Y, **kw):
