@@ -433,7 +433,8 @@ __global__ __launch_bounds__(NT) void k_sample(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < U; j++) {
             const double w = sc.wt.of(l[j]);
-            mass[j0 + j] = keep[j] && q.likely(w) ? sc.wt.mass(w) : 0;
+            // (likely(w), written out: by a call of it a row of 2025 takes 14.0 us instead of 13.0)
+            mass[j0 + j] = keep[j] && (!(q.min_p > 0.f) || w >= fmin((double)q.min_p, 1.)) ? sc.wt.mass(w) : 0;
         }
     }
     const uint64_t all = wave_sums<NV>(s, mass);
@@ -700,13 +701,21 @@ __global__ __launch_bounds__(1024) void k_sample_pick(SampleArgs a, Long g) {
     const uint64_t ahead = s.found[1];
     load_chunk<T, NT>(x, V, id0, l);
     // Without a cut by the comparison that the chunk's mass was kept by and not by a place: weights within 2^-51 of min-p need not
-    // fall with the logits, and a draw past what the tokens of this chunk add up to would be none of them
+    // fall with the logits, and a draw past what the tokens of this chunk add up to would be none of them. (Loops of their own:
+    // one that takes each token's weight and then either test 44.9 us instead of 42.8, 64 rows of 128001 with top-k and top-p)
     uint64_t mass[NV];
+    if (cut) {
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int i = id0 + first + 64 * j;
-        const double w = sc.wt.of(l[j]);
-        mass[j] = i < V && (cut ? place_of(l[j], i) <= last : q.likely(w)) ? sc.wt.mass(w) : 0;
+        for (int j = 0; j < NV; j++) {
+            const int i = id0 + first + 64 * j;
+            mass[j] = i < V && place_of(l[j], i) <= last ? sc.mass(l[j]) : 0;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const double w = sc.wt.of(l[j]);
+            mass[j] = id0 + first + 64 * j < V && q.likely(w) ? sc.wt.mass(w) : 0;
+        }
     }
     wave_sums<NV>(s, mass);
     draw<NV>(s, mass, ahead, all, at, id0, out);
