@@ -17,8 +17,8 @@
 // where scores lie farther apart than the reference's distance), and all rows of a part with a page outside the pool, are
 // taken again by attn_row.
 //
-// Measured (32 heads on 8 of 128): one sequence of 100000 tokens, 205 MB, 39.5 us (5.2 TB/s) and the join 4.8; 64 of 2700
-// tokens 69 us (5.2 TB/s), of up to 8000 with capped scores 90 (4.1 TB/s: long sequences' parts at the end). A block takes
+// Measured (32 heads on 8 of 128, two sets of inputs in turn): one sequence of 100000 tokens, 205 MB, 39.4 us (5.2 TB/s) and the join
+// 4.8; 64 of 2700 tokens 67 us (5.3 TB/s), of up to 8000 with capped scores 91 (4.0 TB/s: long sequences' parts at the end). A block takes
 // a wave 0.88 us, so short sequences are latency: 4 of 1030, 16 heads of 48, five rows: 7.3 us and the join 2.8.
 #include <algorithm>
 

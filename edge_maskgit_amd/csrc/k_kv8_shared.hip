@@ -7,11 +7,11 @@
 // 64 fma that scale a block's share of the output, 64 issue slots of exponentials, 16 to 32 of each other step).
 //
 // Measured (32 heads on 8 of 128, one launch and the join; in brackets k_kv8_attn on the same tables, which reads the shared
-// blocks from the caches): 64 sequences on 8000 shared and up to 500 own tokens 36 us (105; 8.6 GFLOP, 40 MB), 8 groups of 8 on
-// up to 4000 with capped scores 32 (62), 32 sequences on 32000 52 (191), 16 on 8000 21 (35), 8 on 8000 19 (23). With few sequences
-// there is little to share: 4 on 8000 19 (16.7), 4 drafts of 5 tokens on 1024 the same.
-// Loop of one 128-row tile: 0.93 us a block alone on its CU (370 instructions a wave); before it 6 us of dependent loads
-// (arguments, lengths, pages, codes and queries), after it 3 of partial results (17 MB in all).
+// blocks from the caches): 64 sequences on 8000 shared and up to 500 own tokens 37 us (108; 8.6 GFLOP, 40 MB), 8 groups of 8 on
+// up to 4000 with capped scores 31 (58), 32 sequences on 32000 52 (191), 16 on 8000 21 (34), 8 on 8000 18 (22). With few sequences
+// there is little to share: 4 on 8000 18 (16), 4 drafts of 5 tokens on 1024 10.4 (9.7). With fp32 outputs 38, 34, 57, 22, 20, 20 and 10.7.
+// Loop of one 128-row tile: 1.16 us a block beside the own blocks' workgroups (some 400 instructions a wave); before it 4.8 us of
+// dependent loads (arguments, lengths, pages, codes and queries), after it 2 of partial results (17 MB in all).
 #include <algorithm>
 
 #include "k_kv8_attn.h"
@@ -249,7 +249,7 @@ void launch_shared(const Kv8AttnArgs& a, const Kv8SharedPlan& p, hipStream_t s) 
 Kv8SharedPlan kv8_shared_plan(const Kv8AttnArgs& a) {
     Kv8SharedPlan p{};
     const int64_t G = a.H / a.c.Hkv, sets = (a.c.B + a.group - 1) / a.group;
-    // each sequence's own blocks: as a cache of the blocks that are left, in tiles of 16 rows
+    // each sequence's own blocks: as a cache of the blocks that are left, its parts cut as for kv8_plan's tiles, but in tiles of 16 rows
     Kv8AttnArgs own = a;
     own.c.max_blocks = a.c.max_blocks - std::min(a.max_shared, a.c.max_blocks);
     p.own = kv8_plan(own);

@@ -3,7 +3,7 @@
 // (a, b) -> (a cos t - b sin t, a sin t + b cos t), t = f p. Angles are kept in turns of 2^-64: the frequency as a whole
 // number F = 2^64 f / 2 pi (mod 2^64), so that p F mod 2^64 is the angle with its whole turns gone and no rounding,
 // however far the position; its highest 32 bits are used (off by less than 2^-32 turns and what F's rounding gives,
-// |p| 2^-64 each). The remainder within an eighth of a turn of the nearest quarter goes through odd and even polynomials
+// |p| 2^-65). The remainder within an eighth of a turn of the nearest quarter goes through odd and even polynomials
 // (least largest error, 2^-28 of the sine and 2^-33), fp32 throughout.
 #pragma once
 #include "mgh_common.h"
@@ -25,6 +25,7 @@ __device__ __forceinline__ SinCos sincos_turns(uint32_t t) {
 }
 
 // The same in 64 bits, for values whose rounding decides about a code: sine and cosine of t 2^-64 turns to 2^-45, by their series
+// (t itself is off by F's rounding, as above: 2^-45 turns at positions of 2^20, 2^-34 at 2^31)
 struct SinCos64 {
     double s, c;
 };

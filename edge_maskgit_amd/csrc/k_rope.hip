@@ -2,7 +2,8 @@
 //
 // Bound by its bytes: every feature is read and written once. A thread takes V pairs (two accesses of up to 16 bytes in,
 // two out) of up to 8 heads of one token, so their angles are computed once for those heads. Measured: 2 x 8191 tokens, 40 heads
-// of 128 in fp16, 67.0 us (5.0 TB/s); 3 x 1021, 40 heads of 64 in fp32, 11.4; one image (257 tokens) 6, of which the launch is most.
+// of 128 in fp16, 67.0 us (5.0 TB/s); 3 x 1021, 40 heads of 64 in fp32, 11.4; one image (257 tokens) 6, of which the launch is most. Rows, heads or
+// pointers that are not at multiples of 4 elements go feature by feature, one pair per thread: the first of these 90.6 us.
 #include <algorithm>
 
 #include "k_rope.h"

@@ -13,8 +13,9 @@
 // largest weight, exp2 in 64 bits rounded once: they add up exactly in any order, atomics included. S leaves room for the
 // row (63 bits for its sum) and is at most 51, where the rounding is an addition of 2^52.
 //
-// Measured: one row of 2025 with top-k and top-p 13 us, 1028 rows with min-p 9.4 (0.9 TB/s; the exponentials); 64 rows of 128001
-// 32 us without a cut, 42 with top-k and top-p, 53 with top-p alone; one row of 128001 17, 27 and 32, of a million 17, 44 and 70.
+// Measured: one row of 2025 with top-k and top-p 13 us, 1028 rows with min-p 9.7 (0.9 TB/s; the exponentials); 64 rows of 128001
+// 33 us without a cut or with min-p, 43 with top-k and top-p, 55 with top-p alone; one row of 128001 17, 27 and 32, of a million 17,
+// 44 and 70.
 #include <algorithm>
 
 #include "mgh_common.h"

@@ -427,9 +427,9 @@ int mgh_attn_masked(mgh_ctx* ctx, const void* d_q, const void* d_k, const void* 
  *      stay as they are. Axis a has the next pairs[a] pairs (index; row and column; time, row and column; ...).
  *      d_pos: whole positions (any sign) of token i of sequence b on axis a at a pos_strides[2] + b pos_strides[1] +
  *      i pos_strides[0]; NULL: consecutive ones on every axis, from where the call says. h_freqs is read when the call is
- *      made, angles per unit of position in radians, finite, up to 16 in magnitude. An angle is exact to 2^-32 turns however
- *      far the position (up to 2^31), its sine and cosine to 2^-23, products and sums are fp32, rounded once to an fp16 output.
- *      D even up to 128, P up to D / 2. ---- */
+ *      made, angles per unit of position in radians, finite, up to 16 in magnitude. An angle is off by less than
+ *      2^-32 + |p| 2^-65 turns (2^-32 + 2^-34 at the farthest position, 2^31), its sine and cosine by 2^-23, products and sums
+ *      are fp32, rounded once to an fp16 output. D even up to 128, P up to D / 2. ---- */
 enum { MGH_ROPE_HALVES = 0, MGH_ROPE_PAIRS = 1, MGH_ROPE_AXIS_HALVES = 2 };
 typedef struct mgh_rotation {
     int axes;                    /* 1 .. 4 */
@@ -490,8 +490,9 @@ size_t mgh_kv8_tail_bytes(int B, int Hkv, int D);            /* of d_k_tail, and
 /* k, v: {D, S, Hkv, B} views (element strides d, token, head, sequence), fp16 or fp32 (rounded to fp16) */
 int mgh_kv8_append(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_k, const void* d_v, int in_f16,
                    const int64_t strides[4], int S, const int32_t* d_lens, const int32_t* d_new);
-/* mgh_kv8_append with the keys rotated on the way: in fp64 (sine and cosine to 2^-45), from k as it comes, rounded to fp16 once, into
- * the tails and codes, so that codes are the definition's but for one value in 2^30. Where d_q is not NULL the queries ({D, S, H, B}, as
+/* mgh_kv8_append with the keys rotated on the way: in fp64 (sine and cosine to 2^-45, of an angle that is off by |p| 2^-65 turns),
+ * from k as it comes, rounded to fp16 once, into the tails and codes, so that codes are the definition's but for one value
+ * in 2^30 at positions up to 2^20, and past them in proportion (one in 2^20 at the farthest, 2^31). Where d_q is not NULL the queries ({D, S, H, B}, as
  * k's type) are rotated to fp16 rows at d_q_out beside it (q itself where types and strides are the same, else apart from
  * it), as mgh_rope. A rotation without positions takes those in the cache, lens[b] + i. Rows past a sequence's new tokens
  * and sequences whose numbers do not fit are left alone in d_q_out too. */
@@ -513,8 +514,8 @@ int mgh_kv8_attn(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_q, int in_f16
  * a group (the last one may have fewer), and d_shared[g] blocks of group g, 0 .. max_shared, are read from the first of its
  * sequences' rows of the table once for all of them (the other rows' entries for these blocks are not read). Each of
  * its sequences must be at least that long (lens[b] >= 32 shared): one that is shorter gives NaN rows, as do all of a
- * group whose number does not fit. The result is mgh_kv8_attn's but for the last bits. Partial results are
- * kept in the context's workspace: run a shape once before it is captured. */
+ * group whose number does not fit. The result is mgh_kv8_attn's but for the last bits. B S H / Hkv up to 2^24 and
+ * B S H below 2^27. Partial results are kept in the context's workspace: run a shape once before it is captured. */
 int mgh_kv8_attn_shared(mgh_ctx* ctx, const mgh_kv8* cache, const void* d_q, int in_f16, const int64_t q_strides[4], int S,
                         const int32_t* d_lens, const int32_t* d_new, int group, const int32_t* d_shared, int max_shared, int H,
                         float scale, float cap, const float* d_slopes, float* d_o, void* d_o16, const int64_t o_strides[4]);
