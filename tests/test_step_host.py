@@ -302,6 +302,7 @@ finally:
 
 def device_kernels():
     """{name: metadata} of the built library's kernels: the note of each device code object in its bundles"""
+    ema.lib()
     with open(os.path.join(os.path.dirname(ema.__file__), "lib", "libmgh.so"), "rb") as f:
         data = f.read()
     magic, found, at = b"__CLANG_OFFLOAD_BUNDLE__", {}, 0
